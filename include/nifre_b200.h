@@ -400,6 +400,124 @@ int nf_cascade_limits(int32_t dtype, int32_t num_q_heads, int32_t num_kv_heads, 
                       int32_t* max_rows, int32_t* max_keys);
 
 /*
+ * Attention over part of a sequence's cached keys: the last `window` keys
+ * and the first `sinks` keys (nf_window_attention), or the cached context
+ * and the drafted tokens that a bit mask names (nf_tree_attention).  These
+ * operators have no counterpart in the reference, whose attention is always
+ * causal over the whole sequence (attention.py:144-152).
+ *
+ * A query token at absolute position p sees key k when
+ *   window:  k <= p and (k > p - window or k < sinks),
+ *   tree:    k < ctx, or bit k - ctx of the token's mask row is set,
+ * and its output is sum_k softmax_k(q . k * scale) v_k over the keys it sees,
+ * 0 when it sees none.  A key that a token does not see contributes nothing
+ * to it, whatever its rows hold (NaN and infinities included).  Query head j
+ * reads KV head j / (num_q_heads / num_kv_heads); every dtype, head_dim up to
+ * 256, any block size and group size.
+ *
+ * Work lists (device, 16-byte aligned, built by the host once per step and
+ * used by every layer):
+ *   groups[max_groups][8]: slot, q_row0, ntok, pos0, ctx, n_draft, mask0,
+ *     part_row0 -- ntok consecutive query tokens of one sequence, whose rows
+ *     of q and out start at q_row0 and whose absolute positions start at
+ *     pos0.  Tree: ctx cached keys before n_draft drafted ones; the mask rows
+ *     of the group's tokens (ceil(n_draft / 32) words each) start at word
+ *     mask0 of `masks`.  Rows outside [0, num_rows) are neither read nor
+ *     written.
+ *   units[max_units][4]: group, key_begin, key_end, part | n_parts << 16 -- a
+ *     part of the group's keys, counted without the gap that a window leaves:
+ *     with lo = max(0, pos0 - window + 1) rounded down to a multiple of 16 and
+ *     kept = min(sinks rounded up to a multiple of 16, lo), key v is key v of
+ *     the sequence for v < kept and key v + lo - kept from there on; key_begin
+ *     is a multiple of 16.  A group's n_parts units cover its keys once.  At
+ *     most nf_masked_limits' unit_rows query rows (ntok x heads of a KV head)
+ *     a group, at most unit_tokens tokens.
+ *   items[max_items][4]: the same for groups of up to item_rows query rows,
+ *     which the tensor cores take (none where item_rows is 0); key_begin a
+ *     multiple of 128.
+ *   merge[max_merge][4]: q_row, part_row, n_parts, step -- a token whose keys
+ *     are several units: its partial rows part_row + j * step (j < n_parts)
+ *     are merged into row q_row of out.  Unit j of a group writes the partial
+ *     row part_row0 + j * ntok + i for token i.
+ *   counts[4]: units, items, merge rows in use, 0.
+ * Workspace: ws, ws_rows partial rows of num_q_heads records of head_dim
+ * rounded up to a multiple of 4, plus 4, floats; queue: int32[4], zero when
+ * allocated, left zero by every call (calls that share it or ws must not
+ * overlap).  Bad records are skipped and flagged in *status.  Up to three
+ * launches, in stream order.
+ */
+typedef struct NfMaskedArgs {
+  void* out;
+  int64_t out_row_stride;
+  const void* q;
+  int64_t q_row_stride;
+  const void* k_pool;
+  const void* v_pool;
+  const int32_t* block_tables;
+  const int32_t* groups;
+  const int32_t* units;
+  const int32_t* items;
+  const int32_t* merge;
+  const int32_t* counts;
+  const uint32_t* masks;
+  int64_t mask_words;
+  float* ws;
+  int64_t ws_rows;
+  int32_t* queue;
+  int32_t* status;
+  int32_t dtype, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks;
+  int32_t num_slots, max_blocks_per_seq, num_rows;
+  int32_t max_groups, max_units, unit_tokens, max_items, max_merge;
+  int32_t window, sinks;
+  float scale;
+  int32_t pad;
+} NfMaskedArgs;
+
+int nf_window_attention(const NfMaskedArgs* args, void* stream);
+int nf_tree_attention(const NfMaskedArgs* args, void* stream);
+
+/*
+ * nf_masked_limits: the largest groups of this shape, in query rows (tokens
+ * x query heads per KV head): those of units, and those of the tensor cores'
+ * items (0: this shape has none).
+ */
+int nf_masked_limits(int32_t dtype, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                     int32_t* unit_rows, int32_t* item_rows);
+
+/*
+ * nf_kv_move: copies of cache rows within the pools, in every layer, K and V
+ * (copying and forking blocks, keeping an accepted path of drafted tokens,
+ * compacting a pool; no counterpart in the reference).  Layer l's pools start
+ * l * layer_stride bytes after k_pool and v_pool; a row is row_bytes bytes (a
+ * multiple of 2: one token's heads, or a whole block), pool_rows rows a layer.
+ * moves[n_moves][4]: source row, destination row, rows, continues -- `rows`
+ * consecutive rows (at most max_rows).  A record whose last field is not 0
+ * continues the run of the record before it: a run's rows are copied one
+ * after another, in order, so that a row may move onto one that the run has
+ * read already (never onto one that it reads later).  Records that are not
+ * of one run must not touch one another's destinations.  If pos_out
+ * (int64 [num_slots]) is not NULL, pos_out[slot] = value for the n_pos
+ * records pos[n_pos][2] (slot, value).  Rows or slots out of range are
+ * skipped and flagged (NF_STATUS_BAD_SLOT).  on_device 0: the lists are host
+ * memory, at most NF_MOVE_LIST records each, and are read before the call
+ * returns; else device memory (16- and 8-byte aligned).
+ */
+#define NF_MOVE_LIST 128
+int nf_kv_move(void* k_pool, void* v_pool, int64_t layer_stride, int32_t num_layers, int64_t row_bytes,
+               int64_t pool_rows, const int32_t* moves, int32_t n_moves, int32_t max_rows, const int32_t* pos,
+               int32_t n_pos, int64_t* pos_out, int32_t num_slots, int32_t on_device, int32_t* status, void* stream);
+
+/*
+ * nf_copy_blocks: blocks src[i] -> dst[i] (device int32, n each) of every
+ * layer's K and V pool; layer_stride as for nf_kv_move, block_bytes a multiple
+ * of 2.  Destinations must be distinct and no sources.  Ids out of range are
+ * skipped and flagged (NF_STATUS_BAD_BLOCK).
+ */
+int nf_copy_blocks(void* k_pool, void* v_pool, int64_t layer_stride, int32_t num_layers, int64_t block_bytes,
+                   int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t n, int32_t* status,
+                   void* stream);
+
+/*
  * nf_prefill_attention: causal attention of prefill chunks on the tensor
  * cores (tcgen05, tensor memory), for 16-bit pools with head_dim 64 or 128,
  * 1, 2, 4 or 8 query heads per KV head and block_size a multiple of 16.

@@ -11,6 +11,7 @@ from nifre_b200.attention import Attention, causal_attention
 from nifre_b200.block_allocator import BlockAllocator, BlockPoolExhaustedError
 from nifre_b200.block_table import BlockTable
 from nifre_b200.kv_cache import KVCache
+from nifre_b200.masked import MaskedPlan, tree_visibility
 from nifre_b200.paged_kv_cache import PagedKVCache, StepPlan
 from nifre_b200.data_model import (EngineConfig, InferenceRequest, ModelConfig, RequestState, ScheduleResult,
                                    validate_engine_config)
@@ -21,6 +22,6 @@ from nifre_b200.prefix_cache import PrefixCache
 from nifre_b200.scheduler import Scheduler
 
 __all__ = ["Attention", "BlockAllocator", "BlockPoolExhaustedError", "BlockTable", "Engine", "EngineConfig",
-           "GPT_CONFIG_124M", "GptInferenceModel", "GptModel", "InferenceRequest", "KVCache", "ModelConfig",
+           "GPT_CONFIG_124M", "GptInferenceModel", "GptModel", "InferenceRequest", "KVCache", "MaskedPlan", "ModelConfig",
            "ModelRunner", "PagedKVCache", "PrefixCache", "RequestState", "ScheduleResult", "Scheduler", "StepPlan",
-           "causal_attention", "validate_engine_config"]
+           "causal_attention", "tree_visibility", "validate_engine_config"]

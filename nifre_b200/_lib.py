@@ -32,7 +32,8 @@ EXPORTS = ("nf_last_error", "nf_abi_version", "nf_pack_step", "nf_kv_append",
            "nf_last_attention_path", "nf_selftest_umma", "nf_prefill_attention", "nf_prefill_tile_rows",
            "nf_cascade_attention", "nf_selftest_wait", "nf_noalloc_scratch_fill", "nf_paged_attention_gather",
            "nf_prefill_attention_gather", "nf_exchange_barrier", "nf_ipc_handle", "nf_ipc_open", "nf_ipc_close", "nf_qkv_append",
-           "nf_paged_attention_args", "nf_kv_append_args", "nf_cascade_limits")
+           "nf_paged_attention_args", "nf_kv_append_args", "nf_cascade_limits", "nf_window_attention", "nf_tree_attention",
+           "nf_masked_limits", "nf_kv_move", "nf_copy_blocks")
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -74,6 +75,25 @@ class NfAppendArgs(ctypes.Structure):
                 ("n_seqs", ctypes.c_int32), ("slot_mapping", ctypes.c_void_p), ("src_rows", ctypes.c_void_p),
                 ("seqs", ctypes.c_void_p), ("pos_out", ctypes.c_void_p), ("status", ctypes.c_void_p)]
 
+
+class NfMaskedArgs(ctypes.Structure):
+    """struct NfMaskedArgs of include/nifre_b200.h (the arguments of nf_window_attention and nf_tree_attention)."""
+    _fields_ = [("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64), ("q", ctypes.c_void_p),
+                ("q_row_stride", ctypes.c_int64), ("k_pool", ctypes.c_void_p), ("v_pool", ctypes.c_void_p),
+                ("block_tables", ctypes.c_void_p), ("groups", ctypes.c_void_p), ("units", ctypes.c_void_p),
+                ("items", ctypes.c_void_p), ("merge", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+                ("masks", ctypes.c_void_p), ("mask_words", ctypes.c_int64), ("ws", ctypes.c_void_p),
+                ("ws_rows", ctypes.c_int64), ("queue", ctypes.c_void_p), ("status", ctypes.c_void_p),
+                ("dtype", ctypes.c_int32), ("num_q_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("block_size", ctypes.c_int32), ("num_blocks", ctypes.c_int32),
+                ("num_slots", ctypes.c_int32), ("max_blocks_per_seq", ctypes.c_int32), ("num_rows", ctypes.c_int32),
+                ("max_groups", ctypes.c_int32), ("max_units", ctypes.c_int32), ("unit_tokens", ctypes.c_int32),
+                ("max_items", ctypes.c_int32), ("max_merge", ctypes.c_int32), ("window", ctypes.c_int32),
+                ("sinks", ctypes.c_int32), ("scale", ctypes.c_float), ("pad", ctypes.c_int32)]
+
+
+MOVE_LIST = 128  # NF_MOVE_LIST: nf_kv_move records that travel as kernel arguments
+
 _SIGNATURES = {
     "nf_last_error": ([], ctypes.c_char_p),
     "nf_abi_version": ([], ctypes.c_int),
@@ -106,6 +126,11 @@ _SIGNATURES = {
     "nf_kv_append_args": ([_P, _P], ctypes.c_int),
     "nf_qkv_append": ([_P, _I64, _I32, _P, _P, _I32, _I32, _I32, _P, _I64, _P, _P, _I64, _I32, _P, _P, _I32, _P,
                        _P, _P], ctypes.c_int),
+    "nf_window_attention": ([_P, _P], ctypes.c_int),
+    "nf_tree_attention": ([_P, _P], ctypes.c_int),
+    "nf_masked_limits": ([_I32, _I32, _I32, _I32, _I32, ctypes.POINTER(_I32), ctypes.POINTER(_I32)], ctypes.c_int),
+    "nf_kv_move": ([_P, _P, _I64, _I32, _I64, _I64, _P, _I32, _I32, _P, _I32, _P, _I32, _I32, _P, _P], ctypes.c_int),
+    "nf_copy_blocks": ([_P, _P, _I64, _I32, _I64, _I32, _P, _P, _I32, _P, _P], ctypes.c_int),
     "nf_ipc_handle": ([_P, _P, ctypes.POINTER(_I64)], ctypes.c_int),
     "nf_ipc_open": ([_P, _I64, ctypes.POINTER(_P)], ctypes.c_int),
     "nf_ipc_close": ([_P, _I64], ctypes.c_int),

@@ -35,8 +35,16 @@ from nifre_b200.paged_kv_cache import PagedKVCache
 
 
 class Attention(nn.Module):
-    def __init__(self, num_heads, head_dim, layer_id=None, dropout=0.0):
+    def __init__(self, num_heads, head_dim, layer_id=None, dropout=0.0, window=None, sinks=0):
+        """``window`` (no counterpart in the reference): each query sees the last ``window`` keys, its own included,
+        and the first ``sinks`` keys of its sequence, instead of all of them (a cache is then required)."""
         super().__init__()
+        if window is None and sinks:
+            raise ValueError("sinks need a window")
+        if window is not None and (int(window) != window or window <= 0 or int(sinks) != sinks or sinks < 0):
+            raise ValueError(f"window ({window}) must be a positive whole number and sinks ({sinks}) at least 0")
+        self.window = window
+        self.sinks = sinks
         self.num_heads = num_heads
         self.head_dim = head_dim
         self.d_out = num_heads * head_dim
@@ -46,6 +54,8 @@ class Attention(nn.Module):
     def forward(self, q, k, v, kv_cache=None, layer_id=None, input_lens=None, cache_batch_indices=None):
         lid = layer_id if layer_id is not None else self.layer_id
         if kv_cache is None:
+            if self.window is not None:
+                raise ValueError("windowed attention needs a kv_cache")
             return self._forward_full_causal(q, k, v)
         if lid is None:
             raise ValueError("layer_id is required when kv_cache is set")
@@ -95,6 +105,17 @@ class Attention(nn.Module):
         qk = q2 if q2.stride(1) == 1 else q2.contiguous()
         # padding rows of a left-padded prefill stay zero (attention.py:79); without padding every row is written
         ex = cache.exchange
+        if self.window is not None:
+            if ex is not None:
+                raise ValueError("windowed attention does not gather its output over a sharded cache (exchange set)")
+            view = plan.views.get((self.window, self.sinks, self.num_heads))
+            if view is None:  # the step's first layer with this window
+                view = cache.plan_window(plan, self.window, self.sinks, q_heads=self.num_heads)
+                plan.views[(self.window, self.sinks, self.num_heads)] = view
+            out = (torch.zeros if padded else torch.empty)((B * T, q.shape[-1]), dtype=cache.dtype, device=q.device)
+            cache.append_step(layer_id, k2, v2, plan)
+            cache.window_attention_step(layer_id, qk, view, out)
+            return out.view(B, T, -1)
         if ex is not None:
             # KV heads sharded over the ranks of a PeerExchange: the kernels write this rank's heads into every
             # rank's gathered buffer; the result is the gathered output of all heads

@@ -97,6 +97,39 @@ class BlockAllocator:
             self._top += 1
             self._allocated -= 1
 
+    def retain_many(self, block_ids) -> None:
+        """One more reference to each of the distinct blocks."""
+        ids = self._live_ids(block_ids)
+        self._refcount[ids] += 1
+
+    def release_many(self, block_ids) -> None:
+        """One reference less to each of the distinct blocks; those without any are free, in the order given."""
+        ids = self._live_ids(block_ids)
+        self._refcount[ids] -= 1
+        freed = ids[self._refcount[ids] == 0]
+        self._stack[self._top: self._top + len(freed)] = freed
+        self._top += len(freed)
+        self._allocated -= len(freed)
+
+    def _live_ids(self, block_ids) -> np.ndarray:
+        ids = np.asarray(block_ids, dtype=np.int64).reshape(-1)
+        if len(ids) and (ids.min() < 0 or ids.max() >= self._num_blocks):
+            raise ValueError(f"block_id out of range [0, {self._num_blocks})")
+        if (self._refcount[ids] <= 0).any():
+            raise ValueError("a block is not allocated")
+        return ids
+
+    def compact(self) -> tuple[list[int], list[int]]:
+        """Give the live blocks the ids 0 .. allocated_count - 1: (old ids, new ids) of the blocks that move, old and
+        new distinct.  The free ids are handed out in ascending order afterwards."""
+        n = self._allocated
+        src = n + np.flatnonzero(self._refcount[n:] > 0)
+        dst = np.flatnonzero(self._refcount[:n] == 0)
+        self._refcount[dst] = self._refcount[src]
+        self._refcount[src] = 0
+        self._stack[: self._top] = np.arange(self._num_blocks - 1, n - 1, -1)
+        return src.tolist(), dst.tolist()
+
     def refcount(self, block_id: int) -> int:
         self._validate_block_id(block_id)
         return int(self._refcount[block_id])

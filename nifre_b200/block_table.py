@@ -50,7 +50,7 @@ class BlockTable:
 
     def resolve(self, token_index: int) -> tuple[int, int]:
         logical = token_index // self._block_size
-        if logical >= len(self._physical_blocks):
+        if logical >= len(self._physical_blocks) or self._physical_blocks[logical] < 0:
             raise IndexError(f"token_index {token_index} has no allocated block")
         return self._physical_blocks[logical], token_index % self._block_size
 
@@ -62,6 +62,38 @@ class BlockTable:
 
     def clear(self) -> None:
         if self._physical_blocks:
-            self._allocator.free_many(self._physical_blocks)
+            self._allocator.free_many([b for b in self._physical_blocks if b >= 0])
             self._physical_blocks.clear()
         self.epoch += 1
+
+    # Operators without a counterpart in the reference.  An entry of -1 is a
+    # block that was freed behind the sequence's window.
+
+    def share(self, physical_blocks: list[int]) -> None:
+        """Hold another table's blocks too (an empty table; freed entries stay freed)."""
+        if self._physical_blocks:
+            raise ValueError("cannot share blocks with a non-empty block table")
+        self._allocator.retain_many([b for b in physical_blocks if b >= 0])
+        self._physical_blocks = list(physical_blocks)
+        self.epoch += 1
+
+    def shrink(self, n_blocks: int) -> None:
+        """Release every block from entry ``n_blocks`` on."""
+        dropped = self._physical_blocks[n_blocks:]
+        if dropped:
+            self._allocator.release_many([b for b in dropped if b >= 0])
+            del self._physical_blocks[n_blocks:]
+            self.epoch += 1
+
+    def free_blocks(self, first: int, end: int) -> int:
+        """Release the blocks of entries first .. end-1, which stay in the table as -1; returns how many there were."""
+        held = [b for b in self._physical_blocks[first:end] if b >= 0]
+        self._allocator.release_many(held)
+        self._physical_blocks[first:end] = [-1] * len(self._physical_blocks[first:end])
+        return len(held)
+
+    def rename(self, to) -> None:
+        """Replace every block id b by ``to[b]``."""
+        if self._physical_blocks:
+            self._physical_blocks = to[self._physical_blocks].tolist()
+            self.epoch += 1

@@ -1,0 +1,465 @@
+// Windowed and tree attention: the per-warp kernel for every type and shape,
+// the merge of split-K parts and the entry points.  See nf_masked.cuh for the
+// operators' definition and the work records.
+#include "nf_internal.h"
+#include "nf_masked.cuh"
+
+namespace nf {
+
+// Columns (token, query head of the KV head) that one warp task carries.
+constexpr int kVecCols = 4;
+// Query rows of a per-warp group (at least one token).
+constexpr int kVecRows = 16;
+constexpr int kVecWarps = 4;
+
+template <typename T, int VW> struct VecLoad;
+template <> struct VecLoad<float, 4> {
+  static __device__ __forceinline__ void load(const float* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  }
+};
+template <typename H> struct VecLoad<H, 8> {
+  static __device__ __forceinline__ void load(const H* p, float (&x)[8]) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const H* h = reinterpret_cast<const H*>(&v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = Elem<H>::to_f(h[i]);
+  }
+};
+template <typename H> struct VecLoad<H, 1> {
+  static __device__ __forceinline__ void load(const H* p, float (&x)[1]) { x[0] = Elem<H>::to_f(*p); }
+};
+
+// One warp computes C columns of one (unit, KV head): LPK lanes hold a key's
+// row (VW elements a load, EV loads), so 32 / LPK keys are worked on at once,
+// each lane group with its own running maximum, sum and output; they are
+// joined by shuffles at the end.  Bound by the key and value bytes (each
+// column chunk of a group reads them again, from L2 where there are several)
+// and, for short key ranges, by the latency of the dependent loads.
+template <typename T, int VW, int LPK, int EV, int C>
+__global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const MaskedParams p) {
+  constexpr int KPW = 32 / LPK;  // keys per step of the warp
+  constexpr int U = EV * VW >= 8 ? 2 : 4;  // steps in flight
+  constexpr int E = EV * VW;
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, li = lane % LPK, lg = lane / LPK;
+  const int n_units = min(__ldg(p.counts), p.max_units);
+  pdl_wait();
+  const T* q = reinterpret_cast<const T*>(p.q);
+  const T* kp = reinterpret_cast<const T*>(p.kp);
+  const T* vp = reinterpret_cast<const T*>(p.vp);
+  const long long row_elems = (long long)p.Hkv * p.D;
+  const int chunks = (p.unit_tokens * p.G + C - 1) / C;  // of the largest group; a smaller one's last tasks are empty
+  const long long tasks = (long long)n_units * p.Hkv * chunks;
+  for (long long task = (long long)blockIdx.x * kVecWarps + (threadIdx.x >> 5); task < tasks;
+       task += (long long)gridDim.x * kVecWarps) {
+    const int u = (int)(task / (p.Hkv * chunks)), rest = (int)(task - (long long)u * p.Hkv * chunks);
+    const int kvh = rest / chunks, c0 = (rest - kvh * chunks) * C;
+    const int4 un = __ldg(reinterpret_cast<const int4*>(p.units) + u);
+    if (un.x < 0 || un.x >= p.max_groups) {
+      if (lane == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
+      continue;
+    }
+    const MaskedGroup g = load_group(p, un.x);
+    if (!group_ok(p, g)) {
+      if (lane == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
+      continue;
+    }
+    const int cols = g.ntok * p.G;
+    if (c0 >= cols) continue;
+    const VirtualKeys vk(p, g);
+    const int* btrow = p.bt + (long long)g.slot * p.max_blocks;
+    const int v1 = min(un.z, vk.end);
+    float qr[C][E];
+    int tok[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = min(c0 + c, cols - 1);
+      tok[c] = col / p.G;
+      const T* qrow = q + (long long)(g.q_row0 + tok[c]) * p.q_stride +
+                      (long long)(kvh * p.G + (col - tok[c] * p.G)) * p.D;
+#pragma unroll
+      for (int v = 0; v < EV; ++v) {
+        const int e = (v * LPK + li) * VW;
+        float x[VW];
+#pragma unroll
+        for (int i = 0; i < VW; ++i) x[i] = 0.f;
+        if (e < p.D) {
+          // queries may start at any element of their row's allocation: element loads
+#pragma unroll
+          for (int i = 0; i < VW; ++i) x[i] = Elem<T>::to_f(qrow[e + i]);
+        }
+#pragma unroll
+        for (int i = 0; i < VW; ++i) qr[c][v * VW + i] = x[i] * p.scale_log2;
+      }
+    }
+    float m[C], l[C], acc[C][E];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      m[c] = -INFINITY;
+      l[c] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[c][e] = 0.f;
+    }
+    for (int v0 = un.y; v0 < v1; v0 += KPW * U) {
+      float kx[U][E], vx[U][E];
+      int key[U];
+      // every load of the U steps first
+#pragma unroll
+      for (int s = 0; s < U; ++s) {
+        const int v = v0 + s * KPW + lg;
+        key[s] = v < v1 ? vk.key(v) : -1;
+        const long long row = key[s] >= 0 ? key_row(p, btrow, key[s]) : -1;
+        if (row < 0) key[s] = -1;
+#pragma unroll
+        for (int w = 0; w < EV; ++w) {
+          const int e = (w * LPK + li) * VW;
+          float a[VW], b[VW];
+#pragma unroll
+          for (int i = 0; i < VW; ++i) a[i] = b[i] = 0.f;
+          if (row >= 0 && e < p.D) {
+            const long long off = row * row_elems + (long long)kvh * p.D + e;
+            VecLoad<T, VW>::load(kp + off, a);
+            VecLoad<T, VW>::load(vp + off, b);
+          }
+#pragma unroll
+          for (int i = 0; i < VW; ++i) {
+            kx[s][w * VW + i] = a[i];
+            vx[s][w * VW + i] = b[i];
+          }
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float x[U];
+        unsigned vis = 0;  // keys of this column: the others are left out, whatever their value rows hold
+        float mn = m[c];
+#pragma unroll
+        for (int s = 0; s < U; ++s) {
+          float d = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) d = fmaf(qr[c][e], kx[s][e], d);
+#pragma unroll
+          for (int o = LPK / 2; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+          if (key[s] >= 0 && sees(p, g, tok[c], key[s])) {
+            vis |= 1u << s;
+            mn = fmaxf(mn, d);
+          }
+          x[s] = d;
+        }
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float al = ex2(m[c] - base);
+        m[c] = mn;
+        l[c] *= al;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[c][e] *= al;
+#pragma unroll
+        for (int s = 0; s < U; ++s) {
+          if (vis >> s & 1u) {
+            const float w = ex2(x[s] - base);
+            l[c] += w;
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[c][e] = fmaf(w, vx[s][e], acc[c][e]);
+          }
+        }
+      }
+    }
+    // join the lane groups
+    const int part = un.w & 0xffff, n_parts = un.w >> 16;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int o = LPK; o < 32; o <<= 1) {
+        const float mo = __shfl_xor_sync(0xffffffffu, m[c], o), lo = __shfl_xor_sync(0xffffffffu, l[c], o);
+        const float mn = fmaxf(m[c], mo), base = mn == -INFINITY ? 0.f : mn;
+        const float a = ex2(m[c] - base), b = ex2(mo - base);
+        l[c] = l[c] * a + lo * b;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          acc[c][e] = acc[c][e] * a + __shfl_xor_sync(0xffffffffu, acc[c][e], o) * b;
+        m[c] = mn;
+      }
+      const int col = c0 + c;
+      if (col >= cols || lg != 0) continue;
+      const int head = kvh * p.G + (col - tok[c] * p.G);
+      if (n_parts == 1) {
+        const float inv = l[c] > 0.f ? 1.f / l[c] : (l[c] == 0.f ? 0.f : l[c]);
+        T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok[c]) * p.out_stride + (long long)head * p.D;
+#pragma unroll
+        for (int v = 0; v < EV; ++v) {
+          const int e = (v * LPK + li) * VW;
+          if (e < p.D)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) dst[e + i] = Elem<T>::from_f(acc[c][v * VW + i] * inv);
+        }
+      } else {
+        const long long prow = (long long)g.part_row0 + (long long)part * g.ntok + tok[c];
+        if (g.part_row0 < 0 || prow >= p.ws_rows) {
+          if (li == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
+          continue;
+        }
+        float* rec = part_record(p, prow, head);
+#pragma unroll
+        for (int v = 0; v < EV; ++v) {
+          const int e = (v * LPK + li) * VW;
+          if (e < p.D)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) rec[e + i] = acc[c][v * VW + i];
+        }
+        if (li == 0) {
+          rec[p.DP - 4] = m[c];
+          rec[p.DP - 3] = l[c];
+        }
+      }
+    }
+  }
+}
+
+// Merge of split-K parts: one warp per (query row, head): out = sum_j
+// 2^(m_j - M) acc_j / sum_j 2^(m_j - M) l_j, always in the order of the parts.
+// The maxima and sums of up to 32 parts come in one load, a lane each; their
+// weights are then broadcast while the accumulators stream in.
+template <typename T>
+__global__ void __launch_bounds__(256) masked_merge_kernel(const MaskedParams p) {
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const int n = min(__ldg(p.counts + 2), p.max_merge);
+  pdl_wait();
+  const long long tasks = (long long)n * p.Hq;
+  for (long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); task < tasks; task += (long long)gridDim.x * 8) {
+    const int r = (int)(task / p.Hq), head = (int)(task - (long long)r * p.Hq);
+    const int4 mr = __ldg(reinterpret_cast<const int4*>(p.merge) + r);
+    const long long last = mr.y + (long long)(mr.z - 1) * mr.w;
+    if (mr.x < 0 || mr.x >= p.rows || mr.y < 0 || mr.z <= 0 || mr.w <= 0 || last >= p.ws_rows) {
+      if (lane == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
+      continue;
+    }
+    const float* rec = part_record(p, mr.y, head);
+    const long long step = (long long)mr.w * p.Hq * p.DP;  // between consecutive parts
+    // the row's maximum, then its sum and weights
+    float M = -INFINITY;
+    for (int j = lane; j < mr.z; j += 32) M = fmaxf(M, __ldcg(rec + j * step + p.DP - 4));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = 0.f;
+    const int D2 = (p.D + 63) >> 6;  // pairs of elements a lane holds
+    for (int j0 = 0; j0 < mr.z; j0 += 32) {
+      float w = 0.f, lw = 0.f;
+      if (j0 + lane < mr.z) {
+        const float mj = __ldcg(rec + (j0 + lane) * step + p.DP - 4);
+        w = mj == -INFINITY ? 0.f : ex2(mj - base);
+        lw = w * __ldcg(rec + (j0 + lane) * step + p.DP - 3);
+        if (mj == -INFINITY) lw = 0.f;
+      }
+      // in the order of the parts, the same whatever the launch
+      const int jn = min(32, mr.z - j0);
+      for (int j = 0; j < jn; j += 4) {
+        float x[4][8], wj[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          wj[u] = j + u < jn ? __shfl_sync(0xffffffffu, w, j + u) : 0.f;
+          L += j + u < jn ? __shfl_sync(0xffffffffu, lw, j + u) : 0.f;
+          const float* pj = rec + (long long)(j0 + j + u) * step;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int e = (i * 32 + lane) * 2;  // (records are padded to whole pairs)
+            const bool in = i < D2 && e < p.D && j + u < jn && wj[u] != 0.f;
+            const float2 v = in ? __ldcg(reinterpret_cast<const float2*>(pj + e)) : make_float2(0.f, 0.f);
+            x[u][2 * i] = v.x;
+            x[u][2 * i + 1] = v.y;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) a[i] = fmaf(wj[u], x[u][i], a[i]);
+      }
+    }
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    T* dst = reinterpret_cast<T*>(p.out) + (long long)mr.x * p.out_stride + (long long)head * p.D;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int e = (i * 32 + lane) * 2;
+      if (e < p.D) dst[e] = Elem<T>::from_f(a[2 * i] * inv);
+      if (e + 1 < p.D) dst[e + 1] = Elem<T>::from_f(a[2 * i + 1] * inv);
+    }
+  }
+}
+
+// Launch with programmatic stream serialization (the kernel waits for the
+// one before it ahead of its first read of what that writes).
+template <typename K>
+static int launch_masked(K kern, long long blocks, int threads, cudaStream_t st, const MaskedParams& p,
+                         const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(blocks < 1 ? 1 : blocks));
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+  if (e != cudaSuccess) return fail(NF_ECUDA, "%s: launch: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+template <typename T, int VW, int LPK, int EV>
+static int launch_vec(const MaskedParams& p, cudaStream_t st, const char* what) {
+  // one column per warp task where no group has more (decodes of a model without grouped heads), else four
+  const bool one = p.unit_tokens * p.G == 1;
+  const int C = one ? 1 : kVecCols;
+  const long long chunks = (p.unit_tokens * p.G + C - 1) / C;
+  long long blocks = ((long long)p.max_units * p.Hkv * chunks + kVecWarps - 1) / kVecWarps;
+  const long long cap = (long long)sm_count() * 8;
+  if (blocks > cap) blocks = cap;
+  return one ? launch_masked(masked_vec_kernel<T, VW, LPK, EV, 1>, blocks, kVecWarps * 32, st, p, what)
+             : launch_masked(masked_vec_kernel<T, VW, LPK, EV, kVecCols>, blocks, kVecWarps * 32, st, p, what);
+}
+
+template <typename T>
+static int dispatch_vec(const MaskedParams& p, cudaStream_t st, const char* what) {
+  constexpr int VW = sizeof(T) == 4 ? 4 : 8;
+  const bool vec = p.D % VW == 0 &&
+                   ((reinterpret_cast<uintptr_t>(p.kp) | reinterpret_cast<uintptr_t>(p.vp)) & 15) == 0;
+  if (!vec) return launch_vec<T, 1, 32, 8>(p, st, what);
+  const int n = p.D / VW;
+  if (n <= 8) return launch_vec<T, VW, 8, 1>(p, st, what);
+  if (n <= 16) return launch_vec<T, VW, 16, 1>(p, st, what);
+  if (n <= 32) return launch_vec<T, VW, 32, 1>(p, st, what);
+  if constexpr (sizeof(T) == 4) return launch_vec<T, VW, 32, 2>(p, st, what);
+  return fail(NF_EUNSUPPORTED, "%s: head_dim %d > 256", what, p.D);
+}
+
+constexpr int kMaskedMaxHeads = 1 << 12;
+
+static int masked_check(const NfMaskedArgs* a, bool tree, const char* what, MaskedParams& p) {
+  if (!a) return fail(NF_EINVAL, "%s: null argument struct", what);
+  const size_t es = dtype_size(a->dtype);
+  if (!es) return fail(NF_EINVAL, "%s: bad dtype %d", what, a->dtype);
+  if (a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->num_q_heads % a->num_kv_heads ||
+      a->num_q_heads > kMaskedMaxHeads)
+    return fail(NF_EINVAL, "%s: num_q_heads (%d) must be a positive multiple of num_kv_heads (%d), at most %d", what,
+                a->num_q_heads, a->num_kv_heads, kMaskedMaxHeads);
+  if (a->head_dim <= 0 || a->head_dim > 256)
+    return fail(NF_EUNSUPPORTED, "%s: head_dim %d (1 to 256)", what, a->head_dim);
+  if (a->block_size <= 0 || a->num_blocks <= 0 || a->max_blocks_per_seq <= 0 || a->num_slots <= 0 || a->num_rows <= 0)
+    return fail(NF_EINVAL, "%s: sizes must be positive", what);
+  if (a->max_groups <= 0 || a->max_units < 0 || a->max_items < 0 || a->max_merge < 0 || a->ws_rows < 0 ||
+      a->max_units + (int64_t)a->max_items <= 0)
+    return fail(NF_EINVAL, "%s: work list sizes must not be negative, and not all zero", what);
+  if (a->max_units && (a->unit_tokens <= 0 || (int64_t)a->unit_tokens * a->num_q_heads > (1 << 20)))
+    return fail(NF_EINVAL, "%s: unit_tokens (%d) must be positive, and at most 2^20 / num_q_heads", what, a->unit_tokens);
+  if (!a->out || !a->q || !a->k_pool || !a->v_pool || !a->block_tables || !a->groups || !a->counts || !a->queue ||
+      !a->status || (a->max_units && !a->units) || (a->max_items && !a->items) || (a->max_merge && !a->merge) ||
+      (a->ws_rows && !a->ws))
+    return fail(NF_EINVAL, "%s: null pointer argument", what);
+  if (a->q_row_stride < 0 || a->out_row_stride < 0) return fail(NF_EINVAL, "%s: negative row stride", what);
+  if (tree && (!a->masks || a->mask_words <= 0)) return fail(NF_EINVAL, "%s: null mask words", what);
+  if (!tree && (a->window <= 0 || a->sinks < 0))
+    return fail(NF_EINVAL, "%s: window (%d) must be positive and sinks (%d) not negative", what, a->window, a->sinks);
+  auto al = [](const void* ptr, size_t n) { return (reinterpret_cast<uintptr_t>(ptr) % n) == 0; };
+  if (!al(a->groups, 16) || !al(a->units, 16) || !al(a->items, 16) || !al(a->merge, 16) || !al(a->ws, 16) ||
+      !al(a->masks, 4) || !al(a->counts, 4))
+    return fail(NF_EINVAL, "%s: work lists and workspace must be 16-byte aligned", what);
+  if (!al(a->q, es) || !al(a->out, es) || !al(a->k_pool, es) || !al(a->v_pool, es))
+    return fail(NF_EINVAL, "%s: tensors must be aligned to their elements", what);
+  p = MaskedParams{};
+  p.out = static_cast<char*>(a->out);
+  p.out_stride = a->out_row_stride;
+  p.q = static_cast<const char*>(a->q);
+  p.q_stride = a->q_row_stride;
+  p.kp = static_cast<const char*>(a->k_pool);
+  p.vp = static_cast<const char*>(a->v_pool);
+  p.rows = a->num_rows;
+  p.Hq = a->num_q_heads;
+  p.Hkv = a->num_kv_heads;
+  p.D = a->head_dim;
+  p.G = p.Hq / p.Hkv;
+  p.bs = a->block_size;
+  p.num_blocks = a->num_blocks;
+  p.bt = a->block_tables;
+  p.num_slots = a->num_slots;
+  p.max_blocks = a->max_blocks_per_seq;
+  p.groups = a->groups;
+  p.max_groups = a->max_groups;
+  p.units = a->units;
+  p.max_units = a->max_units;
+  p.unit_tokens = a->unit_tokens;
+  p.items = a->items;
+  p.max_items = a->max_items;
+  p.merge = a->merge;
+  p.max_merge = a->max_merge;
+  p.counts = a->counts;
+  p.masks = a->masks;
+  p.mask_words = tree ? a->mask_words : 0;
+  p.tree = tree;
+  // positions stay below 2^30, so windows and sinks beyond it mean the same and no sum of them overflows
+  p.window = a->window < (1 << 30) ? a->window : 1 << 30;
+  p.sinks = a->sinks < (1 << 30) ? a->sinks : 1 << 30;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.ws = a->ws;
+  p.ws_rows = a->ws_rows;
+  p.DP = (a->head_dim + 3) / 4 * 4 + 4;
+  p.queue = a->queue;
+  p.status = a->status;
+  return NF_OK;
+}
+
+static int masked_attention(const NfMaskedArgs* a, bool tree, const char* what, void* stream) {
+  MaskedParams p;
+  int rc = masked_check(a, tree, what, p);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p.max_items)
+    return fail(NF_EUNSUPPORTED, "%s: no tensor-core path for this shape", what);
+  if (p.max_units) {
+    switch (a->dtype) {
+      case NF_F32: rc = dispatch_vec<float>(p, st, what); break;
+      case NF_F16: rc = dispatch_vec<__half>(p, st, what); break;
+      default: rc = dispatch_vec<__nv_bfloat16>(p, st, what); break;
+    }
+    if (rc) return rc;
+  }
+  if (p.max_merge) {
+    const long long want = ((long long)p.max_merge * p.Hq + 7) / 8, cap = (long long)sm_count() * 8;
+    const long long blocks = want < cap ? want : cap;
+    switch (a->dtype) {
+      case NF_F32: return launch_masked(masked_merge_kernel<float>, blocks, 256, st, p, what);
+      case NF_F16: return launch_masked(masked_merge_kernel<__half>, blocks, 256, st, p, what);
+      default: return launch_masked(masked_merge_kernel<__nv_bfloat16>, blocks, 256, st, p, what);
+    }
+  }
+  return ok();
+}
+
+}  // namespace nf
+
+extern "C" int nf_masked_limits(int32_t dtype, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                int32_t block_size, int32_t* unit_rows, int32_t* item_rows) {
+  using namespace nf;
+  if (!unit_rows || !item_rows) return fail(NF_EINVAL, "nf_masked_limits: null pointer argument");
+  if (!dtype_size(dtype)) return fail(NF_EINVAL, "nf_masked_limits: bad dtype %d", dtype);
+  if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads > kMaskedMaxHeads)
+    return fail(NF_EINVAL, "nf_masked_limits: num_q_heads (%d) must be a positive multiple of num_kv_heads (%d), at most %d",
+                num_q_heads, num_kv_heads, kMaskedMaxHeads);
+  if (head_dim <= 0 || head_dim > 256) return fail(NF_EUNSUPPORTED, "nf_masked_limits: head_dim %d (1 to 256)", head_dim);
+  if (block_size <= 0) return fail(NF_EINVAL, "nf_masked_limits: block_size must be positive");
+  const int G = num_q_heads / num_kv_heads;
+  *unit_rows = G > kVecRows ? G : kVecRows;
+  *item_rows = 0;
+  return ok();
+}
+
+extern "C" int nf_window_attention(const NfMaskedArgs* args, void* stream) {
+  return nf::masked_attention(args, false, "nf_window_attention", stream);
+}
+
+extern "C" int nf_tree_attention(const NfMaskedArgs* args, void* stream) {
+  return nf::masked_attention(args, true, "nf_tree_attention", stream);
+}

@@ -23,6 +23,8 @@ from nifre_b200.paged_kv_cache import PagedKVCache
 
 
 class KVCache(PagedKVCache):
+    _tables_move = False  # row b owns block b: no forks, window frees or compaction
+
     def __init__(self, num_layers, max_seq_len, n_heads, head_dim, device="cuda", dtype=torch.float16):
         super().__init__(num_layers, max_seq_len, n_heads, head_dim, device=device, dtype=dtype,
                          block_size=max_seq_len, enable_prefix_cache=False)

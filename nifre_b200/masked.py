@@ -1,0 +1,381 @@
+"""Work lists of attention over part of a sequence's keys (windows with sinks, drafted token trees).
+
+No counterpart in the reference, whose attention is causal over the whole
+sequence (``src/inference/attention.py:144-152``).  The lists are built on the
+host once per step (numpy) and uploaded in one copy; every layer of the step
+uses them.  ``include/nifre_b200.h`` defines the records (``NfMaskedArgs``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import torch
+
+from nifre_b200 import _lib
+
+MAX_PARTS = 32767  # parts of one group (a unit record's 15 bits)
+HEAD = 8  # counts (4) and the kernels' work queue (4, zero) at the start of the buffer
+
+
+def tree_visibility(parents) -> np.ndarray:
+    """(n, n) truth values of one drafted tree: token i sees its ancestors and itself.
+
+    ``parents[i] < i`` is the token that token i continues, -1 the context.
+    """
+    parents = np.asarray(parents, dtype=np.int64).reshape(-1)
+    n = len(parents)
+    if (parents < -1).any() or (parents >= np.arange(n)).any():
+        raise ValueError("parents[i] must be -1 (the context) or the index of an earlier drafted token")
+    seen = np.eye(n, dtype=bool)
+    for i in np.flatnonzero(parents >= 0).tolist():
+        seen[i] |= seen[parents[i]]
+    return seen
+
+
+def mask_words(seen: np.ndarray) -> np.ndarray:
+    """Truth values (n, n) as bit rows: (n, ceil(n / 32)) int32, bit j % 32 of word j // 32 for key j."""
+    n = seen.shape[1]
+    words = (n + 31) // 32
+    padded = np.zeros((seen.shape[0], words * 32), dtype=np.uint8)
+    padded[:, :n] = seen
+    return np.packbits(padded, axis=1, bitorder="little").view(np.int32)
+
+
+def virtual_keys(pos0, ntok, window: int, sinks: int):
+    """Keys of a group whose tokens stand at pos0 .. pos0 + ntok - 1, without the blocks of 16 between the sinks
+    and the first token's window: (kept, gap, count); key v is key v for v < kept, else v + gap."""
+    lo = np.maximum(0, pos0 - window + 1) // 16 * 16
+    kept = np.minimum((sinks + 15) // 16 * 16, lo)
+    gap = lo - kept
+    return kept, gap, pos0 + ntok - gap
+
+
+def part_sizes(keys, split: int, align: int):
+    """Keys per part of each group, a multiple of ``align``: equal parts of at most about ``split`` keys."""
+    parts = np.maximum(1, -(-keys // split))
+    return np.maximum(align, -(-keys // (parts * align)) * align)
+
+
+class WorkLists:
+    """Groups, units, tensor-core items and merge rows of one step, and their place in one int32 buffer."""
+
+    def __init__(self, groups, units, items, merge, part_rows: int, unit_tokens: int, masks):
+        self.groups, self.units, self.items, self.merge, self.masks = groups, units, items, merge, masks
+        self.part_rows, self.unit_tokens = part_rows, unit_tokens
+
+    def sizes(self):
+        """Entries of each list, the partial rows and the tokens of the largest unit's group."""
+        return (len(self.groups), len(self.units), len(self.items), len(self.merge), len(self.masks), self.part_rows,
+                self.unit_tokens)
+
+    @staticmethod
+    def room(sizes):
+        """Capacities for lists of these sizes: whole multiples of 64 entries, so that the next steps' lists of the
+        same batch fit as well (the launches are sized by the capacities)."""
+        up = [-(-n // 64) * 64 for n in sizes[:6]]
+        return (*up, sizes[6])
+
+    @staticmethod
+    def offsets(room):
+        """Start of each list in the buffer and its length."""
+        at = np.cumsum([HEAD, 8 * room[0], 4 * room[1], 4 * room[2], 4 * room[3], -(-room[4] // 4) * 4]).tolist()
+        return at[:5], at[5]
+
+    def pack(self, room) -> np.ndarray:
+        at, total = self.offsets(room)
+        host = np.zeros(total, dtype=np.int32)
+        host[:4] = (len(self.units), len(self.items), len(self.merge), 0)
+        for start, part in zip(at, (self.groups, self.units, self.items, self.merge, self.masks)):
+            host[start:start + part.size] = part.reshape(-1)
+        return host
+
+
+def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_rows: int, workers: int, kv_heads: int,
+                window=None, sinks: int = 0, words=None, unit_split=None, item_split=None) -> WorkLists:
+    """Work lists of a step whose sequences get ``q_lens`` new tokens behind ``ctx`` cached ones.
+
+    ``window``/``sinks``, or ``words``: each sequence's mask rows (``mask_words``).
+    ``group``: query heads per KV head.  Groups of units hold up to
+    ``unit_rows`` query rows; sequences with more tokens than that go to the
+    tensor cores' items (``item_rows`` rows) where there are any.
+    """
+    slots, q_lens, q_starts, ctx = (np.asarray(a, dtype=np.int64) for a in (slots, q_lens, q_starts, ctx))
+    t_unit, t_item = max(1, unit_rows // group), item_rows // group
+    routed = (q_lens > t_unit) & (t_item > 0)
+    per = np.where(routed, max(1, t_item), t_unit)
+    n_groups = -(-q_lens // per)
+    seq = np.repeat(np.arange(len(slots)), n_groups)
+    first = np.cumsum(n_groups) - n_groups
+    tok0 = (np.arange(len(seq)) - first[seq]) * per[seq]
+    ntok = np.minimum(per[seq], q_lens[seq] - tok0)
+    pos0 = ctx[seq] + tok0
+    if words is None:
+        keys = virtual_keys(pos0, ntok, window, sinks)[2]
+        mask0 = np.zeros(len(seq), dtype=np.int64)
+        masks = np.zeros(0, dtype=np.int32)
+    else:
+        keys = ctx[seq] + q_lens[seq]
+        start = np.cumsum([0] + [w.size for w in words])
+        mask0 = start[:-1][seq] + tok0 * np.asarray([w.shape[1] for w in words], dtype=np.int64)[seq]
+        masks = np.concatenate([w.reshape(-1) for w in words])
+    on_items = routed[seq]
+    size = np.zeros(len(seq), dtype=np.int64)
+    if (~on_items).any():
+        k = keys[~on_items]
+        split = unit_split or unit_split_for(k, workers)
+        size[~on_items] = part_sizes(k, split, 16)
+    if on_items.any():
+        k = keys[on_items]
+        split = item_split or item_split_for(k, workers, kv_heads)
+        size[on_items] = part_sizes(k, split, 128)
+    parts = -(-keys // size)
+    if parts.size and parts.max() > MAX_PARTS:
+        raise ValueError(f"a sequence's keys are cut into {int(parts.max())} parts, at most {MAX_PARTS}")
+    rows = np.where(parts > 1, parts * ntok, 0)
+    part0 = np.cumsum(rows) - rows
+    groups = np.stack([slots[seq], q_starts[seq] + tok0, ntok, pos0, ctx[seq], q_lens[seq], mask0, part0], axis=1)
+    if groups.size and groups.max() >= 1 << 31:
+        raise ValueError("the step's work lists exceed 32-bit indices")
+
+    def cut(sel):
+        """Units of the groups in sel, the largest first (a queue over the list then ends on short ones)."""
+        g = np.repeat(sel, parts[sel])
+        j = np.arange(len(g)) - np.repeat(np.cumsum(parts[sel]) - parts[sel], parts[sel])
+        k0 = j * size[g]
+        k1 = np.minimum(keys[g], k0 + size[g])
+        u = np.stack([g, k0, k1, j | parts[g] << 16], axis=1)
+        return u[np.argsort(k0 - k1, kind="stable")].astype(np.int32)
+
+    split_groups = np.flatnonzero(parts > 1)
+    m = np.repeat(split_groups, ntok[split_groups])
+    t = np.arange(len(m)) - np.repeat(np.cumsum(ntok[split_groups]) - ntok[split_groups], ntok[split_groups])
+    merge = np.stack([groups[m, 1] + t, part0[m] + t, parts[m], ntok[m]], axis=1).astype(np.int32)
+    return WorkLists(groups.astype(np.int32), cut(np.flatnonzero(~on_items)), cut(np.flatnonzero(on_items)), merge,
+                     int(rows.sum()), int(ntok[~on_items].max()) if (~on_items).any() else 0, masks)
+
+
+def unit_split_for(keys: np.ndarray, workers: int) -> int:
+    """Keys per unit: about four units per worker, at least 64 keys each."""
+    return max(64, -(-int(keys.sum()) // (4 * workers * 16)) * 16)
+
+
+def item_split_for(keys: np.ndarray, workers: int, kv_heads: int) -> int:
+    """Keys per tensor-core item (one per KV head): one item per worker, at least 256 keys each."""
+    want = max(1, int(keys.sum()) * kv_heads // workers)
+    return max(256, -(-want // 128) * 128)
+
+
+class MaskedPlan:
+    """Device work lists of one step for one window, or one set of drafted trees (``PagedKVCache.plan_window`` and
+    ``plan_tree``); valid for every layer of the step, as long as the sequences' blocks stay theirs."""
+
+    def __init__(self, kind: str, window: int, sinks: int, q_heads: int, rows_needed: int):
+        self.kind, self.window, self.sinks, self.q_heads, self.rows_needed = kind, window, sinks, q_heads, rows_needed
+        self.room = None
+        self.buf = self.ws = None  # the uploaded lists; partial rows of the split keys
+        self.args = None  # NfMaskedArgs of the step; a layer's call sets its pointers
+        self.args_ptr = 0
+        self.fn = None
+        self.owner = None
+        self.streams = set()  # streams that the buffers are known to
+        self.ready = None
+        self.upload_bytes = 0
+
+
+class MaskedAttentionOps:
+    """Windowed and tree attention of ``PagedKVCache`` (and the dense ``KVCache``)."""
+
+    def plan_window(self, plan, window: int, sinks: int = 0, q_heads: int | None = None,
+                    into: MaskedPlan | None = None) -> MaskedPlan:
+        """Work lists of ``plan``'s step for layers whose queries see the last ``window`` keys (their own position
+        included) and the first ``sinks`` keys of their sequence.
+
+        ``plan`` is the step's ``plan(...)``; layers with different windows, or
+        with none, share it: each window has a ``MaskedPlan`` of its own.
+        ``q_heads``: query heads of the attention calls (default: those of
+        ``plan``).  ``into``: a plan of the same window from an earlier step of
+        the batch, whose device buffers are filled again, so that a CUDA graph
+        captured with it reads the new step; ValueError where the new lists do
+        not fit them (then capture again with a new plan).
+        """
+        if int(window) != window or window <= 0:
+            raise ValueError(f"window must be a positive whole number, got {window}")
+        if int(sinks) != sinks or sinks < 0:
+            raise ValueError(f"sinks must be a whole number of at least 0, got {sinks}")
+        window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
+        self._check_window_holes(plan.slots, plan.ctx_before, window, sinks)
+        return self._plan_masked("window", plan, q_heads, into, window, sinks, None)
+
+    def plan_tree(self, plan, parents=None, masks=None, q_heads: int | None = None,
+                  into: MaskedPlan | None = None) -> MaskedPlan:
+        """Work lists of ``plan``'s step where each sequence's new tokens are a drafted tree.
+
+        The new tokens of sequence i see its whole cached context and, among
+        themselves, what ``parents[i]`` or ``masks[i]`` says: ``parents[i][j]``
+        is the earlier drafted token that token j continues (-1: the context),
+        and token j sees its ancestors and itself; ``masks[i]`` is an (n, n)
+        array of truth values, row j for what token j sees (a row with nothing
+        to see, before an empty context, gives zeros).  Exactly one of the two;
+        ``None`` for a sequence: its tokens are a chain.  ``q_heads`` and
+        ``into`` as for ``plan_window``.
+        """
+        if (parents is None) == (masks is None):
+            raise ValueError("plan_tree takes parents or masks")
+        given = parents if masks is None else masks
+        if len(given) != plan.n_seqs:
+            raise ValueError(f"{len(given)} trees for {plan.n_seqs} sequences")
+        if self._holes_of(plan.slots):
+            raise ValueError("a sequence whose blocks were freed behind its window cannot be attended as a whole")
+        words = []
+        for n, t in zip(plan.q_lens.tolist(), given):
+            if t is None:
+                seen = np.tril(np.ones((n, n), dtype=bool))
+            elif masks is None:
+                seen = tree_visibility(t)
+            else:
+                seen = np.asarray(t.cpu() if torch.is_tensor(t) else t).astype(bool)
+            if seen.shape != (n, n):
+                raise ValueError(f"a tree of {seen.shape} for {n} new tokens")
+            words.append(mask_words(seen))
+        return self._plan_masked("tree", plan, q_heads, into, 0, 0, words)
+
+    def masked_limits(self, q_heads: int) -> tuple[int, int]:
+        """Query rows of the largest unit's and the largest tensor-core item's group (``nf_masked_limits``)."""
+        memo = self.__dict__.setdefault("_masked_limit_memo", {})
+        if q_heads not in memo:
+            a, b = ctypes.c_int32(0), ctypes.c_int32(0)
+            _lib.check(_lib.load().nf_masked_limits(_lib.dtype_code(self.dtype), q_heads, self.n_heads, self.head_dim,
+                                                    self.block_size, ctypes.byref(a), ctypes.byref(b)),
+                       "nf_masked_limits")
+            memo[q_heads] = (a.value, b.value)
+        return memo[q_heads]
+
+    def _plan_masked(self, kind, plan, q_heads, into, window, sinks, words) -> MaskedPlan:
+        q_heads = plan.q_heads if q_heads is None else int(q_heads)
+        if q_heads is None or q_heads <= 0 or q_heads % self.n_heads:
+            raise ValueError(f"q_heads must be a positive multiple of the cache's {self.n_heads} heads, got {q_heads}")
+        if int(plan.slots.max()) >= self.batch_size:
+            raise IndexError(f"cache slot out of range [0, {self.batch_size})")
+        unit_rows, item_rows = self.masked_limits(q_heads)
+        lists = build_lists(plan.slots, plan.q_lens, plan.q_starts, plan.ctx_before, q_heads // self.n_heads, unit_rows,
+                            item_rows, self.masked_workers, self.n_heads, window, sinks, words)
+        sizes = lists.sizes()
+        if into is None:
+            view = MaskedPlan(kind, window, sinks, q_heads, plan.rows_needed)
+            view.room = lists.room(sizes)
+        else:
+            view = into
+            if (view.kind, view.window, view.sinks, view.q_heads) != (kind, window, sinks, q_heads) \
+                    or view.owner is not self:
+                raise ValueError("into is the plan of another cache, window or set of heads")
+            if any(n > r for n, r in zip(sizes, view.room)):
+                raise ValueError(f"the step's lists {sizes} do not fit the plan's room {view.room}")
+            view.rows_needed = plan.rows_needed
+        host = torch.from_numpy(lists.pack(view.room)).pin_memory()
+        view.upload_bytes = host.numel() * 4
+        if into is not None:
+            view.buf.copy_(host, non_blocking=True)
+            view.ready.record()
+            return view
+        view.buf = host.to(self.device, non_blocking=True)
+        D, room = self.head_dim, view.room
+        view.ws = torch.empty(room[5] * q_heads * (-(-D // 4) * 4 + 4), dtype=torch.float32, device=self.device)
+        at, _ = lists.offsets(room)
+        base = view.buf.data_ptr()
+        ptr = lambda i: base + 4 * at[i] if room[i] else None  # noqa: E731
+        view.args = _lib.NfMaskedArgs(
+            block_tables=self._bt_ptr, groups=ptr(0), units=ptr(1), items=ptr(2), merge=ptr(3), counts=base,
+            masks=ptr(4), mask_words=room[4], ws=view.ws.data_ptr() if room[5] else None, ws_rows=room[5],
+            queue=base + 16, status=self._status_ptr, dtype=self._dt_code, num_q_heads=q_heads,
+            num_kv_heads=self.n_heads, head_dim=D, block_size=self.block_size, num_blocks=self.num_blocks,
+            num_slots=self.batch_size, max_blocks_per_seq=self.max_blocks_per_seq, max_groups=room[0],
+            max_units=room[1], unit_tokens=room[6], max_items=room[2], max_merge=room[3], window=window, sinks=sinks)
+        view.args_ptr = ctypes.addressof(view.args)
+        lib = _lib.load()
+        view.fn = lib.nf_tree_attention if kind == "tree" else lib.nf_window_attention
+        view.owner = self
+        view.ready = torch.cuda.Event()
+        view.ready.record(torch.cuda.current_stream(self.device))
+        view.streams = {self._stream()}
+        return view
+
+    @property
+    def masked_workers(self) -> int:
+        """Workers the masked kernels' units are sized for: one per SM."""
+        return self.sm_count
+
+    def window_attention_step(self, layer_id: int, q: torch.Tensor, view: MaskedPlan, out: torch.Tensor,
+                              scale: float | None = None) -> torch.Tensor:
+        """out[row] = attention of q[row] over the keys of its sequence in ``view``'s window and sinks, for the step's
+        rows; the other rows of ``out`` are left untouched.
+
+        ``q``/``out``: (rows, Hq*D) in the pool dtype with unit column stride
+        (``out`` must not overlap ``q``).  ``scale`` defaults to 1 / sqrt(D).
+        Keys that a query does not see contribute nothing, whatever their rows
+        hold.  Calls with the same plan must not overlap on the GPU (its work
+        queue and partial rows are shared); a CUDA graph that captured one needs
+        the plan kept alive.
+        """
+        if view.kind != "window":
+            raise ValueError("the plan is a tree's: use tree_attention_step")
+        return self._masked_step(layer_id, q, view, out, scale)
+
+    def tree_attention_step(self, layer_id: int, q: torch.Tensor, view: MaskedPlan, out: torch.Tensor,
+                            scale: float | None = None) -> torch.Tensor:
+        """out[row] = attention of the drafted token q[row] over its sequence's context and the drafted tokens that it
+        sees (``plan_tree``).  Arguments as for ``window_attention_step``."""
+        if view.kind != "tree":
+            raise ValueError("the plan is a window's: use window_attention_step")
+        return self._masked_step(layer_id, q, view, out, scale)
+
+    def _masked_step(self, layer_id, q, view, out, scale):
+        if not q.is_cuda or q.device != out.device:
+            _lib.require_cuda(q, "q")
+            raise ValueError("q and out must be on the same device")
+        if view.owner is not self:
+            raise ValueError("the plan belongs to another cache")
+        if view.args.block_tables != self._bt_ptr:
+            raise ValueError("the plan was made before the cache's last init_batch")
+        width = view.q_heads * self.head_dim
+        shape = q.shape
+        if len(shape) != 2 or shape[1] != width or q.stride(1) != 1:
+            raise ValueError(f"q must be (rows, {width}) with unit column stride")
+        if out.shape != shape or out.stride(1) != 1 or (shape[0] > 1 and out.stride(0) < width):
+            raise ValueError("out must have q's shape, unit column stride and rows of their own")
+        if q.dtype != self.dtype or out.dtype != self.dtype:
+            raise ValueError(f"q/out dtype must be the cache dtype {self.dtype}")
+        if shape[0] < view.rows_needed:
+            raise ValueError(f"q has {shape[0]} rows, the step uses rows up to {view.rows_needed}")
+        if not 0 <= layer_id < self.num_layers:
+            raise IndexError(f"layer_id {layer_id} out of range [0, {self.num_layers})")
+        if q.device.index != self._dev_index:
+            raise ValueError(f"q is on {q.device}, the cache on {self.device}")
+        if torch.cuda.current_device() != self._dev_index:
+            with torch.cuda.device(self._dev_index):
+                return self._masked_step(layer_id, q, view, out, scale)
+        stream = self._stream()
+        if stream not in view.streams:
+            self._adopt_stream(view, stream)
+        a = view.args
+        a.out, a.q, a.k_pool, a.v_pool = out.data_ptr(), q.data_ptr(), self._k_ptr[layer_id], self._v_ptr[layer_id]
+        a.out_row_stride, a.q_row_stride, a.num_rows = out.stride(0), q.stride(0), shape[0]
+        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        rc = view.fn(view.args_ptr, stream)
+        if rc:
+            _lib.check(rc, "nf_%s_attention" % view.kind)
+        return out
+
+    @staticmethod
+    def _adopt_stream(view, stream) -> None:
+        """First call of a plan on another stream than its own: the upload comes first, and the buffers stay until
+        that stream is done with them.  (A capturing stream orders and keeps nothing: its graph's user does.)"""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        cur = torch.cuda.current_stream()
+        cur.wait_event(view.ready)
+        view.buf.record_stream(cur)
+        if view.ws.numel():
+            view.ws.record_stream(cur)
+        view.streams.add(stream)

@@ -38,6 +38,8 @@ import torch
 from nifre_b200 import _lib
 from nifre_b200.block_allocator import BlockAllocator
 from nifre_b200.block_table import BlockTable
+from nifre_b200.masked import MaskedAttentionOps
+from nifre_b200.pages import PageOps
 from nifre_b200.prefix_cache import PrefixCache
 
 
@@ -129,13 +131,15 @@ class StepPlan:
         self.sched = None
         # per-plan constant arguments of the layers' C ABI calls, built on first use
         self.append_args = self.decode_args = None
+        self.holes = False  # some sequence's blocks were freed behind its window
+        self.views = {}  # the step's plans of windows, made by Attention: (window, sinks, query heads) -> MaskedPlan
 
     @property
     def kv_lens(self) -> np.ndarray:
         return self.ctx_before + self.q_lens
 
 
-class PagedKVCache:
+class PagedKVCache(MaskedAttentionOps, PageOps):
     def __init__(self, num_layers: int, max_seq_len: int, n_heads: int, head_dim: int,
                  device="cuda", dtype: torch.dtype = torch.float16, block_size: int = 16,
                  enable_prefix_cache: bool = True, prefix_cache_max_entries: int = 1024,
@@ -197,6 +201,9 @@ class PagedKVCache:
         self._dt_code = _lib.dtype_code(self.dtype)
         self._pool_rows = self.num_blocks * self.block_size
         self._row_width = self.n_heads * self.head_dim
+        self._row_bytes = self._row_width * self._k_all.element_size()
+        self._layer_bytes = self._pool_rows * self._row_bytes
+        self._init_holes(batch_size)
         self.bt_dev = torch.zeros((batch_size, self.max_blocks_per_seq), dtype=torch.int32, device=self.device)
         # per slot: the table epoch and the number of entries mirrored on the device
         self._sync_epoch = np.full(batch_size, -1, dtype=np.int64)
@@ -224,6 +231,7 @@ class PagedKVCache:
         self.prefix_cache = None
         self._plan = None
         self._k_all = self._v_all = None
+        self._bt_ptr = None  # plans made before are not of the next batch
 
     # ------------------------------------------------------------------ reference API
     def try_load_prefix(self, batch_idx: int, token_ids: list[int]) -> int:
@@ -239,7 +247,10 @@ class PagedKVCache:
     def register_prefix(self, batch_idx: int, token_ids: list[int]) -> None:
         if self.prefix_cache is None:
             return
-        self.prefix_cache.insert(token_ids, self.block_tables[batch_idx].physical_blocks())
+        blocks = self.block_tables[batch_idx].physical_blocks()
+        if -1 in blocks:  # blocks freed behind the sequence's window end the prefix
+            blocks = blocks[:blocks.index(-1)]
+        self.prefix_cache.insert(token_ids, blocks)
 
     def append(self, batch_idx: int, layer_id: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Append ``key``/``value`` (n, H, D) of one sequence (reference per-row API)."""
@@ -252,6 +263,8 @@ class PagedKVCache:
         if pos == 0:
             empty = torch.empty(0, self.n_heads, self.head_dim, device=self.device, dtype=self.dtype)
             return empty, empty.clone()
+        if self._hole_end[batch_idx]:
+            raise ValueError("blocks of the sequence were freed behind its window")
         nb = (pos + self.block_size - 1) // self.block_size
         idx = torch.tensor(self.block_tables[batch_idx].physical_blocks()[:nb], device=self.device)
         k = self.k[layer_id].index_select(0, idx).reshape(-1, self.n_heads, self.head_dim)[:pos]
@@ -266,6 +279,7 @@ class PagedKVCache:
 
     def reset_slot(self, batch_idx: int) -> None:
         self.block_tables[batch_idx].clear()
+        self._clear_hole(batch_idx)
         self._set_pos(batch_idx, 0)
 
     @property
@@ -491,7 +505,7 @@ class PagedKVCache:
         patches = []
         for i in np.flatnonzero(have > done).tolist():
             s_, blocks = sl[i], tabs[sl[i]]._physical_blocks
-            patches.extend((s_, lb, blocks[lb]) for lb in range(int(done[i]), int(have[i])))
+            patches.extend((s_, lb, blocks[lb]) for lb in range(int(done[i]), int(have[i])) if blocks[lb] >= 0)
         self._sync_epoch[slots] = epochs
         self._sync_len[slots] = have
         P = len(patches)
@@ -500,8 +514,13 @@ class PagedKVCache:
         kv = np.repeat(ctx + 1, q_lens) + (np.arange(T) - np.repeat(np.cumsum(q_lens) - q_lens, q_lens))
         routed = (q_lens >= self.PREFILL_MIN_TOKENS) if self.prefill_supported(q_heads) else np.zeros(S, bool)
         dec = ~routed
-        if self.cascade_supported(q_heads) and dec.any():
-            shared, nparts, ctasks, ctoks = self._cascade_groups(slots, q_lens, q_starts, ctx, dec,
+        holes = self._hole_end[slots] > 0  # blocks freed behind a window: no full attention
+        if holes.any():
+            dec_shared = dec & ~holes
+        else:
+            dec_shared = dec
+        if self.cascade_supported(q_heads) and dec_shared.any():
+            shared, nparts, ctasks, ctoks = self._cascade_groups(slots, q_lens, q_starts, ctx, dec_shared,
                                                                  q_heads // self.n_heads, epochs)
         else:
             shared, nparts, ctasks, ctoks = np.zeros(S, np.int32), np.zeros(S, np.int32), [], []
@@ -573,6 +592,7 @@ class PagedKVCache:
         plan.layout_key = (meta.data_ptr(), off_ct, off_tok, off_slot, off_units, off_counts, max_units, S, T,
                            n_ct, n_tok, n_tiles, q_heads)
         plan.decode_units = n_units
+        plan.holes = bool(holes.any())
         plan.q_heads = q_heads
         plan.shared_keys = shared
         plan.n_casc_tasks, plan.n_casc_toks = n_ct, n_tok
@@ -702,6 +722,8 @@ class PagedKVCache:
             raise ValueError(f"q has {q.shape[0]} rows, the step uses rows up to {plan.rows_needed}")
         if not 0 <= layer_id < self.num_layers:
             raise IndexError(f"layer_id {layer_id} out of range [0, {self.num_layers})")
+        if plan.holes:
+            raise ValueError("blocks of a sequence were freed behind its window: use window_attention_step")
         hq = q.shape[1] // D
         if (plan.n_tiles or plan.n_casc_tasks) and hq != plan.q_heads:
             raise ValueError(f"the plan's prefill tiles / cascade groups are for {plan.q_heads} query heads, q has {hq}")

@@ -1,0 +1,397 @@
+"""Windowed and tree attention over the paged pools against the definition in 64 bits (needs a B200).
+
+Tolerances are oracle.masked.tolerance (derived there from the roundings the
+kernels make).  The pools start as NaN everywhere, so that a key row no token
+sees (behind the window, past the sequence, never written) shows if it reaches
+an output.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle.masked import attend, tolerance, tree_seen, window_seen
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib_built():
+    from nifre_b200 import _lib
+    _lib.load()
+
+
+class Step:
+    """A cache with contexts of ``ctx`` tokens and a step of ``n`` new ones (rows ``pad`` apart in q and out)."""
+
+    def __init__(self, ctx, n, hq, hkv, d, bs, dtype, seed=0, layers=1, pad=0, room=16, cls=None):
+        from nifre_b200 import PagedKVCache
+        g = torch.Generator().manual_seed(seed)
+        self.ctx, self.n, self.hq, self.hkv, self.d, self.dtype = list(ctx), list(n), hq, hkv, d, dtype
+        S = len(ctx)
+        most = max(c + m for c, m in zip(ctx, n)) + room
+        if cls is None:
+            self.cache = PagedKVCache(layers, most, hkv, d, device=DEV, dtype=dtype, block_size=bs,
+                                      enable_prefix_cache=False)
+        else:
+            self.cache = cls(layers, most, hkv, d, device=DEV, dtype=dtype)
+        self.cache.init_batch(S)
+        for t in (*self.cache.k, *self.cache.v):
+            t.fill_(float("nan"))
+        if cls is None:
+            self.cache.block_allocator.set_free_order(torch.randperm(self.cache.num_blocks, generator=g).tolist())
+        self.g = g
+        filled = [i for i in range(S) if ctx[i]]
+        # k[s], v[s]: rows of every layer's keys and values of sequence s (layers, tokens, Hkv, D)
+        self.k = [torch.empty(layers, 0, hkv, d, dtype=dtype, device=DEV) for _ in range(S)]
+        self.v = [t.clone() for t in self.k]
+        if filled:
+            self._append(filled, [ctx[i] for i in filled])
+        self.start, at = [], pad
+        for m in self.n:
+            self.start.append(at)
+            at += m + pad
+        self.rows = at
+        self.plan = self._append(list(range(S)), self.n, self.start, at, q_heads=hq)
+        self.q = self.rand(layers, self.rows, hq * d)
+
+    def rand(self, *shape):
+        return torch.randn(*shape, generator=self.g).to(self.dtype).to(DEV)
+
+    def _append(self, slots, lens, starts=None, rows=None, q_heads=None):
+        starts = starts or [sum(lens[:i]) for i in range(len(lens))]
+        rows = rows or sum(lens)
+        plan = self.cache.plan(slots, lens, starts, q_heads=q_heads)
+        ks, vs = [], []
+        for layer in range(self.cache.num_layers):
+            k, v = self.rand(rows, self.hkv * self.d), self.rand(rows, self.hkv * self.d)
+            self.cache.append_step(layer, k, v, plan)
+            ks.append(k.view(rows, self.hkv, self.d))
+            vs.append(v.view(rows, self.hkv, self.d))
+        k, v = torch.stack(ks), torch.stack(vs)
+        for s, m, st in zip(slots, lens, starts):
+            self.k[s] = torch.cat([self.k[s], k[:, st:st + m]], 1)
+            self.v[s] = torch.cat([self.v[s], v[:, st:st + m]], 1)
+        return plan
+
+    def check(self, out, seen_of, layer=0, scale=None, q=None):
+        """out against the definition, every row; rows between the sequences' keep their 7."""
+        q = self.q[layer] if q is None else q
+        used = torch.zeros(self.rows, dtype=torch.bool)
+        scale = self.d ** -0.5 if scale is None else scale
+        for s, (c, m, st) in enumerate(zip(self.ctx, self.n, self.start)):
+            used[st:st + m] = True
+            ref, wabs, most = attend(q[st:st + m].view(m, self.hq, self.d), self.k[s][layer], self.v[s][layer],
+                                     seen_of(s), scale)
+            tol = tolerance(ref, wabs, most, c + m, self.d, self.dtype)
+            got = out[st:st + m].view(m, self.hq, self.d).double()
+            err = (got - ref).abs()
+            assert torch.isfinite(got).all(), (s, c, m)
+            assert (err <= tol).all(), (s, c, m, float((err / tol).max()), float(err.max()))
+        assert (out[~used.to(out.device)] == 7).all()
+        self.cache.check_status()
+
+    def window(self, window, sinks, layer=0, q=None, **kw):
+        view = self.cache.plan_window(self.plan, window, sinks, q_heads=self.hq)
+        q = self.q[layer] if q is None else q
+        out = torch.full((self.rows, self.hq * self.d), 7, dtype=self.dtype, device=DEV)
+        self.cache.window_attention_step(layer, q, view, out, **kw)
+        self.check(out, lambda s: window_seen(self.ctx[s], self.n[s], window, sinks), layer, q=q, **kw)
+        return out
+
+    def tree(self, masks, layer=0, q=None, parents=None, **kw):
+        given = dict(masks=masks) if parents is None else dict(parents=parents)
+        view = self.cache.plan_tree(self.plan, q_heads=self.hq, **given)
+        q = self.q[layer] if q is None else q
+        out = torch.full((self.rows, self.hq * self.d), 7, dtype=self.dtype, device=DEV)
+        self.cache.tree_attention_step(layer, q, view, out, **kw)
+        self.check(out, lambda s: tree_seen(self.ctx[s], torch.as_tensor(masks[s])), layer, q=q, **kw)
+        return out
+
+
+# query heads, KV heads, head_dim, block size, type
+SHAPES = [(32, 8, 64, 16, BF), (8, 8, 64, 32, HF), (8, 1, 128, 16, HF), (16, 4, 128, 64, BF), (4, 2, 64, 16, BF),
+          (12, 12, 64, 16, F32), (6, 2, 80, 8, HF), (4, 4, 32, 5, F32), (3, 1, 7, 3, BF), (16, 1, 256, 16, F32),
+          (40, 2, 64, 16, BF), (6, 2, 64, 16, HF), (8, 1, 64, 48, BF), (4, 4, 96, 16, BF)]
+IDS = [f"{a}q{b}kv{c}d{d}b{str(e)[6:]}" for a, b, c, d, e in SHAPES]
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 1), (64, 4), (130, 33), (1000, 0), (1 << 30, 0)])
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+def test_window_attention(shape, window, sinks):
+    """Empty and short contexts, block and tile edges, decodes, short chunks and prefill chunks in one step."""
+    hq, hkv, d, bs, dtype = shape
+    st = Step([0, 1, 15, 16, 300, 777, 0], [1, 5, 1, 40, 2, 1, 70], hq, hkv, d, bs, dtype, seed=window + sinks, pad=2)
+    st.window(window, sinks)
+
+
+def _random_tree(n, g):
+    parents = [-1] + [int(torch.randint(-1, i, (1,), generator=g)) for i in range(1, n)]
+    return parents
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+def test_tree_attention(shape):
+    from nifre_b200 import tree_visibility
+    hq, hkv, d, bs, dtype = shape
+    n = [1, 7, 33, 2, 64, 16, 90]
+    st = Step([0, 3, 16, 250, 600, 31, 129], n, hq, hkv, d, bs, dtype, seed=3, pad=1)
+    parents = [_random_tree(m, st.g) for m in n]
+    parents[3] = None  # a chain
+    masks = [np.tril(np.ones((m, m), bool)) if p is None else tree_visibility(p) for m, p in zip(n, parents)]
+    st.tree(masks, parents=parents)
+
+
+@pytest.mark.parametrize("shape", [SHAPES[i] for i in (0, 2, 5, 6, 10)], ids=[IDS[i] for i in (0, 2, 5, 6, 10)])
+def test_tree_masks_that_leave_rows_empty(shape):
+    """Any mask goes, later tokens and empty rows among it; a token that sees nothing gets zeros."""
+    hq, hkv, d, bs, dtype = shape
+    n = [9, 40, 3, 65]
+    st = Step([0, 0, 50, 130], n, hq, hkv, d, bs, dtype, seed=4)
+    rng = np.random.default_rng(0)
+    masks = [rng.integers(0, 2, size=(m, m)).astype(bool) for m in n]
+    masks[0][3] = False
+    masks[1][:] = False
+    masks[2][:] = False
+    out = st.tree(masks)
+    assert (out[st.start[0] + 3] == 0).all() and (out[st.start[1]:st.start[1] + 40] == 0).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES[:7], ids=IDS[:7])
+def test_values_of_unseen_keys_do_not_matter(shape):
+    """NaN and infinities in keys and values that a token does not see, though others of its group do."""
+    hq, hkv, d, bs, dtype = shape
+    n = [12, 30]
+    st = Step([70, 200], n, hq, hkv, d, bs, dtype, seed=5)
+    masks = [np.eye(m, dtype=bool) for m in n]
+    for s in range(2):
+        masks[s][:, 0] = True
+        masks[s][5, 4] = True
+    bad = {4: float("nan"), 7: float("inf"), 9: float("-inf")}
+    for s in range(2):
+        for j, x in bad.items():
+            t = st.ctx[s] + j
+            block, off = st.cache.block_tables[s].resolve(t)
+            st.cache.k[0][block, off] = x
+            st.cache.v[0][block, off] = x
+            st.k[s][0, t], st.v[s][0, t] = x, x
+    view = st.cache.plan_tree(st.plan, masks=masks, q_heads=hq)
+    out = torch.full((st.rows, hq * d), 7, dtype=dtype, device=DEV)
+    st.cache.tree_attention_step(0, st.q[0], view, out)
+    hit = {4, 5, 7, 9}
+    for s in range(2):
+        for i in range(n[s]):
+            row = out[st.start[s] + i]
+            if i in hit:
+                assert not torch.isfinite(row).any()
+                continue
+            ref, wabs, most = attend(st.q[0][st.start[s] + i].view(1, hq, d), st.k[s][0], st.v[s][0],
+                                     tree_seen(st.ctx[s], torch.as_tensor(masks[s]))[i:i + 1], d ** -0.5)
+            tol = tolerance(ref, wabs, most, st.ctx[s] + n[s], d, dtype)
+            assert ((row.view(1, hq, d).double() - ref).abs() <= tol).all()
+    # a window's chunk: keys behind the later tokens' windows
+    st = Step([40], [40], hq, hkv, d, bs, dtype, seed=6)
+    for t in (45, 50):
+        block, off = st.cache.block_tables[0].resolve(t)
+        st.cache.v[0][block, off] = float("nan")
+    view = st.cache.plan_window(st.plan, 8, 2, q_heads=hq)
+    out = torch.full((st.rows, hq * d), 7, dtype=dtype, device=DEV)
+    st.cache.window_attention_step(0, st.q[0], view, out)
+    seen = window_seen(40, 40, 8, 2)
+    touched = seen[:, 45] | seen[:, 50]
+    assert torch.isfinite(out[~touched]).all() and not torch.isfinite(out[touched]).any()
+    ref, wabs, most = attend(st.q[0].view(40, hq, d), st.k[0][0], st.v[0][0], seen, d ** -0.5)
+    tol = tolerance(ref, wabs, most, 80, d, dtype)
+    err = (out.view(40, hq, d).double() - ref).abs()
+    assert (err[~touched] <= tol[~touched]).all()
+
+
+@pytest.mark.parametrize("shape", [SHAPES[i] for i in (0, 2, 3, 5, 8)], ids=[IDS[i] for i in (0, 2, 3, 5, 8)])
+def test_keys_split_into_many_parts(shape, monkeypatch):
+    from nifre_b200 import masked, tree_visibility
+    hq, hkv, d, bs, dtype = shape
+    monkeypatch.setattr(masked, "unit_split_for", lambda *a: 16)
+    monkeypatch.setattr(masked, "item_split_for", lambda *a: 128)
+    n = [1, 3, 48]
+    st = Step([1300, 650, 500], n, hq, hkv, d, bs, dtype, seed=7, pad=1)
+    st.window(700, 20)
+    masks = [tree_visibility(_random_tree(m, st.g)) for m in n]
+    st.tree(masks)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_strided_unaligned_queries_and_scale(dtype):
+    """q as a column slice of a wider projection (rows not 16-byte aligned), out rows with their own stride, a scale
+    of the caller's, several layers with windows of their own."""
+    st = Step([100, 0, 37], [1, 20, 3], 8, 2, 64, 16, dtype, seed=8, layers=3, pad=1)
+    for layer, (w, s) in enumerate([(30, 2), (1 << 20, 0), (9, 0)]):
+        wide = st.rand(st.rows, 8 * 64 + 131)
+        q = wide[:, 65:65 + 512]
+        st.window(w, s, layer=layer, q=q, scale=0.31)
+    view = st.cache.plan_window(st.plan, 30, 2, q_heads=8)
+    buf = torch.full((st.rows, 530), 7, dtype=dtype, device=DEV)
+    st.cache.window_attention_step(1, st.q[1], view, buf[:, 9:521])
+    st.check(buf[:, 9:521], lambda s: window_seen(st.ctx[s], st.n[s], 30, 2), 1)
+    assert (buf[:, :9] == 7).all() and (buf[:, 521:] == 7).all()
+
+
+def test_large_scores_and_long_window():
+    """Scores far from 0 (one key takes all the weight) and a running maximum that moves late."""
+    st = Step([3000], [4], 8, 2, 64, 16, BF, seed=9)
+    for t in (10, 1500, 2999):
+        block, off = st.cache.block_tables[0].resolve(t)
+        st.cache.k[0][block, off] *= 8
+        st.k[0][0, t] *= 8
+    st.window(2500, 16)
+    st.window(4000, 0, scale=2.0)
+
+
+def test_dense_cache_rows():
+    from nifre_b200 import KVCache
+    for room in (16, 13):
+        st = Step([30, 100], [1, 19], 4, 4, 64, None, HF, seed=10, cls=KVCache, room=room)
+        st.window(50, 3)
+        st.tree([np.tril(np.ones((m, m), bool)) for m in st.n])
+
+
+def test_plans_of_other_caches_and_kinds_are_refused():
+    a, b = (Step([10], [2], 4, 2, 64, 16, HF, seed=i) for i in range(2))
+    out = torch.empty_like(a.q[0])
+    w = a.cache.plan_window(a.plan, 4, q_heads=4)
+    t = a.cache.plan_tree(a.plan, [None], q_heads=4)
+    with pytest.raises(ValueError, match="another cache"):
+        b.cache.window_attention_step(0, a.q[0], w, out)
+    with pytest.raises(ValueError, match="window's"):
+        a.cache.tree_attention_step(0, a.q[0], w, out)
+    with pytest.raises(ValueError, match="tree's"):
+        a.cache.window_attention_step(0, a.q[0], t, out)
+    with pytest.raises(IndexError, match="layer_id"):
+        a.cache.window_attention_step(1, a.q[0], w, out)
+    for q, o in ((a.q[0][:1], out[:1]), (a.q[0][:, :128], out), (a.q[0].float(), out), (a.q[0], out.float()),
+                 (a.q[0], out[:1]), (a.q[0], out[:1].expand(2, -1))):
+        with pytest.raises(ValueError):
+            a.cache.window_attention_step(0, q, w, o)
+    with pytest.raises(ValueError, match="another cache, window"):
+        a.cache.plan_window(a.plan, 5, q_heads=4, into=w)
+    from nifre_b200 import _lib
+    with pytest.raises(_lib.NifreError, match="CUDA tensor"):
+        a.cache.window_attention_step(0, a.q[0].cpu(), w, out.cpu())
+    a.cache.free()
+    a.cache.init_batch(1)
+    with pytest.raises(ValueError, match="init_batch"):
+        a.cache.window_attention_step(0, a.q[0], w, out)
+
+
+def test_bad_records_are_flagged_not_followed():
+    """Work lists and block tables with values out of range: skipped and flagged by the kernels' own checks."""
+    from nifre_b200 import _lib
+    st = Step([40, 40], [1, 1], 4, 2, 64, 16, F32, seed=12)
+    view = st.cache.plan_window(st.plan, 30, 0, q_heads=4)
+    at, _ = __import__("nifre_b200.masked", fromlist=["WorkLists"]).WorkLists.offsets(view.room)
+    good = view.buf.clone()
+    for index, value, bit in ((at[0], 99, "bad slot=1"), (at[0] + 1, 77, "bad slot=1"), (at[1], 1 << 20, "unit overflow=1")):
+        view.buf.copy_(good)
+        view.buf[index] = value
+        out = torch.full((2, 256), 7, dtype=F32, device=DEV)
+        st.cache.window_attention_step(0, st.q[0], view, out)
+        with pytest.raises(_lib.NifreError, match=bit):
+            st.cache.check_status()
+        assert (out == 7).all(1).sum() == 1  # the other sequence's row is there
+    view.buf.copy_(good)
+    st.cache.bt_dev[0, 1] = 10_000
+    out = torch.full((2, 256), 7, dtype=F32, device=DEV)
+    st.cache.window_attention_step(0, st.q[0], view, out)
+    with pytest.raises(_lib.NifreError, match="bad block=1"):
+        st.cache.check_status()
+
+
+@pytest.mark.parametrize("shape", [SHAPES[i] for i in (0, 3, 5)], ids=[IDS[i] for i in (0, 3, 5)])
+def test_captured_decode_steps_with_refilled_plans(shape):
+    """A CUDA graph of a layer's append and windowed attention, replayed over the next steps of the batch with
+    plan(fixed_layout=True) and plan_window(into=...)."""
+    from nifre_b200 import PagedKVCache
+    hq, hkv, d, bs, dtype = shape
+    S, ctx = 5, [3, 100, 47, 260, 15]
+    st = Step(ctx, [1] * S, hq, hkv, d, bs, dtype, seed=13, room=64)
+    cache = st.cache
+    q, out = torch.empty(S, hq * d, dtype=dtype, device=DEV), torch.empty(S, hq * d, dtype=dtype, device=DEV)
+    k, v = (torch.empty(S, hkv * d, dtype=dtype, device=DEV) for _ in range(2))
+    graph = view = key = None
+    replays = 0
+    for step in range(12):
+        for t in (q, k, v):
+            t.copy_(st.rand(*t.shape))
+        plan = cache.plan(range(S), [1] * S, range(S), q_heads=hq, fixed_layout=True)
+        fresh = view is None or plan.layout_key != key
+        view = cache.plan_window(plan, 40, 4, q_heads=hq, into=None if fresh else view)
+        if fresh:
+            key = plan.layout_key
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                cache.append_step(0, k, v, plan)
+                cache.window_attention_step(0, q, view, out)
+        else:
+            cache._close(plan)
+            replays += 1
+        graph.replay()
+        for s in range(S):
+            st.k[s] = torch.cat([st.k[s], k[s].view(1, 1, hkv, d)], 1)
+            st.v[s] = torch.cat([st.v[s], v[s].view(1, 1, hkv, d)], 1)
+            c = st.k[s].shape[1] - 1
+            ref, wabs, most = attend(q[s].view(1, hq, d), st.k[s][0], st.v[s][0], window_seen(c, 1, 40, 4), d ** -0.5)
+            tol = tolerance(ref, wabs, most, c + 1, d, dtype)
+            assert ((out[s].view(1, hq, d).double() - ref).abs() <= tol).all(), (step, s)
+    assert replays >= 6
+    cache.check_status()
+
+
+def test_two_plans_on_two_streams():
+    """Plans have work queues and partial rows of their own: different plans' calls may overlap."""
+    st = Step([2000, 1500, 900], [1, 8, 20], 32, 8, 64, 16, BF, seed=14)
+    views = [st.cache.plan_window(st.plan, 1200, 4, q_heads=32) for _ in range(2)]
+    want = torch.empty_like(st.q[0])
+    st.cache.window_attention_step(0, st.q[0], views[0], want)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.zeros_like(want) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for view, stream, out in zip(views, streams, outs):
+            with torch.cuda.stream(stream):
+                st.cache.window_attention_step(0, st.q[0], view, out)
+    torch.cuda.synchronize()
+    for out in outs:
+        assert torch.equal(out, want)  # and the same bits every time
+    st.cache.check_status()
+
+
+def test_attention_module_with_a_window():
+    """Attention(window=...) over padded prefills and decodes, layers with and without windows sharing a step."""
+    from nifre_b200 import Attention, PagedKVCache
+    g = torch.Generator().manual_seed(15)
+    hq, hkv, d, L = 8, 2, 64, 3
+    cache = PagedKVCache(L, 256, hkv, d, device=DEV, dtype=BF, block_size=16, enable_prefix_cache=False)
+    cache.init_batch(3)
+    layers = [Attention(hq, d, window=20, sinks=3), Attention(hq, d), Attention(hq, d, window=5)]
+    ks = [[torch.empty(0, hkv, d, dtype=BF, device=DEV) for _ in range(3)] for _ in range(L)]
+    vs = [[t.clone() for t in r] for r in ks]
+    rand = lambda *s: torch.randn(*s, generator=g).to(BF).to(DEV)  # noqa: E731
+    for T, lens in ((50, [50, 17, 33]), (1, None), (1, None), (4, [4, 1, 3])):
+        for layer, att in enumerate(layers):
+            q, k, v = rand(3, T, hq * d), rand(3, T, hkv * d), rand(3, T, hkv * d)
+            out = att(q, k, v, kv_cache=cache, layer_id=layer, input_lens=lens)
+            for b in range(3):
+                n = lens[b] if lens else T
+                assert torch.count_nonzero(out[b, :T - n]) == 0
+                c = ks[layer][b].shape[0]
+                ks[layer][b] = torch.cat([ks[layer][b], k[b, T - n:].view(n, hkv, d)])
+                vs[layer][b] = torch.cat([vs[layer][b], v[b, T - n:].view(n, hkv, d)])
+                seen = window_seen(c, n, att.window or 1 << 20, att.sinks)
+                ref, wabs, most = attend(q[b, T - n:].view(n, hq, d), ks[layer][b], vs[layer][b], seen, d ** -0.5)
+                tol = tolerance(ref, wabs, most, c + n, d, BF)
+                assert ((out[b, T - n:].view(n, hq, d).double() - ref).abs() <= tol).all()
+    cache.check_status()

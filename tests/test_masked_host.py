@@ -1,0 +1,339 @@
+"""Work lists and host checks of windowed and tree attention and of the page operators (CPU only)."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from nifre_b200 import Attention, PagedKVCache, _lib
+from nifre_b200.block_allocator import BlockAllocator
+from nifre_b200.block_table import BlockTable
+from nifre_b200.masked import WorkLists, build_lists, mask_words, part_sizes, tree_visibility, virtual_keys
+from oracle.masked import window_seen
+
+
+def _keys_of(lists, g, window, sinks):
+    """The keys that the units of group g read, in order."""
+    _, _, ntok, pos0, ctx, n_draft, _, _ = lists.groups[g].tolist()
+    kept, gap, count = virtual_keys(np.asarray([pos0]), np.asarray([ntok]), window, sinks)
+    return int(kept[0]), int(gap[0]), int(count[0])
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (7, 1), (16, 16), (100, 4), (1000, 40), (1 << 30, 0), (33, 1 << 30)])
+@pytest.mark.parametrize("rows", [(16, 0), (8, 256), (32, 128)])
+def test_units_cover_each_tokens_keys_once(window, sinks, rows):
+    """Every key a token sees is read exactly once by its group's units, every token is in one group, parts are
+    numbered in order, and the merge rows name exactly the tokens with several parts."""
+    rng = np.random.default_rng(window + sinks)
+    S = 9
+    n = rng.integers(1, 90, size=S)
+    n[:3] = 1
+    ctx = rng.integers(0, 700, size=S)
+    ctx[0] = 0
+    slots = rng.permutation(20)[:S]
+    starts = np.cumsum(n) - n + 3
+    unit_rows, item_rows = rows
+    group = 4
+    lists = build_lists(slots, n, starts, ctx, group, unit_rows, item_rows, workers=8, kv_heads=2, window=window,
+                        sinks=sinks, unit_split=64, item_split=256)
+    cover = {}
+    for g, rec in enumerate(lists.groups.tolist()):
+        slot, q0, ntok, pos0, c, nd, _, part0 = rec
+        s = slots.tolist().index(slot)
+        assert c == ctx[s] and nd == n[s] and q0 - starts[s] == pos0 - ctx[s]
+        for t in range(ntok):
+            assert (s, pos0 + t) not in cover
+            cover[(s, pos0 + t)] = g
+    assert len(cover) == n.sum()
+    units = {}
+    for kind, recs in (("unit", lists.units), ("item", lists.items)):
+        for g, k0, k1, pp in recs.tolist():
+            assert k0 % (128 if kind == "item" else 16) == 0 and k0 < k1
+            units.setdefault(g, []).append((pp & 0xffff, k0, k1, pp >> 16, kind))
+    merged = {tuple(r) for r in lists.merge.tolist()}
+    n_merge = 0
+    taken = np.zeros(lists.part_rows, dtype=int)
+    for g, rec in enumerate(lists.groups.tolist()):
+        _, q0, ntok, pos0, c, nd, _, part0 = rec
+        us = sorted(units[g])
+        kept, gap, count = _keys_of(lists, g, window, sinks)
+        assert [u[0] for u in us] == list(range(len(us))) and {u[3] for u in us} == {len(us)}
+        assert us[0][1] == 0 and us[-1][2] == count and all(a[2] == b[1] for a, b in zip(us, us[1:]))
+        limit = item_rows if us[0][4] == "item" else max(unit_rows, group)
+        assert ntok * group <= limit
+        read = [v if v < kept else v + gap for v in range(count)]
+        assert len(set(read)) == len(read)
+        seen = window_seen(int(pos0), int(ntok), window, sinks)
+        assert set(seen.any(0).nonzero().squeeze(1).tolist()) <= set(read)
+        if len(us) > 1:
+            taken[part0:part0 + len(us) * ntok] += 1
+            for t in range(ntok):
+                assert (q0 + t, part0 + t, len(us), ntok) in merged
+                n_merge += 1
+    assert n_merge == len(merged) == len(lists.merge) and (taken == 1).all()
+
+
+def test_tree_lists_carry_every_mask_row():
+    parents = [[-1, 0, 0, 1], [-1] * 40, [-1]]
+    words = [mask_words(tree_visibility(p)) for p in parents]
+    lists = build_lists([2, 0, 1], [4, 40, 1], [0, 4, 44], [100, 0, 5], 8, 16, 0, 8, 1, words=words, unit_split=64)
+    for slot, q0, ntok, pos0, ctx, nd, mask0, _ in lists.groups.tolist():
+        s = [2, 0, 1].index(slot)
+        seen = tree_visibility(parents[s])
+        w = (nd + 31) // 32
+        for t in range(ntok):
+            row = lists.masks[mask0 + t * w: mask0 + (t + 1) * w].astype(np.uint32)
+            bits = [(int(row[j // 32]) >> (j % 32)) & 1 for j in range(nd)]
+            assert bits == seen[pos0 - ctx + t].astype(int).tolist()
+
+
+def test_tree_visibility_and_bits():
+    assert tree_visibility([-1, 0, 1, 0, -1]).astype(int).tolist() == [
+        [1, 0, 0, 0, 0], [1, 1, 0, 0, 0], [1, 1, 1, 0, 0], [1, 0, 0, 1, 0], [0, 0, 0, 0, 1]]
+    for bad in ([0], [-1, 1], [-2], [-1, 0, 5]):
+        with pytest.raises(ValueError, match="parents"):
+            tree_visibility(bad)
+    rng = np.random.default_rng(0)
+    for n in (1, 31, 32, 33, 64, 65):
+        seen = rng.integers(0, 2, size=(n, n)).astype(bool)
+        w = mask_words(seen).astype(np.uint32)
+        assert w.shape == (n, (n + 31) // 32)
+        back = [[(int(w[i, j // 32]) >> (j % 32)) & 1 for j in range(n)] for i in range(n)]
+        assert back == seen.astype(int).tolist()
+
+
+def test_part_sizes_are_even_and_aligned():
+    keys = np.asarray([1, 15, 16, 17, 127, 128, 129, 1000, 100_000])
+    for split, align in ((64, 16), (256, 128)):
+        size = part_sizes(keys, split, align)
+        assert (size % align == 0).all() and (size <= -(-split // align) * align).all()
+        assert (-(-keys // size) * size - keys < size).all()
+
+
+def test_packed_lists_and_room():
+    lists = build_lists([0, 1], [1, 40], [0, 1], [500, 20], 4, 16, 0, 4, 1, window=300, sinks=3, unit_split=64)
+    room = lists.room(lists.sizes())
+    assert all(r >= n and r % 64 == 0 for r, n in zip(room[:6], lists.sizes()[:6]))
+    host = lists.pack(room)
+    at, total = WorkLists.offsets(room)
+    assert len(host) == total and all(a % 4 == 0 for a in at)
+    assert host[:8].tolist() == [len(lists.units), 0, len(lists.merge), 0, 0, 0, 0, 0]
+    assert host[at[1]:at[1] + lists.units.size].tolist() == lists.units.reshape(-1).tolist()
+
+
+def test_too_many_parts_are_refused():
+    with pytest.raises(ValueError, match="parts"):
+        build_lists([0], [1], [0], [40_000 * 16], 1, 16, 0, 1, 1, window=1 << 30, unit_split=16)
+
+
+def test_masked_arguments_struct_matches_the_header(tmp_path):
+    import shutil
+    import subprocess
+    from pathlib import Path
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "nifre_b200.h"', 'int main(void) {',
+             '  printf("%zu %d\\n", sizeof(NfMaskedArgs), NF_MOVE_LIST);']
+    lines += [f'  printf("%zu\\n", offsetof(NfMaskedArgs, {f}));' for f, _ in _lib.NfMaskedArgs._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["  return 0;\n}"]))
+    root = Path(__file__).resolve().parent.parent
+    subprocess.check_call([cc, "-I", str(root / "include"), str(src), "-o", str(exe)])
+    got = [int(x) for x in subprocess.check_output([str(exe)], text=True).split()]
+    assert got == [ctypes.sizeof(_lib.NfMaskedArgs), _lib.MOVE_LIST,
+                   *(getattr(_lib.NfMaskedArgs, f).offset for f, _ in _lib.NfMaskedArgs._fields_)]
+
+
+def _args(**kw):
+    base = dict(out=256, q=256, k_pool=256, v_pool=256, block_tables=256, groups=256, units=256, items=256, merge=256,
+                counts=256, masks=256, mask_words=4, ws=256, ws_rows=4, queue=256, status=256, dtype=2, num_q_heads=8,
+                num_kv_heads=2, head_dim=64, block_size=16, num_blocks=4, num_slots=1, max_blocks_per_seq=4, num_rows=1,
+                max_groups=1, max_units=1, unit_tokens=1, max_items=0, max_merge=0, window=4, sinks=0, scale=1.0)
+    base.update(kw)
+    return _lib.NfMaskedArgs(**base)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(dtype=7), "dtype"), (dict(num_q_heads=7), "multiple"), (dict(num_kv_heads=0), "multiple"),
+    (dict(num_q_heads=1 << 13, num_kv_heads=1), "at most"), (dict(head_dim=257), "head_dim"), (dict(head_dim=0), "head_dim"),
+    (dict(block_size=0), "sizes"), (dict(num_rows=0), "sizes"), (dict(max_units=-1), "work list"),
+    (dict(max_units=0), "work list"), (dict(unit_tokens=0), "unit_tokens"), (dict(unit_tokens=1 << 20), "unit_tokens"),
+    (dict(q=None), "null"), (dict(units=None), "null"), (dict(ws=None), "null"), (dict(status=None), "null"),
+    (dict(q_row_stride=-1), "stride"), (dict(groups=260), "aligned"), (dict(q=257), "aligned"),
+    (dict(window=0), "window"), (dict(sinks=-1), "sinks")])
+def test_window_entry_point_refuses(change, match):
+    """Host-side checks: nothing is launched."""
+    lib = _lib.load()
+    a = _args(**change)
+    assert lib.nf_window_attention(ctypes.addressof(a), None) in (1, 3)
+    assert match in lib.nf_last_error().decode()
+
+
+def test_tree_entry_point_and_limits_refuse():
+    lib = _lib.load()
+    a = _args(masks=None)
+    assert lib.nf_tree_attention(ctypes.addressof(a), None) == 1 and b"mask" in lib.nf_last_error()
+    assert lib.nf_tree_attention(None, None) == 1
+    x, y = ctypes.c_int32(0), ctypes.c_int32(0)
+    assert lib.nf_masked_limits(2, 8, 2, 64, 16, ctypes.byref(x), ctypes.byref(y)) == 0 and x.value >= 4
+    assert lib.nf_masked_limits(2, 8, 3, 64, 16, ctypes.byref(x), ctypes.byref(y)) == 1
+    assert lib.nf_masked_limits(2, 8, 2, 300, 16, ctypes.byref(x), ctypes.byref(y)) == 3
+
+
+def test_move_entry_points_refuse():
+    lib = _lib.load()
+
+    def move(**kw):
+        d = dict(k=256, v=256, ls=0, layers=1, row=16, rows=4, moves=256, n=1, most=1, pos=None, n_pos=0, pos_out=None,
+                 slots=0, dev=1, status=256)
+        d.update(kw)
+        return lib.nf_kv_move(d["k"], d["v"], d["ls"], d["layers"], d["row"], d["rows"], d["moves"], d["n"], d["most"],
+                              d["pos"], d["n_pos"], d["pos_out"], d["slots"], d["dev"], d["status"], None)
+
+    for bad in (dict(k=None), dict(row=0), dict(row=3), dict(layers=0), dict(rows=0), dict(n=-1), dict(moves=None),
+                dict(n_pos=1), dict(k=257), dict(moves=258), dict(dev=0, n=129), dict(status=None)):
+        assert move(**bad) == 1, bad
+    assert move(n=0) == 0
+    rec = np.asarray([[0, 1, 5, 0]], dtype=np.int32)  # more rows than max_rows
+    assert move(dev=0, moves=rec.ctypes.data) == 1 and b"max_rows" in lib.nf_last_error()
+    assert lib.nf_copy_blocks(256, 256, 0, 1, 32, 4, None, None, 1, 256, None) == 1
+    assert lib.nf_copy_blocks(256, 256, 0, 1, 32, 4, None, None, 0, 256, None) == 0
+
+
+def test_attention_window_arguments():
+    with pytest.raises(ValueError, match="sinks need"):
+        Attention(4, 64, sinks=2)
+    for w, s in ((0, 0), (-3, 0), (2.5, 0), (4, -1)):
+        with pytest.raises(ValueError, match="window"):
+            Attention(4, 64, window=w, sinks=s)
+    q = torch.zeros(1, 3, 256)
+    with pytest.raises(ValueError, match="needs a kv_cache"):
+        Attention(4, 64, window=2)(q, q, q)
+
+
+# ---------------------------------------------------------------- block bookkeeping
+def test_allocator_retains_and_releases_many():
+    a, b = BlockAllocator(8), BlockAllocator(8)
+    x, y = a.allocate_many(5), b.allocate_many(5)
+    assert x == y
+    a.retain_many([x[1], x[3]])
+    for i in (x[1], x[3]):
+        b.retain(i)
+    a.release_many([x[3], x[0], x[4]])
+    for i in (x[3], x[0], x[4]):
+        b.release(i)
+    assert a.free_ids() == b.free_ids() and a.allocated_count == b.allocated_count == 3
+    a.release_many([])
+    for bad in ([8], [-1]):
+        with pytest.raises(ValueError, match="out of range"):
+            a.retain_many(bad)
+    with pytest.raises(ValueError, match="not allocated"):
+        a.release_many([x[0]])
+
+
+def test_allocator_compaction():
+    a = BlockAllocator(10)
+    ids = a.allocate_many(7)  # 9 .. 3
+    a.release_many([ids[0], ids[4], ids[5]])  # 9, 5, 4
+    a.retain(8)
+    src, dst = a.compact()
+    assert sorted(src) == [6, 7, 8] and len(set(dst)) == 3 and max(dst) < 4 and 3 not in dst
+    assert [a.refcount(i) for i in range(5)].count(1) == 3 and sorted(a.refcount(i) for i in range(4)) == [1, 1, 1, 2]
+    assert a.refcount(dst[src.index(8)]) == 2
+    assert a.allocate_many(2) == [4, 5] and a.free_count == 4
+    full = BlockAllocator(3)
+    full.allocate_many(3)
+    assert full.compact() == ([], [])
+    assert BlockAllocator(3).compact() == ([], [])
+
+
+def test_table_sharing_shrinking_and_freed_entries():
+    a = BlockAllocator(10)
+    t, u = BlockTable(a, 4), BlockTable(a, 4)
+    t.ensure_capacity(20)
+    blocks = t.physical_blocks()
+    u.share(blocks[:3])
+    assert [a.refcount(b) for b in blocks] == [2, 2, 2, 1, 1]
+    with pytest.raises(ValueError, match="non-empty"):
+        u.share(blocks[:1])
+    e = t.epoch
+    assert t.free_blocks(1, 3) == 2 and t.free_blocks(1, 3) == 0
+    assert t.physical_blocks() == [blocks[0], -1, -1, *blocks[3:]] and a.refcount(blocks[1]) == 1
+    with pytest.raises(IndexError, match="no allocated block"):
+        t.resolve(5)
+    t.shrink(4)
+    assert t.epoch != e and len(t) == 4 and a.refcount(blocks[4]) == 0
+    t.rename(np.asarray([*range(10), -1]))
+    assert t.physical_blocks() == [blocks[0], -1, -1, blocks[3]]
+    t.clear()
+    u.clear()
+    assert a.free_count == 10
+
+
+def test_page_and_plan_refusals_before_any_launch():
+    """Arguments are checked on the host (no CUDA device needed)."""
+    from nifre_b200 import KVCache
+    from types import SimpleNamespace
+    c = PagedKVCache(1, 64, 2, 64, device="cpu", dtype=torch.float16)
+    c.batch_size, c.num_blocks, c._dev_index, c._plan = 4, 8, 0, None
+    c.pos_host = np.asarray([20, 0, 0, 0])
+    c.block_allocator = BlockAllocator(8)
+    c.block_tables = [BlockTable(c.block_allocator, 16) for _ in range(4)]
+    c._init_holes(4)
+    for src, dst, match in (([0], [1, 2], "source slots"), ([0, 0], [1, 1], "distinct"), ([0], [0], "distinct")):
+        with pytest.raises(ValueError, match=match):
+            c.fork(src, dst)
+    with pytest.raises(IndexError, match="out of range"):
+        c.fork([0], [4])
+    for src, dst in (([0], [1, 2]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([8], [0]), ([-1], [0])):
+        with pytest.raises(ValueError):
+            c.copy_blocks(src, dst)
+    with pytest.raises(ValueError, match="int32"):
+        c.copy_blocks(torch.zeros(2), torch.ones(2))
+    with pytest.raises(_lib.NifreError, match="CUDA tensor"):
+        c.copy_blocks(torch.zeros(2, dtype=torch.int32), torch.ones(2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="length"):
+        c.truncate(0, 21)
+    with pytest.raises(ValueError, match="window"):
+        c.free_outside_window(0, 0)
+    plan = SimpleNamespace(closed=False, slots=np.asarray([0]), ctx_before=np.asarray([16]), q_lens=np.asarray([4]), n_seqs=1,
+                           q_heads=4, rows_needed=4, q_starts=np.asarray([0]))
+    with pytest.raises(RuntimeError, match="not finished"):
+        c.keep_tokens(plan, [[0]])
+    plan.closed = True
+    for path in ([1, 1], [2, 1], [-1], [4]):
+        with pytest.raises(ValueError, match="ascending"):
+            c.keep_tokens(plan, [path])
+    with pytest.raises(ValueError, match="paths"):
+        c.keep_tokens(plan, [])
+    plan.ctx_before = np.asarray([10])
+    with pytest.raises(ValueError, match="not the 14"):
+        c.keep_tokens(plan, [[0]])
+    open_plan = SimpleNamespace(closed=False, slots=np.asarray([2]))
+    c._plan = open_plan
+    with pytest.raises(RuntimeError, match="not finished"):
+        c.fork([0], [2])
+    with pytest.raises(RuntimeError, match="not finished"):
+        c.compact()
+    for w, s in ((0, 0), (1.5, 0), (4, -1)):
+        with pytest.raises(ValueError, match="window|sinks"):
+            c.plan_window(plan, w, s)
+    with pytest.raises(ValueError, match="parents or masks"):
+        c.plan_tree(plan)
+    with pytest.raises(ValueError, match="trees for"):
+        c.plan_tree(plan, [])
+    with pytest.raises(ValueError, match="a tree of"):
+        c.plan_tree(plan, [[-1]])
+    with pytest.raises(ValueError, match="q_heads"):
+        c.plan_window(plan, 4, q_heads=3)
+    c._hole_first[0], c._hole_end[0] = 0, 16
+    with pytest.raises(ValueError, match="freed"):
+        c.plan_tree(plan, [[-1, 0, 1, 2]])
+    with pytest.raises(ValueError, match="were freed"):
+        c.plan_window(plan, 100, 0)
+    dense = KVCache(1, 64, 2, 64, device="cpu", dtype=torch.float16)
+    for call in (lambda: dense.fork([0], [1]), dense.compact):
+        with pytest.raises(ValueError, match="dense"):
+            call()
