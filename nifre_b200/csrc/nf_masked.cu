@@ -419,7 +419,8 @@ static int masked_attention(const NfMaskedArgs* a, bool tree, const char* what, 
   if (p.max_items)
     return fail(NF_EUNSUPPORTED, "%s: no tensor-core path for this shape", what);
   if (p.max_units) {
-    switch (a->dtype) {
+    rc = launch_masked_tma(p, a->dtype, stream, what);
+    if (rc == NF_EUNSUPPORTED) switch (a->dtype) {
       case NF_F32: rc = dispatch_vec<float>(p, st, what); break;
       case NF_F16: rc = dispatch_vec<__half>(p, st, what); break;
       default: rc = dispatch_vec<__nv_bfloat16>(p, st, what); break;
@@ -451,7 +452,8 @@ extern "C" int nf_masked_limits(int32_t dtype, int32_t num_q_heads, int32_t num_
   if (head_dim <= 0 || head_dim > 256) return fail(NF_EUNSUPPORTED, "nf_masked_limits: head_dim %d (1 to 256)", head_dim);
   if (block_size <= 0) return fail(NF_EINVAL, "nf_masked_limits: block_size must be positive");
   const int G = num_q_heads / num_kv_heads;
-  *unit_rows = G > kVecRows ? G : kVecRows;
+  *unit_rows = masked_tma_rows(dtype, num_q_heads, num_kv_heads, head_dim, block_size);
+  if (!*unit_rows) *unit_rows = G > kVecRows ? G : kVecRows;
   *item_rows = 0;
   return ok();
 }

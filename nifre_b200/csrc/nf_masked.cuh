@@ -121,11 +121,9 @@ __device__ __forceinline__ float* part_record(const MaskedParams& p, long long r
   return p.ws + (row * p.Hq + head) * p.DP;
 }
 
-// The tensor-core and tensor-map paths (NF_EUNSUPPORTED: not for this shape).
-int launch_masked_tma(const MaskedParams& p, int dtype, void* stream);
-int launch_masked_tc(const MaskedParams& p, int dtype, void* stream);
-// Largest groups of each path for a shape, in query rows (0: no such path).
+// The tensor-map path (NF_EUNSUPPORTED, nothing launched: not for this shape).
+int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char* what);
+// Largest group for a shape, in query rows (0: no such path).
 int masked_tma_rows(int dtype, int Hq, int Hkv, int D, int bs);
-int masked_tc_rows(int dtype, int Hq, int Hkv, int D, int bs);
 
 }  // namespace nf

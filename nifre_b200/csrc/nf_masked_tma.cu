@@ -1,0 +1,573 @@
+// Windowed and tree attention of groups of few query rows (decodes, short
+// drafts), for 16-bit pools with head_dim 64 or 128 and a block size that is
+// a multiple of 16.  Bound by the key and value bytes.
+//
+// A CTA owns HG KV heads.  Its producer thread takes (unit, head group) pairs
+// from a queue and issues, for each 16-key step of a unit, one tensor copy for
+// K and one for V: 16 tokens of one block x HG heads x head_dim, landing
+// head-major and 128-byte swizzled.  Steps skip the gap between a window's
+// sinks and its last keys, so a group reads its visible keys (rounded to 16)
+// and no others.  Consumer warp h computes KV head h for all of the group's
+// columns (token x query head) at once: S^T = K Q^T and O^T += V^T P^T with
+// mma.sync m16n8k16, the columns as NT tiles of 8, so K and V are read once
+// whatever the number of drafted tokens.  (tcgen05 needs 64 rows or more; a
+// group has at most 32, larger ones go to nf_masked_tc.cu.)
+//
+// Only steps that some column does not wholly see apply the mask.  There the
+// weights of unseen keys are 0; as 0 * NaN would still reach the sum, such a
+// step looks its value rows over and, where they hold anything not finite,
+// adds the seen rows one by one instead.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "nf_internal.h"
+#include "nf_masked.cuh"
+#include "nf_tma.cuh"
+
+namespace nf {
+
+constexpr int kMtHeader = 1024;
+constexpr int kMtMaxStages = 8;
+
+// One 16-key step as the producer describes it to the consumers; the unit's
+// fields (from slot on) are set on its first step only.
+struct __align__(16) MtStep {
+  int u, key0, nv, flags;  // u < 0: no more work; first key, keys before the unit's end, kMt* bits
+  int q_row0, ntok, pos0, ctx;
+  int n_draft, mask0, part_row0, part;  // part: part | n_parts << 16
+  int hg, pad0, pad1, pad2;
+};
+constexpr int kMtFirst = 1, kMtLast = 2, kMtMasked = 4;
+
+struct MtLaunch {
+  int HG, n_hg, stages, stage_bytes, box_bytes, one_box, evict_first, q_align4;
+};
+
+// Byte offset of key row r, 16-byte chunk c, in one head's staged tile.
+__device__ __forceinline__ int mt_off(int r, int c) {
+  return (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+template <int D_>
+__device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUtensorMap* tk, const CUtensorMap* tv,
+                            unsigned char* base, int total) {
+  constexpr int NDH = D_ / 64;
+  const uint32_t hdr = smem_u32(base);
+  auto full = [&](int s) { return hdr + 8 * s; };
+  auto empty = [&](int s) { return hdr + 64 + 8 * s; };
+  MtStep* recs = reinterpret_cast<MtStep*>(base + 128);
+  const uint32_t stage0 = hdr + kMtHeader;
+  // the switch to the next unit needs four dependent round trips (ticket,
+  // unit, group, block id): each is asked for kGap steps after the one before
+  constexpr int kGap = 2, kAhead = 4 * kGap;
+  const uint64_t pol = L.evict_first ? l2_evict_first() : l2_evict_last();
+  const int4* units = reinterpret_cast<const int4*>(p.units);
+  int k = 0, s = 0;
+  uint32_t pe = 1;
+  bool ok = true;
+  int w = blockIdx.x;
+  int4 un = make_int4(0, 0, 0, 0);
+  MaskedGroup g{};
+  bool good = false;
+  auto fetch_group = [&](const int4& unit, MaskedGroup& gr) {
+    const bool in = unit.x >= 0 && unit.x < p.max_groups;
+    if (in) gr = load_group(p, unit.x);
+    return in;
+  };
+  if (w < total) {
+    un = __ldg(units + w / L.n_hg);
+    good = fetch_group(un, g);
+  }
+  pdl_wait();
+  while (w < total) {
+    const int u = w / L.n_hg, hg = w - u * L.n_hg, h0 = hg * L.HG;
+    if (!good || !group_ok(p, g)) {
+      atomicOr(p.status, good ? NF_STATUS_BAD_SLOT : NF_STATUS_UNIT_OVERFLOW);
+      w = (int)gridDim.x + atomicAdd(p.queue, 1);
+      if (w < total) {
+        un = __ldg(units + w / L.n_hg);
+        good = fetch_group(un, g);
+      }
+      continue;
+    }
+    const VirtualKeys vk(p, g);
+    const int v1 = min(un.z, vk.end);
+    const int* btrow = p.bt + (long long)g.slot * p.max_blocks;
+    const int nsteps = max(1, (v1 - un.y + 15) >> 4);  // (a unit without keys still ends in an epilogue)
+    const int ask = nsteps - 1 - min(kAhead, nsteps - 1);
+    int wn = total;
+    int4 nu = make_int4(0, 0, 0, 0);
+    MaskedGroup ng{};
+    bool ngood = false;
+    int have = 0;  // what is known of the next unit: 1 ticket, 2 unit, 3 group
+    for (int i = 0, v = un.y; i < nsteps; ++i, v += 16, ++k) {
+      if (i == ask) {
+        wn = (int)gridDim.x + atomicAdd(p.queue, 1);
+        have = 1;
+      } else if (i == ask + kGap && wn < total) {
+        nu = __ldg(units + wn / L.n_hg);
+        have = 2;
+      } else if (i == ask + 2 * kGap && wn < total) {
+        ngood = fetch_group(nu, ng);
+        have = 3;
+      } else if (i == ask + 3 * kGap && wn < total && ngood && ng.slot >= 0 && ng.slot < p.num_slots) {
+        const int lb = VirtualKeys(p, ng).key(nu.y) / p.bs;
+        if (lb >= 0 && lb < p.max_blocks)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(p.bt + (long long)ng.slot * p.max_blocks + lb));
+      }
+      if (!mbar_wait(empty(s), pe, p.status)) {
+        ok = false;
+        break;
+      }
+      const int key0 = vk.key(v), key1 = key0 + 15, last_pos = g.pos0 + g.ntok - 1;
+      const int lb = key0 / p.bs;
+      int phys = lb < p.max_blocks ? __ldg(btrow + lb) : -1;
+      // a block that is not there: nothing of it is seen (nv 0 on a masked step), and block 0 stands in
+      const bool bad = phys < 0 || phys >= p.num_blocks;
+      if (bad) {
+        atomicOr(p.status, NF_STATUS_BAD_BLOCK);
+        phys = 0;
+      }
+      const int nv = bad ? 0 : max(0, min(16, v1 - v));
+      const bool whole = nv == 16 && (p.tree ? key1 < g.ctx
+                                             : key1 <= g.pos0 && (key0 > last_pos - p.window || key1 < p.sinks));
+      MtStep& r = recs[s];
+      *reinterpret_cast<int4*>(&r) =
+          make_int4(u, key0, nv, (i == 0 ? kMtFirst : 0) | (i == nsteps - 1 ? kMtLast : 0) | (whole ? 0 : kMtMasked));
+      if (i == 0) {
+        reinterpret_cast<int4*>(&r)[1] = make_int4(g.q_row0, g.ntok, g.pos0, g.ctx);
+        reinterpret_cast<int4*>(&r)[2] = make_int4(g.n_draft, g.mask0, g.part_row0, un.w);
+        r.hg = hg;
+      }
+      const int off = key0 - lb * p.bs;
+      const uint32_t sb = stage0 + s * L.stage_bytes;
+      mbar_arrive_expect_tx(full(s), 2 * L.box_bytes);
+      if (L.one_box) {
+        if constexpr (D_ == 64) {
+          tma_load_4d(sb, tk, 0, off, h0, phys, full(s), pol);
+          tma_load_4d(sb + L.box_bytes, tv, 0, off, h0, phys, full(s), pol);
+        } else {
+          tma_load_5d(sb, tk, 0, off, 0, h0, phys, full(s), pol);
+          tma_load_5d(sb + L.box_bytes, tv, 0, off, 0, h0, phys, full(s), pol);
+        }
+      } else {
+        for (int h = 0; h < L.HG; ++h)
+#pragma unroll
+          for (int dh = 0; dh < NDH; ++dh) {
+            const uint32_t d = sb + (h * NDH + dh) * 2048;
+            if constexpr (D_ == 64) {
+              tma_load_4d(d, tk, 0, h0 + h, off, phys, full(s), pol);
+              tma_load_4d(d + L.box_bytes, tv, 0, h0 + h, off, phys, full(s), pol);
+            } else {
+              tma_load_5d(d, tk, 0, dh, h0 + h, off, phys, full(s), pol);
+              tma_load_5d(d + L.box_bytes, tv, 0, dh, h0 + h, off, phys, full(s), pol);
+            }
+          }
+      }
+      if (++s == L.stages) {
+        s = 0;
+        pe ^= 1;
+      }
+    }
+    if (!ok) break;
+    if (wn < total) {  // a short unit: what the steps did not get to
+      if (have < 2) nu = __ldg(units + wn / L.n_hg);
+      if (have < 3) ngood = fetch_group(nu, ng);
+    }
+    w = wn;
+    un = nu;
+    g = ng;
+    good = ngood;
+  }
+  if (ok && mbar_wait(empty(s), pe, p.status)) {
+    recs[s].u = -1;
+    mbar_arrive(full(s));
+    return;
+  }
+  // a wait ran out: leave no copy in flight into this CTA's shared memory
+  for (int j = max(0, k - L.stages); j < k; ++j) mbar_wait(full(j % L.stages), (j / L.stages) & 1, p.status);
+}
+
+// A unit as its consumer warp holds it, and the running state of NT tiles of
+// 8 columns: column c = 8 j + 2 (lane % 4) (+1) of token c / G.
+template <int D_, int NT>
+struct MtState {
+  static constexpr int KS = D_ / 16;
+  uint32_t qf[NT][KS][2];
+  float m[NT][2], l[NT][2];
+  float o[KS][NT][4];
+};
+
+// PT staged 16-key tiles of this warp's head in one update.
+template <typename T, int D_, int NT, int PT>
+__device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGroup& g, const uint32_t (&kb)[PT],
+                                          const uint32_t (&vb)[PT], const int (&key0)[PT], const int (&nv)[PT],
+                                          int masked, MtState<D_, NT>& st) {
+  constexpr int KS = D_ / 16;
+  const int lane = threadIdx.x & 31, tq = lane >> 2, n0 = 2 * (lane & 3);
+  const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;
+  const int vr = (lane & 7) + ((lane >> 4) & 1) * 8, vc = (lane >> 3) & 1;
+  float x[PT][NT][4];
+#pragma unroll
+  for (int t = 0; t < PT; ++t) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) x[t][j][0] = x[t][j][1] = x[t][j][2] = x[t][j][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t a0, a1, a2, a3;
+      ldsm_x4(kb[t] + mt_off(kr, 2 * ks + kc), a0, a1, a2, a3);
+#pragma unroll
+      for (int j = 0; j < NT; ++j) mma16816<T>(x[t][j], a0, a1, a2, a3, st.qf[j][ks][0], st.qf[j][ks][1]);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][j][e] *= p.scale_log2;
+    if (masked >> t & 1) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = tq + (e >> 1) * 8, tok = min((8 * j + n0 + (e & 1)) / p.G, g.ntok - 1);
+          if (row >= nv[t] || !sees(p, g, tok, key0[t] + row)) x[t][j][e] = -INFINITY;
+        }
+    }
+  }
+  float mx[NT][2];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    mx[j][0] = fmaxf(x[0][j][0], x[0][j][2]);
+    mx[j][1] = fmaxf(x[0][j][1], x[0][j][3]);
+#pragma unroll
+    for (int t = 1; t < PT; ++t) {
+      mx[j][0] = fmaxf(mx[j][0], fmaxf(x[t][j][0], x[t][j][2]));
+      mx[j][1] = fmaxf(mx[j][1], fmaxf(x[t][j][1], x[t][j][3]));
+    }
+  }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      mx[j][0] = fmaxf(mx[j][0], __shfl_xor_sync(0xffffffffu, mx[j][0], o));
+      mx[j][1] = fmaxf(mx[j][1], __shfl_xor_sync(0xffffffffu, mx[j][1], o));
+    }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const float mn0 = fmaxf(st.m[j][0], mx[j][0]), mn1 = fmaxf(st.m[j][1], mx[j][1]);
+    const float b0 = mn0 == -INFINITY ? 0.f : mn0, b1 = mn1 == -INFINITY ? 0.f : mn1;
+    const float al0 = ex2(st.m[j][0] - b0), al1 = ex2(st.m[j][1] - b1);
+    st.m[j][0] = mn0;
+    st.m[j][1] = mn1;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int t = 0; t < PT; ++t) {
+      x[t][j][0] = ex2(x[t][j][0] - b0);
+      x[t][j][1] = ex2(x[t][j][1] - b1);
+      x[t][j][2] = ex2(x[t][j][2] - b0);
+      x[t][j][3] = ex2(x[t][j][3] - b1);
+      s0 += x[t][j][0] + x[t][j][2];
+      s1 += x[t][j][1] + x[t][j][3];
+    }
+    st.l[j][0] = st.l[j][0] * al0 + s0;
+    st.l[j][1] = st.l[j][1] * al1 + s1;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      st.o[i][j][0] *= al0;
+      st.o[i][j][1] *= al1;
+      st.o[i][j][2] *= al0;
+      st.o[i][j][3] *= al1;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < PT; ++t) {
+    bool plain = true;
+    if (masked >> t & 1) {
+      // anything not finite among the value rows? (all exponent bits set, either half of a word)
+      constexpr uint32_t EX = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+      bool odd = false;
+      for (int c = lane; c < 16 * D_ / 8; c += 32) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(vb[t] + c * 16));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= (w[e] & EX) == EX || ((w[e] >> 16) & EX) == EX;
+      }
+      plain = !__any_sync(0xffffffffu, odd);
+    }
+    if (plain) {
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        pb[j][0] = movmatrix_t(pack2<T>(x[t][j][0], x[t][j][1]));
+        pb[j][1] = movmatrix_t(pack2<T>(x[t][j][2], x[t][j][3]));
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        uint32_t a0, a1, a2, a3;
+        ldsm_x4_t(vb[t] + mt_off(vr, 2 * i + vc), a0, a1, a2, a3);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mma16816<T>(st.o[i][j], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+      }
+    } else {
+      for (int row = 0; row < 16; ++row) {
+        const int src = (row & 7) * 4 + (lane & 3);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float lo0 = __shfl_sync(0xffffffffu, x[t][j][0], src), lo1 = __shfl_sync(0xffffffffu, x[t][j][1], src);
+          const float hi0 = __shfl_sync(0xffffffffu, x[t][j][2], src), hi1 = __shfl_sync(0xffffffffu, x[t][j][3], src);
+          const float w0 = row < 8 ? lo0 : hi0, w1 = row < 8 ? lo1 : hi1;
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int d = 16 * i + tq + 8 * h;
+              unsigned short b;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(vb[t] + mt_off(row, d >> 3) + (d & 7) * 2));
+              const float v = Elem<T>::to_f(*reinterpret_cast<T*>(&b));
+              if (w0 != 0.f) st.o[i][j][2 * h] = fmaf(w0, v, st.o[i][j][2 * h]);
+              if (w1 != 0.f) st.o[i][j][2 * h + 1] = fmaf(w1, v, st.o[i][j][2 * h + 1]);
+            }
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int D_, int NT>
+__device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned char* base) {
+  constexpr int KS = D_ / 16, NDH = D_ / 64;
+  constexpr bool kPairs = NT == 1 && D_ == 64;  // two steps an update where one has little to do
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tq = lane >> 2, n0 = 2 * (lane & 3);
+  const uint32_t hdr = smem_u32(base);
+  const MtStep* recs = reinterpret_cast<const MtStep*>(base + 128);
+  const uint32_t stage0 = hdr + kMtHeader;
+  const int head_region = warp * NDH * 2048;
+  MtState<D_, NT> st;
+  MaskedGroup g{};
+  int part = 0, kvh = 0;
+  int s = 0;
+  uint32_t ph = 0;
+  pdl_wait();  // the queries may come from the launch before this one
+  for (;;) {
+    if (!mbar_wait(hdr + 8 * s, ph, p.status)) return;
+    const int4 r = *reinterpret_cast<const int4*>(recs + s);
+    if (r.x < 0) return;
+    const int s0 = s;
+    if (r.w & kMtFirst) {
+      const int4 a = reinterpret_cast<const int4*>(recs + s)[1], b = reinterpret_cast<const int4*>(recs + s)[2];
+      g = MaskedGroup{0, a.x, a.y, a.z, a.w, b.x, b.y, b.z};
+      part = b.w;
+      kvh = recs[s].hg * L.HG + warp;
+      const int cols = g.ntok * p.G;
+      // the group's queries, straight into the B operand's layout: column 8 j + lane / 4, elements
+      // 16 ks + 2 (lane % 4) (+1) and 8 further (once a unit, while the ring fills)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int c = 8 * j + tq, tok = c / p.G;
+        const T* q = reinterpret_cast<const T*>(p.q) + (long long)(g.q_row0 + tok) * p.q_stride +
+                     (long long)(kvh * p.G + (c - tok * p.G)) * D_ + n0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t v = 0;
+            if (c < cols) {
+              const T* e = q + 16 * ks + 8 * h;
+              if (L.q_align4) {
+                v = *reinterpret_cast<const uint32_t*>(e);
+              } else {
+                v = *reinterpret_cast<const unsigned short*>(e) |
+                    (uint32_t)*reinterpret_cast<const unsigned short*>(e + 1) << 16;
+              }
+            }
+            st.qf[j][ks][h] = v;
+          }
+        st.m[j][0] = st.m[j][1] = -INFINITY;
+        st.l[j][0] = st.l[j][1] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) st.o[i][j][0] = st.o[i][j][1] = st.o[i][j][2] = st.o[i][j][3] = 0.f;
+    }
+    if (++s == L.stages) {
+      s = 0;
+      ph ^= 1;
+    }
+    bool last = r.w & kMtLast;
+    const uint32_t sb0 = stage0 + s0 * L.stage_bytes;
+    if (kPairs && !last) {
+      if (!mbar_wait(hdr + 8 * s, ph, p.status)) return;
+      const int4 r1 = *reinterpret_cast<const int4*>(recs + s);
+      const int s1 = s;
+      const uint32_t sb1 = stage0 + s1 * L.stage_bytes;
+      if (++s == L.stages) {
+        s = 0;
+        ph ^= 1;
+      }
+      last = r1.w & kMtLast;
+      const uint32_t kb[2] = {sb0 + head_region, sb1 + head_region};
+      const uint32_t vb[2] = {kb[0] + L.box_bytes, kb[1] + L.box_bytes};
+      const int key0[2] = {r.y, r1.y}, nv[2] = {r.z, r1.z};
+      mt_update<T, D_, NT, 2>(p, g, kb, vb, key0, nv, (r.w & kMtMasked ? 1 : 0) | (r1.w & kMtMasked ? 2 : 0), st);
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(hdr + 64 + 8 * s0);
+        mbar_arrive(hdr + 64 + 8 * s1);
+      }
+    } else {
+      const uint32_t kb[1] = {sb0 + head_region}, vb[1] = {kb[0] + L.box_bytes};
+      const int key0[1] = {r.y}, nv[1] = {r.z};
+      mt_update<T, D_, NT, 1>(p, g, kb, vb, key0, nv, r.w & kMtMasked ? 1 : 0, st);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(hdr + 64 + 8 * s0);
+    }
+    if (!last) continue;
+    const int cols = g.ntok * p.G, n_parts = part >> 16;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l = st.l[j][e];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const int c = 8 * j + n0 + e;
+        if (c >= cols) continue;
+        const int tok = c / p.G, head = kvh * p.G + (c - tok * p.G);
+        if (n_parts == 1) {
+          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+          T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride + (long long)head * D_ + tq;
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            dst[16 * i] = Elem<T>::from_f(st.o[i][j][e] * inv);
+            dst[16 * i + 8] = Elem<T>::from_f(st.o[i][j][2 + e] * inv);
+          }
+        } else {
+          const long long row = (long long)g.part_row0 + (long long)(part & 0xffff) * g.ntok + tok;
+          if (g.part_row0 < 0 || row >= p.ws_rows) {
+            atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
+            continue;
+          }
+          float* rec = part_record(p, row, head);
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            __stcg(rec + 16 * i + tq, st.o[i][j][e]);
+            __stcg(rec + 16 * i + tq + 8, st.o[i][j][2 + e]);
+          }
+          if (tq == 0) __stcg(reinterpret_cast<float2*>(rec + D_), make_float2(st.m[j][e], l));
+        }
+      }
+  }
+}
+
+template <typename T, int D_, int NT>
+__global__ void __launch_bounds__(D_ == 64 ? 288 : 160, D_ == 64 ? 1 : 2)
+    masked_tma_kernel(const MaskedParams p, const MtLaunch L, const __grid_constant__ CUtensorMap tk,
+                      const __grid_constant__ CUtensorMap tv) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* base =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  if (threadIdx.x == 32 * L.HG) {
+    tma_prefetch_map(&tk);
+    tma_prefetch_map(&tv);
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L.stages; ++s) {
+      mbar_init(smem_u32(base) + 8 * s, 1);
+      mbar_init(smem_u32(base) + 64 + 8 * s, L.HG);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  const int total = min(__ldg(p.counts), p.max_units) * L.n_hg;
+  if (warp < L.HG)
+    mt_consumer<T, D_, NT>(p, L, base);
+  else if ((threadIdx.x & 31) == 0)
+    mt_producer<D_>(p, L, &tk, &tv, base, total);
+  __syncthreads();
+  // the last CTA out rewinds the queue (every ticket of every CTA is taken)
+  if (threadIdx.x == 0 && atomicAdd(p.queue + 1, 1) == (int)gridDim.x - 1) {
+    p.queue[0] = 0;
+    p.queue[1] = 0;
+    __threadfence();
+  }
+}
+
+// Query rows of a group: 32 columns of a 64-wide head fit a warp's registers
+// (accumulators 64, queries 32 of them), 16 of a 128-wide one.
+int masked_tma_rows(int dtype, int Hq, int Hkv, int D, int bs) {
+  if (dtype != NF_BF16 && dtype != NF_F16) return 0;
+  if ((D != 64 && D != 128) || bs % 16) return 0;
+  const int rows = D == 64 ? 32 : 16;
+  return Hq / Hkv <= rows ? rows : 0;
+}
+
+int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char* what) {
+  if (!masked_tma_rows(dtype, p.Hq, p.Hkv, p.D, p.bs)) return NF_EUNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(p.kp) | reinterpret_cast<uintptr_t>(p.vp)) & 15) return NF_EUNSUPPORTED;
+  if (p.unit_tokens * p.G > masked_tma_rows(dtype, p.Hq, p.Hkv, p.D, p.bs)) return NF_EUNSUPPORTED;
+  // as many KV heads a CTA as eight warps an SM take; the rest of the SM goes to stages (32 KB each, about
+  // 220 KB in flight an SM)
+  const int max_hg = p.D == 64 ? 8 : 4;
+  int hg = 1;
+  for (int h = p.Hkv < max_hg ? p.Hkv : max_hg; h > 1; --h)
+    if (p.Hkv % h == 0) {
+      hg = h;
+      break;
+    }
+  MtLaunch L;
+  L.HG = hg;
+  L.n_hg = p.Hkv / hg;
+  L.box_bytes = hg * 16 * p.D * 2;
+  L.stage_bytes = 2 * L.box_bytes;
+  const int want = (p.D == 64 ? 1 : 2) * (max_hg / hg);
+  int stages = (228 * 1024 / want - 1024 - kMtHeader - 1024) / L.stage_bytes;
+  L.stages = stages > kMtMaxStages ? kMtMaxStages : stages;
+  if (L.stages < 2) return NF_EUNSUPPORTED;
+  CUtensorMap tk, tv;
+  L.one_box = encode_pool_map(&tk, p.kp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, hg, true) &&
+              encode_pool_map(&tv, p.vp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, hg, true);
+  if (!L.one_box && !(encode_pool_map(&tk, p.kp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, hg, false) &&
+                      encode_pool_map(&tv, p.vp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, hg, false)))
+    return NF_EUNSUPPORTED;
+  L.evict_first = 1;
+  L.q_align4 = (reinterpret_cast<uintptr_t>(p.q) % 4 == 0) && p.q_stride % 2 == 0;
+  const int cols = p.unit_tokens * p.G;
+  using Kern = void (*)(const MaskedParams, const MtLaunch, const CUtensorMap, const CUtensorMap);
+  Kern kern;
+  if (dtype == NF_BF16) {
+    using T = __nv_bfloat16;
+    kern = p.D == 64 ? (cols <= 8 ? masked_tma_kernel<T, 64, 1> : cols <= 16 ? masked_tma_kernel<T, 64, 2>
+                                                                             : masked_tma_kernel<T, 64, 4>)
+                     : (cols <= 8 ? masked_tma_kernel<T, 128, 1> : masked_tma_kernel<T, 128, 2>);
+  } else {
+    using T = __half;
+    kern = p.D == 64 ? (cols <= 8 ? masked_tma_kernel<T, 64, 1> : cols <= 16 ? masked_tma_kernel<T, 64, 2>
+                                                                             : masked_tma_kernel<T, 64, 4>)
+                     : (cols <= 8 ? masked_tma_kernel<T, 128, 1> : masked_tma_kernel<T, 128, 2>);
+  }
+  const int threads = (hg + 1) * 32, smem = kMtHeader + L.stages * L.stage_bytes + 1024;
+  int per_sm = 1;
+  cudaError_t e = prepare_launch(reinterpret_cast<const void*>(kern), smem, threads, &per_sm);
+  if (e != cudaSuccess) return fail(NF_ECUDA, "%s: smem attribute: %s", what, cudaGetErrorString(e));
+  long long grid = (long long)sm_count() * per_sm;
+  const long long need = (long long)p.max_units * L.n_hg;
+  if (need < grid) grid = need;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, p, L, tk, tv);
+  if (e != cudaSuccess) return fail(NF_ECUDA, "%s: launch: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+}  // namespace nf

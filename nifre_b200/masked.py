@@ -303,8 +303,10 @@ class MaskedAttentionOps:
 
     @property
     def masked_workers(self) -> int:
-        """Workers the masked kernels' units are sized for: one per SM."""
-        return self.sm_count
+        """Units at work at once that a step's keys are cut for: the tensor-map kernel keeps eight KV heads an SM on
+        the go, the per-warp kernel (other types and shapes) about 32."""
+        heads = 8 if self.dtype != torch.float32 and self.head_dim in (64, 128) and self.block_size % 16 == 0 else 32
+        return max(1, self.sm_count * heads // self.n_heads)
 
     def window_attention_step(self, layer_id: int, q: torch.Tensor, view: MaskedPlan, out: torch.Tensor,
                               scale: float | None = None) -> torch.Tensor:
