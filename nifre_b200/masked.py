@@ -52,10 +52,34 @@ def virtual_keys(pos0, ntok, window: int, sinks: int):
     return kept, gap, pos0 + ntok - gap
 
 
-def part_sizes(keys, split: int, align: int):
-    """Keys per part of each group, a multiple of ``align``: equal parts of at most about ``split`` keys."""
-    parts = np.maximum(1, -(-keys // split))
-    return np.maximum(align, -(-keys // (parts * align)) * align)
+def even_shares(keys, share: int, align: int, least: int):
+    """Cut groups of ``keys`` keys into units by laying them end to end and cutting every ``share`` keys (then every
+    worker's share is one or two units, whatever the groups' lengths, and no group has more parts than it needs).
+
+    Cuts sit at multiples of ``align`` of their group and at least ``least``
+    keys from its ends.  Returns per unit (group, first key, end), in order.
+    """
+    keys = np.asarray(keys, dtype=np.int64)
+    end = np.cumsum(keys)
+    start = end - keys
+    cuts = np.arange(share, int(end[-1]), share) if len(keys) else np.zeros(0, dtype=np.int64)
+    g = np.searchsorted(end, cuts, side="right")
+    at = (cuts - start[g] + align // 2) // align * align
+    keep = (at >= least) & (keys[g] - at >= least)
+    g, at = g[keep], at[keep]
+    group = np.concatenate([np.arange(len(keys)), g])
+    first = np.concatenate([np.zeros(len(keys), dtype=np.int64), at])
+    order = np.lexsort((first, group))
+    group, first = group[order], first[order]
+    distinct = np.ones(len(group), dtype=bool)
+    distinct[1:] = (group[1:] != group[:-1]) | (first[1:] != first[:-1])
+    group, first = group[distinct], first[distinct]
+    last = np.ones(len(group), dtype=bool)
+    last[:-1] = group[1:] != group[:-1]
+    stop = np.empty_like(first)
+    stop[:-1] = first[1:]
+    stop[last] = keys[group[last]]
+    return group, first, stop
 
 
 class WorkLists:
@@ -93,7 +117,7 @@ class WorkLists:
 
 
 def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_rows: int, workers: int, kv_heads: int,
-                window=None, sinks: int = 0, words=None, unit_split=None, item_split=None) -> WorkLists:
+                window=None, sinks: int = 0, words=None, unit_share=None, item_share=None) -> WorkLists:
     """Work lists of a step whose sequences get ``q_lens`` new tokens behind ``ctx`` cached ones.
 
     ``window``/``sinks``, or ``words``: each sequence's mask rows (``mask_words``).
@@ -121,30 +145,30 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
         mask0 = start[:-1][seq] + tok0 * np.asarray([w.shape[1] for w in words], dtype=np.int64)[seq]
         masks = np.concatenate([w.reshape(-1) for w in words])
     on_items = routed[seq]
-    size = np.zeros(len(seq), dtype=np.int64)
-    if (~on_items).any():
-        k = keys[~on_items]
-        split = unit_split or unit_split_for(k, workers)
-        size[~on_items] = part_sizes(k, split, 16)
-    if on_items.any():
-        k = keys[on_items]
-        split = item_split or item_split_for(k, workers, kv_heads)
-        size[on_items] = part_sizes(k, split, 128)
-    parts = -(-keys // size)
-    if parts.size and parts.max() > MAX_PARTS:
+    cuts = []  # (group, first key, end) of every unit and of every item
+    for on, share, align, share_for in ((~on_items, unit_share, 16, unit_share_for),
+                                        (on_items, item_share, 128, item_share_for)):
+        mine = np.flatnonzero(on)
+        g, k0, k1 = even_shares(keys[mine], share or share_for(keys[mine], workers, kv_heads), align, 4 * align) \
+            if len(mine) else (mine, mine, mine)
+        cuts.append((mine[g], k0, k1))
+    parts = np.zeros(len(seq), dtype=np.int64)
+    for g, _, _ in cuts:
+        parts += np.bincount(g, minlength=len(seq))
+    if parts.max() > MAX_PARTS:
         raise ValueError(f"a sequence's keys are cut into {int(parts.max())} parts, at most {MAX_PARTS}")
     rows = np.where(parts > 1, parts * ntok, 0)
     part0 = np.cumsum(rows) - rows
     groups = np.stack([slots[seq], q_starts[seq] + tok0, ntok, pos0, ctx[seq], q_lens[seq], mask0, part0], axis=1)
-    if groups.size and groups.max() >= 1 << 31:
+    if groups.max() >= 1 << 31:
         raise ValueError("the step's work lists exceed 32-bit indices")
 
-    def cut(sel):
-        """Units of the groups in sel, the largest first (a queue over the list then ends on short ones)."""
-        g = np.repeat(sel, parts[sel])
-        j = np.arange(len(g)) - np.repeat(np.cumsum(parts[sel]) - parts[sel], parts[sel])
-        k0 = j * size[g]
-        k1 = np.minimum(keys[g], k0 + size[g])
+    def listed(g, k0, k1):
+        """Unit records, the largest first (a queue over the list then ends on short ones)."""
+        first = np.zeros(len(seq), dtype=np.int64)
+        n = np.bincount(g, minlength=len(seq))
+        first[:] = np.cumsum(n) - n
+        j = np.arange(len(g)) - first[g]
         u = np.stack([g, k0, k1, j | parts[g] << 16], axis=1)
         return u[np.argsort(k0 - k1, kind="stable")].astype(np.int32)
 
@@ -152,16 +176,19 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
     m = np.repeat(split_groups, ntok[split_groups])
     t = np.arange(len(m)) - np.repeat(np.cumsum(ntok[split_groups]) - ntok[split_groups], ntok[split_groups])
     merge = np.stack([groups[m, 1] + t, part0[m] + t, parts[m], ntok[m]], axis=1).astype(np.int32)
-    return WorkLists(groups.astype(np.int32), cut(np.flatnonzero(~on_items)), cut(np.flatnonzero(on_items)), merge,
+    return WorkLists(groups.astype(np.int32), listed(*cuts[0]), listed(*cuts[1]), merge,
                      int(rows.sum()), int(ntok[~on_items].max()) if (~on_items).any() else 0, masks)
 
 
-def unit_split_for(keys: np.ndarray, workers: int) -> int:
-    """Keys per unit: about four units per worker, at least 64 keys each."""
-    return max(64, -(-int(keys.sum()) // (4 * workers * 16)) * 16)
+def unit_share_for(keys: np.ndarray, workers: int, kv_heads: int) -> int:
+    """Keys per unit: one share a worker (a partial row costs about as much as 4 keys to write and merge), up to four
+    where shares stay at 512 keys or more (then the queue evens out the workers' speeds); 64 keys at least."""
+    total = int(keys.sum())
+    waves = min(4, max(1, total // (workers * 512)))
+    return max(64, -(-total // (workers * waves * 16)) * 16)
 
 
-def item_split_for(keys: np.ndarray, workers: int, kv_heads: int) -> int:
+def item_share_for(keys: np.ndarray, workers: int, kv_heads: int) -> int:
     """Keys per tensor-core item (one per KV head): one item per worker, at least 256 keys each."""
     want = max(1, int(keys.sum()) * kv_heads // workers)
     return max(256, -(-want // 128) * 128)

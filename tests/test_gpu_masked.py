@@ -213,10 +213,10 @@ def test_values_of_unseen_keys_do_not_matter(shape):
 def test_keys_split_into_many_parts(shape, monkeypatch):
     from nifre_b200 import masked, tree_visibility
     hq, hkv, d, bs, dtype = shape
-    monkeypatch.setattr(masked, "unit_split_for", lambda *a: 16)
-    monkeypatch.setattr(masked, "item_split_for", lambda *a: 128)
+    monkeypatch.setattr(masked, "unit_share_for", lambda *a: 64)
+    monkeypatch.setattr(masked, "item_share_for", lambda *a: 512)
     n = [1, 3, 48]
-    st = Step([1300, 650, 500], n, hq, hkv, d, bs, dtype, seed=7, pad=1)
+    st = Step([1300, 2500, 1500], n, hq, hkv, d, bs, dtype, seed=7, pad=1)
     st.window(700, 20)
     masks = [tree_visibility(_random_tree(m, st.g)) for m in n]
     st.tree(masks)

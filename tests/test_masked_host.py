@@ -9,7 +9,7 @@ import torch
 from nifre_b200 import Attention, PagedKVCache, _lib
 from nifre_b200.block_allocator import BlockAllocator
 from nifre_b200.block_table import BlockTable
-from nifre_b200.masked import WorkLists, build_lists, mask_words, part_sizes, tree_visibility, virtual_keys
+from nifre_b200.masked import WorkLists, build_lists, even_shares, mask_words, tree_visibility, virtual_keys
 from oracle.masked import window_seen
 
 
@@ -36,7 +36,7 @@ def test_units_cover_each_tokens_keys_once(window, sinks, rows):
     unit_rows, item_rows = rows
     group = 4
     lists = build_lists(slots, n, starts, ctx, group, unit_rows, item_rows, workers=8, kv_heads=2, window=window,
-                        sinks=sinks, unit_split=64, item_split=256)
+                        sinks=sinks, unit_share=64, item_share=256)
     cover = {}
     for g, rec in enumerate(lists.groups.tolist()):
         slot, q0, ntok, pos0, c, nd, _, part0 = rec
@@ -77,7 +77,7 @@ def test_units_cover_each_tokens_keys_once(window, sinks, rows):
 def test_tree_lists_carry_every_mask_row():
     parents = [[-1, 0, 0, 1], [-1] * 40, [-1]]
     words = [mask_words(tree_visibility(p)) for p in parents]
-    lists = build_lists([2, 0, 1], [4, 40, 1], [0, 4, 44], [100, 0, 5], 8, 16, 0, 8, 1, words=words, unit_split=64)
+    lists = build_lists([2, 0, 1], [4, 40, 1], [0, 4, 44], [100, 0, 5], 8, 16, 0, 8, 1, words=words, unit_share=64)
     for slot, q0, ntok, pos0, ctx, nd, mask0, _ in lists.groups.tolist():
         s = [2, 0, 1].index(slot)
         seen = tree_visibility(parents[s])
@@ -103,16 +103,24 @@ def test_tree_visibility_and_bits():
         assert back == seen.astype(int).tolist()
 
 
-def test_part_sizes_are_even_and_aligned():
-    keys = np.asarray([1, 15, 16, 17, 127, 128, 129, 1000, 100_000])
-    for split, align in ((64, 16), (256, 128)):
-        size = part_sizes(keys, split, align)
-        assert (size % align == 0).all() and (size <= -(-split // align) * align).all()
-        assert (-(-keys // size) * size - keys < size).all()
+def test_even_shares_cover_every_group_in_order():
+    rng = np.random.default_rng(1)
+    for n, most, share, align in ((1, 5, 64, 16), (9, 3000, 448, 16), (40, 200, 64, 16), (5, 9000, 256, 128), (64, 1041, 464, 16)):
+        keys = rng.integers(1, most, size=n)
+        g, k0, k1 = even_shares(keys, share, align, 4 * align)
+        assert (k0 < k1).all() and (k0 % align == 0).all()
+        assert (np.diff(g) >= 0).all() and set(g.tolist()) == set(range(n))
+        for i in range(n):
+            mine = g == i
+            assert k0[mine][0] == 0 and k1[mine][-1] == keys[i] and (k1[mine][:-1] == k0[mine][1:]).all()
+            if mine.sum() > 1:
+                assert (k1[mine] - k0[mine]).min() >= min(4 * align, share - align)
+        # a share, the pieces next to a cut that was left out, and the rounding
+        assert (k1 - k0).max() <= 2 * share + 8 * align + align
 
 
 def test_packed_lists_and_room():
-    lists = build_lists([0, 1], [1, 40], [0, 1], [500, 20], 4, 16, 0, 4, 1, window=300, sinks=3, unit_split=64)
+    lists = build_lists([0, 1], [1, 40], [0, 1], [500, 20], 4, 16, 0, 4, 1, window=300, sinks=3, unit_share=64)
     room = lists.room(lists.sizes())
     assert all(r >= n and r % 64 == 0 for r, n in zip(room[:6], lists.sizes()[:6]))
     host = lists.pack(room)
@@ -124,7 +132,7 @@ def test_packed_lists_and_room():
 
 def test_too_many_parts_are_refused():
     with pytest.raises(ValueError, match="parts"):
-        build_lists([0], [1], [0], [40_000 * 16], 1, 16, 0, 1, 1, window=1 << 30, unit_split=16)
+        build_lists([0], [1], [0], [40_000 * 64], 1, 16, 0, 1, 1, window=1 << 30, unit_share=64)
 
 
 def test_masked_arguments_struct_matches_the_header(tmp_path):
