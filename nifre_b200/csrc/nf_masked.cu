@@ -416,8 +416,10 @@ static int masked_attention(const NfMaskedArgs* a, bool tree, const char* what, 
   int rc = masked_check(a, tree, what, p);
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (p.max_items)
-    return fail(NF_EUNSUPPORTED, "%s: no tensor-core path for this shape", what);
+  if (p.max_items) {
+    rc = launch_masked_tc(p, a->dtype, stream, what);
+    if (rc) return rc;
+  }
   if (p.max_units) {
     rc = launch_masked_tma(p, a->dtype, stream, what);
     if (rc == NF_EUNSUPPORTED) switch (a->dtype) {
@@ -454,7 +456,7 @@ extern "C" int nf_masked_limits(int32_t dtype, int32_t num_q_heads, int32_t num_
   const int G = num_q_heads / num_kv_heads;
   *unit_rows = masked_tma_rows(dtype, num_q_heads, num_kv_heads, head_dim, block_size);
   if (!*unit_rows) *unit_rows = G > kVecRows ? G : kVecRows;
-  *item_rows = 0;
+  *item_rows = masked_tc_rows(dtype, num_q_heads, num_kv_heads, head_dim, block_size);
   return ok();
 }
 

@@ -123,7 +123,10 @@ __device__ __forceinline__ float* part_record(const MaskedParams& p, long long r
 
 // The tensor-map path (NF_EUNSUPPORTED, nothing launched: not for this shape).
 int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char* what);
+// The tensor-core items.
+int launch_masked_tc(const MaskedParams& p, int dtype, void* stream, const char* what);
 // Largest group for a shape, in query rows (0: no such path).
 int masked_tma_rows(int dtype, int Hq, int Hkv, int D, int bs);
+int masked_tc_rows(int dtype, int Hq, int Hkv, int D, int bs);
 
 }  // namespace nf

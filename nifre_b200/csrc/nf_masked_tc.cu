@@ -1,0 +1,869 @@
+// Windowed and tree attention of larger groups (prefill chunks, wide drafts)
+// on fifth-generation tensor cores (tcgen05, tensor memory), for 16-bit pools
+// with head_dim 64 or 128 and a block size that is a multiple of 16.
+//
+// An item is (unit, KV head): up to 256 query rows (row = token * G + query
+// head), as two 128-row halves, against the unit's part of the group's
+// virtual keys in tiles of 128.  Each 16-key block of a tile has its own
+// place in the pools, so the gap between a window's sinks and its last keys
+// costs nothing: tiles hold visible keys (rounded to 16) only.
+//
+//   producer warp: tensor copies of the queries and of K and V tiles (one
+//     16-token box per block and 64-element part of a head) into rings;
+//   MMA warp: S_h = Q_h K^T (M = N = 128) into tensor memory, then
+//     O_h += P_h V with P_h from tensor memory;
+//   two softmax warpgroups (thread = row), one per half.
+//
+// An item of one half and several tiles (a draft of up to 128 rows) would
+// leave the second warpgroup idle and be bound by the first one's
+// exponentials; there both halves take the same queries, half h the tiles
+// j = h (mod 2) with an accumulator of its own, joined at the item's end.
+//
+// The mask is applied only on tiles that some row does not wholly see: each
+// row's 128 truth values are built as four words (two runs for a window, the
+// shifted mask words for a tree).  Unseen keys get weight 0; as 0 * NaN would
+// still reach the sum, a masked tile's value rows are looked over by one
+// thread each: rows that are not finite are zeroed, and where some row of the
+// item does see one of them, the item's rows are computed again one by one
+// (slow, and right: such values are rare and wrong already).
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "nf_internal.h"
+#include "nf_masked.cuh"
+#include "nf_softmax.cuh"
+#include "nf_tma.cuh"
+#include "nf_umma.cuh"
+
+namespace nf {
+
+template <int D_>
+struct TcCfg {
+  static constexpr uint32_t TILE = 128 * D_ * 2;  // a 128-row Q half, or a 128-key K or V tile
+  static constexpr int QST = D_ == 64 ? 2 : 1;    // Q ring (an item's halves per stage)
+  static constexpr int KST = D_ == 64 ? 4 : 2;
+  static constexpr int VST = D_ == 64 ? 5 : 3;    // (held one tile longer than K)
+  static constexpr bool P_ALIAS = D_ == 128;      // P_h over the first 64 columns of S_h (no room left)
+  static constexpr uint32_t Q_OFF = 2048;         // after the header
+  static constexpr uint32_t K_OFF = Q_OFF + QST * 2 * TILE;
+  static constexpr uint32_t V_OFF = K_OFF + KST * TILE;
+  static constexpr uint32_t SMEM = 1024 + V_OFF + VST * TILE;  // + alignment slack
+  static constexpr int THREADS = 384;  // warp 0 producer, 1 MMA, 4-7 half 0, 8-11 half 1
+  // setmaxnreg split of the launch's 384 x 168 registers
+  static constexpr int REGS_CTRL = 72, REGS_SOFTMAX = 216;
+  static_assert(REGS_CTRL * 128 + REGS_SOFTMAX * 256 <= 168 * THREADS, "register split exceeds the launch");
+  static constexpr uint32_t TMEM_COLS = 512;
+  static __device__ __forceinline__ uint32_t s_col(int h) { return h * 128; }
+  static __device__ __forceinline__ uint32_t o_col(int h) { return 256 + h * D_; }
+  static __device__ __forceinline__ uint32_t p_col(int h) { return P_ALIAS ? h * 128 : 2 * (128 + D_) + h * 64; }
+};
+
+constexpr int kTcItemRing = 4;
+constexpr uint32_t kTcTmemPtr = 512, kTcPoison = 520, kTcSlots = 576, kTcStats = 1024;
+
+struct TcBars {
+  uint32_t hdr;
+  __device__ explicit TcBars(uint32_t h) : hdr(h) {}
+  __device__ uint32_t k_full(int s) const { return hdr + 8 * s; }
+  __device__ uint32_t k_empty(int s) const { return hdr + 64 + 8 * s; }
+  __device__ uint32_t v_full(int s) const { return hdr + 128 + 8 * s; }
+  __device__ uint32_t v_empty(int s) const { return hdr + 192 + 8 * s; }
+  __device__ uint32_t s_full(int h) const { return hdr + 256 + 8 * h; }
+  __device__ uint32_t s_free(int h) const { return hdr + 272 + 8 * h; }
+  __device__ uint32_t p_full(int h) const { return hdr + 288 + 8 * h; }
+  __device__ uint32_t o_done(int h) const { return hdr + 304 + 8 * h; }
+  __device__ uint32_t q_full(int s) const { return hdr + 320 + 8 * s; }
+  __device__ uint32_t q_empty(int s) const { return hdr + 336 + 8 * s; }
+  __device__ uint32_t item_full(int s) const { return hdr + 384 + 8 * s; }
+  __device__ uint32_t item_empty(int s) const { return hdr + 416 + 8 * s; }
+  __device__ uint32_t join_full() const { return hdr + 448; }   // half 1's accumulator and statistics are in place
+  __device__ uint32_t join_empty() const { return hdr + 456; }  // half 0 has read them
+};
+
+// One work item as every role sees it.
+struct TcItem {
+  MaskedGroup g;
+  VirtualKeys vk;
+  int kvh, k0, k1, part, nkt, n_half;
+  bool bad, dup;
+  __device__ TcItem(const MaskedParams& p, int item, int4 un, const MaskedGroup& gr, bool known, int TT)
+      : g(gr), vk(p, gr) {
+    kvh = item % p.Hkv;
+    k0 = un.y;
+    k1 = min(un.z, vk.end);
+    part = un.w;
+    bad = !known || !group_ok(p, g) || k0 < 0 || (k0 & 15) || k0 >= k1 || g.ntok > 2 * TT;
+    nkt = bad ? 0 : (k1 - k0 + 127) >> 7;
+    n_half = g.ntok > TT ? 2 : 1;
+    dup = n_half == 1 && nkt > 1;
+  }
+  __device__ __forceinline__ bool active(int h, int j) const {
+    return j >= 0 && j < nkt && (dup ? (j & 1) == h : h < n_half);
+  }
+  // tiles of half h
+  __device__ __forceinline__ int tiles(int h) const {
+    return dup ? (nkt + 1 - h) >> 1 : (h < n_half ? nkt : 0);
+  }
+  // whether some row of the group does not see the whole of tile j
+  __device__ __forceinline__ bool masked(const MaskedParams& p, int j) const {
+    const int v0 = k0 + 128 * j, v1 = v0 + 127;
+    if (v1 >= k1) return true;
+    if (p.tree) return v1 >= g.ctx;
+    if (v0 < vk.kept) return v1 >= vk.kept || v1 >= p.sinks;
+    const int key0 = v0 + vk.gap, key1 = v1 + vk.gap;
+    return key1 > g.pos0 || !(key0 > g.pos0 + g.ntok - 1 - p.window || key1 < p.sinks);
+  }
+  // the half that looks masked tile j's values over (it is active there)
+  __device__ __forceinline__ int keeper(int j) const { return dup ? j & 1 : n_half - 1; }
+};
+
+// Bits [lo, hi) of word w of a 128-bit row.
+__device__ __forceinline__ uint32_t run_bits(int lo, int hi, int w) {
+  lo = max(lo - 32 * w, 0);
+  hi = min(hi - 32 * w, 32);
+  if (hi <= lo) return 0u;
+  return (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo);
+}
+
+// Truth values of token t's row over tile j: bit i of word i / 32 for key i.
+__device__ __forceinline__ void row_bits(const MaskedParams& p, const TcItem& w, int t, int j, uint32_t (&bits)[4]) {
+  const int v0 = w.k0 + 128 * j, lim = w.k1 - v0;
+  if (p.tree) {
+    const int words = (w.g.n_draft + 31) >> 5;
+    const uint32_t* row = p.masks + w.g.mask0 + (long long)t * words;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int s = v0 + 32 * q - w.g.ctx;  // drafted token of the word's first bit
+      uint32_t b;
+      if (s <= -32) {
+        b = 0xffffffffu;
+      } else if (s < 0) {
+        b = (0xffffffffu >> (32 + s)) | (__ldg(row) << -s);
+      } else {
+        const int i = s >> 5, sh = s & 31;
+        const uint32_t a = i < words ? __ldg(row + i) : 0u, c = i + 1 < words ? __ldg(row + i + 1) : 0u;
+        b = __funnelshift_r(a, c, sh);
+      }
+      bits[q] = b & run_bits(0, lim, q);
+    }
+    return;
+  }
+  const int pos = w.g.pos0 + t;
+  const int a = (w.vk.gap ? p.sinks : min(p.sinks, pos + 1)) - v0;
+  const int b = max(pos - p.window + 1, 0) - w.vk.gap - v0, c = min(pos - w.vk.gap - v0 + 1, lim);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) bits[q] = run_bits(0, min(a, lim), q) | run_bits(max(b, 0), c, q);
+}
+
+// Whether any token of the group sees the key.
+__device__ __noinline__ bool seen_by_any(const MaskedParams& p, const MaskedGroup g, int key) {
+  for (int t = 0; t < g.ntok; ++t)
+    if (sees(p, g, t, key)) return true;
+  return false;
+}
+
+// The ring that hands items to the CTA's warps; a slot holds the item number
+// (-1: no more), its unit, whether its group is known, and the group.
+struct TcRing {
+  const TcBars& bar;
+  unsigned char* slots;
+  Ring r;
+  __device__ TcRing(const TcBars& b, unsigned char* base) : bar(b), slots(base + kTcSlots) {}
+  __device__ int4* slot(int st) const { return reinterpret_cast<int4*>(slots + 64 * st); }
+  __device__ bool next(int& item, int4& un, MaskedGroup& g, bool& known, int* status) {
+    if (!mbar_wait(bar.item_full(r.st), r.ph, status)) return false;
+    const int4* sl = slot(r.st);
+    const int4 a = sl[0], b = sl[1], c = sl[2], d = sl[3];
+    item = a.x;
+    known = a.y != 0;
+    un = b;
+    g = MaskedGroup{c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w};
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar.item_empty(r.st));
+    r.next(kTcItemRing);
+    return item >= 0;
+  }
+};
+
+__device__ __forceinline__ bool tc_claim(const MaskedParams& p, TcRing& ring, int n_items, int& claims, int& item,
+                                         int4& un, MaskedGroup& g, bool& known) {
+  const int lane = threadIdx.x & 31;
+  int pos = blockIdx.x;  // the first item is the CTA's own, the queue hands out the rest
+  if (claims > 0) {
+    if (lane == 0) pos = (int)gridDim.x + atomicAdd(p.queue + 2, 1);
+    pos = __shfl_sync(0xffffffffu, pos, 0);
+  }
+  ++claims;
+  item = pos < n_items ? pos : -1;
+  un = make_int4(0, 0, 0, 0);
+  g = MaskedGroup{};
+  known = false;
+  if (item >= 0) {
+    un = __ldg(reinterpret_cast<const int4*>(p.items) + item / p.Hkv);
+    known = un.x >= 0 && un.x < p.max_groups;
+    if (known) g = load_group(p, un.x);
+  }
+  if (!mbar_wait(ring.bar.item_empty(ring.r.st), ring.r.ph ^ 1, p.status)) return false;
+  if (lane == 0) {
+    int4* sl = ring.slot(ring.r.st);
+    sl[0] = make_int4(item, known, 0, 0);
+    sl[1] = un;
+    sl[2] = make_int4(g.slot, g.q_row0, g.ntok, g.pos0);
+    sl[3] = make_int4(g.ctx, g.n_draft, g.mask0, g.part_row0);
+    mbar_arrive(ring.bar.item_full(ring.r.st));
+  }
+  __syncwarp();
+  ring.r.next(kTcItemRing);
+  return item >= 0;
+}
+
+// Block id of 16-key block `lane` (< 8) of tile j and its first key; -1: none there.
+__device__ __forceinline__ int tc_block(const MaskedParams& p, const TcItem& w, const int* btrow, int j, int lane,
+                                        int& key) {
+  const int v = w.k0 + (j * 8 + lane) * 16;
+  key = w.vk.key(v);
+  const int lb = key / p.bs;
+  if (lane >= 8 || v >= w.k1) return 0;
+  return lb < p.max_blocks ? __ldg(btrow + lb) : -1;
+}
+
+// Copies of one 128-key K or V tile, lane b < nb the 16-key block b.
+template <int D_>
+__device__ __forceinline__ void tc_load(const MaskedParams& p, const CUtensorMap* tm, uint32_t dst0, uint32_t full,
+                                        int phys, int key, int nb, int kvh, uint64_t pol, int lane) {
+  constexpr int NDH = D_ / 64;
+  if (lane == 0) mbar_arrive_expect_tx(full, nb * NDH * 2048);
+  __syncwarp();
+  if (lane < nb) {
+    const int off = key % p.bs;
+    if (phys < 0 || phys >= p.num_blocks) {
+      atomicOr(p.status, NF_STATUS_BAD_BLOCK);
+      phys = 0;
+    }
+#pragma unroll
+    for (int dh = 0; dh < NDH; ++dh) {
+      const uint32_t dst = dst0 + dh * 128 * 128 + lane * 2048;
+      if constexpr (D_ == 64)
+        tma_load_4d(dst, tm, 0, kvh, off, phys, full, pol);
+      else
+        tma_load_5d(dst, tm, 0, dh, kvh, off, phys, full, pol);
+    }
+  }
+}
+
+// Queries whose rows no tensor copy takes (not 16-byte aligned): element
+// loads into the copies' swizzled layout.
+template <typename T, int D_>
+__device__ void tc_load_queries(const MaskedParams& p, const TcItem& w, int TT, uint32_t dst0, uint32_t full, int lane) {
+  constexpr int NDH = D_ / 64;
+  const int rows = w.n_half * TT * p.G, half = TT * p.G;
+  for (int c = lane; c < rows * NDH * 8; c += 32) {
+    const int R = c / (NDH * 8), rest = c % (NDH * 8), h = R / half, row = R - h * half;
+    const int tok = h * TT + row / p.G, hd = row % p.G;
+    uint32_t v[4] = {0, 0, 0, 0};
+    if (tok < w.g.ntok) {
+      const unsigned short* q = reinterpret_cast<const unsigned short*>(p.q) + (long long)(w.g.q_row0 + tok) * p.q_stride +
+                                (long long)(w.kvh * p.G + hd) * D_ + rest * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = q[2 * i] | (uint32_t)q[2 * i + 1] << 16;
+    }
+    const uint32_t dst = dst0 + h * TcCfg<D_>::TILE + (rest >> 3) * 128 * 128 + row * 128 + (((rest & 7) ^ (row & 7)) << 4);
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                 : "memory");
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) mbar_arrive(full);
+}
+
+template <typename T, int D_>
+__device__ void tc_producer(const MaskedParams& p, int TT, bool q_tma, const CUtensorMap* tq, const CUtensorMap* tk,
+                            const CUtensorMap* tv, const TcBars& bar, uint32_t q_s, uint32_t k_s, uint32_t v_s,
+                            int n_items, TcRing& ring) {
+  using C = TcCfg<D_>;
+  constexpr int NDH = D_ / 64;
+  const int lane = threadIdx.x & 31;
+  const uint64_t pol = l2_evict_last(), pol_q = l2_evict_first();
+  Ring qr, kr, vr;
+  int it, claims = 0;
+  int4 un;
+  MaskedGroup g;
+  bool known;
+  pdl_wait();  // queries, keys and values may come from the launch before this one
+  while (tc_claim(p, ring, n_items, claims, it, un, g, known)) {
+    const TcItem w(p, it, un, g, known, TT);
+    if (w.bad) {
+      if (lane == 0) atomicOr(p.status, known ? NF_STATUS_BAD_SLOT : NF_STATUS_UNIT_OVERFLOW);
+      continue;
+    }
+    const int* btrow = p.bt + (long long)w.g.slot * p.max_blocks;
+    int key, cur = tc_block(p, w, btrow, 0, lane, key);
+    if (!mbar_wait(bar.q_empty(qr.st), qr.ph ^ 1, p.status)) return;
+    const uint32_t q_full = bar.q_full(qr.st), q_dst = q_s + qr.st * 2 * C::TILE;
+    if (q_tma) {
+      const int nq = w.n_half * NDH;
+      if (lane == 0) mbar_arrive_expect_tx(q_full, nq * TT * p.G * 128);
+      __syncwarp();
+      if (lane < nq) {
+        const int h = lane / NDH, dh = lane - h * NDH;
+        const uint32_t dst = q_dst + h * C::TILE + dh * 128 * 128;
+        const int row0 = w.g.q_row0 + h * TT;
+        if constexpr (D_ == 64)
+          tma_load_3d(dst, tq, 0, w.kvh * p.G, row0, q_full, pol_q);
+        else
+          tma_load_4d(dst, tq, 0, dh, w.kvh * p.G, row0, q_full, pol_q);
+      }
+    } else {
+      tc_load_queries<T, D_>(p, w, TT, q_dst, q_full, lane);
+    }
+    qr.next(C::QST);
+    for (int j = 0; j < w.nkt; ++j) {
+      const int nb = min(8, (w.k1 - w.k0 - j * 128 + 15) >> 4);
+      if (!mbar_wait(bar.k_empty(kr.st), kr.ph ^ 1, p.status)) return;
+      tc_load<D_>(p, tk, k_s + kr.st * C::TILE, bar.k_full(kr.st), cur, key, nb, w.kvh, pol, lane);
+      kr.next(C::KST);
+      if (!mbar_wait(bar.v_empty(vr.st), vr.ph ^ 1, p.status)) return;
+      tc_load<D_>(p, tv, v_s + vr.st * C::TILE, bar.v_full(vr.st), cur, key, nb, w.kvh, pol, lane);
+      vr.next(C::VST);
+      if (j + 1 < w.nkt) cur = tc_block(p, w, btrow, j + 1, lane, key);
+    }
+  }
+}
+
+template <int D_>
+__device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_t tmem, uint32_t q_s, uint32_t k_s,
+                       uint32_t v_s, bool bf, TcRing& ring) {
+  using C = TcCfg<D_>;
+  const bool leader = elect_one();
+  constexpr uint32_t REG = 128 * 128;  // one 64-element region of a 128-row operand
+  const uint32_t idesc_s = umma_idesc_f16(bf, 128, 128, false, false);
+  const uint32_t idesc_o = umma_idesc_f16(bf, 128, D_, false, true);
+  Ring qr, kr, vr;
+  int n_s[2] = {0, 0}, n_p[2] = {0, 0};
+  auto wait_p = [&](int h) -> bool {
+    if (!mbar_wait(bar.p_full(h), n_p[h] & 1, p.status)) return false;
+    ++n_p[h];
+    return true;
+  };
+  // warp-uniform bases; stages, halves and k-steps are offsets of the descriptors' address field
+  tmem = __shfl_sync(0xffffffffu, tmem, 0);
+  const uint64_t dq = umma_sdesc_sw128(__shfl_sync(0xffffffffu, q_s, 0), 16, 1024);
+  const uint64_t dk = umma_sdesc_sw128(__shfl_sync(0xffffffffu, k_s, 0), 16, 1024);
+  const uint64_t dv = umma_sdesc_sw128(__shfl_sync(0xffffffffu, v_s, 0), REG, 1024);
+  auto issue_pv = [&](int h, int vst, bool first) {
+    tc_fence_after();
+    const uint64_t b0 = dv + (uint64_t)(vst * (C::TILE >> 4));
+    const uint32_t d = tmem + C::o_col(h), a0 = tmem + C::p_col(h);
+    if (leader) {
+      umma_f16_ts(d, a0, b0, idesc_o, first ? 0u : 1u);
+#pragma unroll
+      for (int kk = 1; kk < 8; ++kk) umma_f16_ts(d, a0 + kk * 8, b0 + (uint64_t)(kk * 16 * 128 >> 4), idesc_o, 1u);
+      umma_commit(bar.o_done(h));
+    }
+    __syncwarp();
+  };
+  auto issue_s = [&](int h, int qh, int kst) {
+    const uint64_t a0 = dq + (uint64_t)((qr.st * 2 + qh) * (C::TILE >> 4)), b0 = dk + (uint64_t)(kst * (C::TILE >> 4));
+    const uint32_t d = tmem + C::s_col(h);
+    if (leader) {
+#pragma unroll
+      for (int k = 0; k < D_ / 16; ++k) {
+        const uint64_t off = (uint64_t)(((k >> 2) * REG + (k & 3) * 32) >> 4);
+        umma_f16_ss(d, a0 + off, b0 + off, idesc_s, k > 0 ? 1u : 0u);
+      }
+      umma_commit(bar.s_full(h));
+    }
+    __syncwarp();
+  };
+  int it;
+  int4 un;
+  MaskedGroup g;
+  bool known;
+  while (ring.next(it, un, g, known, p.status)) {
+    const TcItem w(p, it, un, g, known, TT);
+    if (w.bad) continue;
+    int vprev = -1;  // V stage of tile j-1
+    bool waited = false;  // tile j-1's weights were waited for already
+    auto first_of = [&](int j) { return w.dup ? j < 2 : j == 0; };  // a half's first tile overwrites O_h
+    // both halves' weights of a masked tile must be in before either P V: the keeper half may zero value rows
+    auto wait_all = [&](int j) -> bool {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (w.active(h, j) && !wait_p(h)) return false;
+      return true;
+    };
+    if (!mbar_wait(bar.q_full(qr.st), qr.ph, p.status)) return;
+    for (int j = 0; j < w.nkt; ++j) {
+      if (!mbar_wait(bar.k_full(kr.st), kr.ph, p.status)) return;
+      waited = false;
+      if (C::P_ALIAS && j > 0 && !w.dup && w.masked(p, j - 1)) {
+        if (!wait_all(j - 1)) return;
+        waited = true;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (C::P_ALIAS && !w.dup && w.active(h, j - 1)) {
+          // P_h of tile j-1 sits in S_h: consume it before S_h is rewritten
+          if (!waited && !wait_p(h)) return;
+          issue_pv(h, vprev, first_of(j - 1));
+        }
+        if (!w.active(h, j)) continue;
+        if (!C::P_ALIAS) {
+          if (!mbar_wait(bar.s_free(h), (n_s[h] & 1) ^ 1, p.status)) return;
+          ++n_s[h];
+        }
+        tc_fence_after();
+        issue_s(h, w.dup ? 0 : h, kr.st);
+      }
+      if (leader) umma_commit(bar.k_empty(kr.st));
+      kr.next(C::KST);
+      if (j > 0) {
+        if (!C::P_ALIAS || w.dup) {
+          // (dup: half h's weights of tile j-2 in S_h were consumed before S_h of tile j was issued)
+          if (w.masked(p, j - 1)) {
+            if (!wait_all(j - 1)) return;
+            waited = true;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (!w.active(h, j - 1)) continue;
+            if (!waited && !wait_p(h)) return;
+            issue_pv(h, vprev, first_of(j - 1));
+          }
+        }
+        if (leader) umma_commit(bar.v_empty(vprev));
+      }
+      if (!mbar_wait(bar.v_full(vr.st), vr.ph, p.status)) return;
+      vprev = vr.st;
+      vr.next(C::VST);
+    }
+    // every S of the item is issued: the Q stage is free once they complete
+    if (leader) umma_commit(bar.q_empty(qr.st));
+    qr.next(C::QST);
+    const int jl = w.nkt - 1;
+    if (!wait_all(jl)) return;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (w.active(h, jl)) issue_pv(h, vprev, first_of(jl));
+    if (leader) umma_commit(bar.v_empty(vprev));
+  }
+}
+
+// One row's attention over the item's keys in plain float32, one key at a
+// time (an item whose values are not finite where some of its rows see them).
+template <typename T, int D_>
+__device__ __noinline__ void tc_row_again(const MaskedParams& p, const MaskedGroup g, int k0, int k1, int part, int kvh,
+                                          int tok, int hd) {
+  const VirtualKeys vk(p, g);
+  const int* btrow = p.bt + (long long)g.slot * p.max_blocks;
+  const int head = kvh * p.G + hd;
+  const T* q = reinterpret_cast<const T*>(p.q) + (long long)(g.q_row0 + tok) * p.q_stride + (long long)head * D_;
+  float acc[D_], m = -INFINITY, l = 0.f;
+  for (int d = 0; d < D_; ++d) acc[d] = 0.f;
+  for (int v = k0; v < k1; ++v) {
+    const int key = vk.key(v);
+    if (!sees(p, g, tok, key)) continue;
+    const long long row = key_row(p, btrow, key);
+    if (row < 0) continue;
+    const long long off = (row * p.Hkv + kvh) * D_;
+    const T* kr = reinterpret_cast<const T*>(p.kp) + off;
+    const T* vr = reinterpret_cast<const T*>(p.vp) + off;
+    float x = 0.f;
+    for (int d = 0; d < D_; ++d) x = fmaf(Elem<T>::to_f(q[d]), Elem<T>::to_f(kr[d]), x);
+    x *= p.scale_log2;
+    const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.f : mn;
+    const float a = ex2(m - base), e = ex2(x - base);
+    m = mn;
+    l = l * a + e;
+    for (int d = 0; d < D_; ++d) acc[d] = fmaf(e, Elem<T>::to_f(vr[d]), acc[d] * a);
+  }
+  if (part >> 16 == 1) {
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride + (long long)head * D_;
+    for (int d = 0; d < D_; ++d) dst[d] = Elem<T>::from_f(acc[d] * inv);
+  } else {
+    const long long prow = (long long)g.part_row0 + (long long)(part & 0xffff) * g.ntok + tok;
+    if (g.part_row0 < 0 || prow >= p.ws_rows) return;
+    float* rec = part_record(p, prow, head);
+    for (int d = 0; d < D_; ++d) rec[d] = acc[d];
+    rec[D_] = m;
+    rec[D_ + 1] = l;
+  }
+}
+
+template <typename T, int D_>
+__device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBars& bar, unsigned char* base,
+                           uint32_t tmem, uint32_t v_s, int h, TcRing& ring) {
+  using C = TcCfg<D_>;
+  constexpr int NDH = D_ / 64;
+  constexpr uint32_t REG = 128 * 128;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quad = warp & 3, row = quad * 32 + lane;  // tensor-memory lanes of this warp: quad*32..
+  const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+  const uint32_t s_addr = tmem + lane_addr + C::s_col(h), o_addr = tmem + lane_addr + C::o_col(h);
+  const uint32_t p_addr = tmem + lane_addr + C::p_col(h);
+  volatile int* poison = reinterpret_cast<volatile int*>(base + kTcPoison);  // [2]: the last poisoned item of each parity
+  float2* stats = reinterpret_cast<float2*>(base + kTcStats);  // half 1's (m, l) of a joined item
+  int n_s = 0, n_o = 0, n_join = 0;
+  // a scale of 0 or less cannot follow the maximum and the mask: the scores are scaled before them then
+  const float scale = p.scale_log2 > 0.f ? p.scale_log2 : 1.f;
+  bool join_pending = false;  // half 1: its accumulator is still to be read by half 0
+  Ring vr;
+  int it, seq = 0;
+  int4 un;
+  MaskedGroup g;
+  bool known;
+  while (ring.next(it, un, g, known, p.status)) {
+    const TcItem w(p, it, un, g, known, TT);
+    if (w.bad) continue;
+    ++seq;
+    const Ring v0r = vr;  // V stage of the item's first tile
+    vr = vr.ahead(w.nkt, C::VST);
+    if (w.tiles(h) == 0) continue;
+    const int tok = (w.dup ? 0 : h * TT) + row / p.G, hd = row % p.G;
+    const bool valid = row < TT * p.G && tok < w.g.ntok;
+    float m = -INFINITY, l = 0.f;
+    int n = 0;  // tiles done
+    for (int j = w.dup ? h : 0; j < w.nkt; j += w.dup ? 2 : 1, ++n) {
+      if (!mbar_wait(bar.s_full(h), n_s & 1, p.status)) return;
+      ++n_s;
+      tc_fence_after();
+      uint32_t x[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+      tmem_wait_ld();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_reg_fence(*reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+      if (!C::P_ALIAS) {  // S_h is in registers: the next S_h may be computed
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar.s_free(h));
+      }
+      if (p.scale_log2 <= 0.f) {
+#pragma unroll
+        for (int i = 0; i < 128; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * p.scale_log2);
+      }
+      const bool masked = w.masked(p, j);
+      if (masked) {
+        uint32_t bits[4] = {0u, 0u, 0u, 0u};
+        if (valid) row_bits(p, w, tok, j, bits);
+#pragma unroll
+        for (int i = 0; i < 128; ++i)
+          if (!(bits[i >> 5] >> (i & 31) & 1u)) x[i] = 0xff800000u;
+      }
+      float acc[8];
+#pragma unroll
+      for (int a = 0; a < 8; ++a) acc[a] = fmaxf(__uint_as_float(x[a]), __uint_as_float(x[a + 8]));
+#pragma unroll
+      for (int i = 16; i < 128; i += 16)
+#pragma unroll
+        for (int a = 0; a < 8; ++a) acc[a] = fmax3(acc[a], __uint_as_float(x[i + a]), __uint_as_float(x[i + 8 + a]));
+      float mt = fmaxf(fmaxf(fmaxf(acc[0], acc[1]), fmaxf(acc[2], acc[3])),
+                       fmaxf(fmaxf(acc[4], acc[5]), fmaxf(acc[6], acc[7])));
+      mt *= scale;
+      // lazy rescaling: the reference max moves only when the tile's max exceeds it by more than 8
+      const bool grow = mt > m + 8.f;
+      const float mn = grow ? mt : m;
+      const float alpha = grow ? ex2(m - mn) : 1.f;
+      const float nbase = mn == -INFINITY ? 0.f : -mn;
+      const uint64_t sc2 = f2_pack(scale, scale), nb2 = f2_pack(nbase, nbase);
+      uint64_t sum2[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) sum2[a] = 0ull;
+#pragma unroll
+      for (int i = 0; i < 128; i += 2) {
+        const uint64_t y2 = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, nb2);
+        float y0, y1;
+        f2_unpack(y2, y0, y1);
+        const float p0 = ex2(y0), p1 = ex2(y1);
+        sum2[(i >> 1) & 3] = f2_add(sum2[(i >> 1) & 3], f2_pack(p0, p1));
+        x[i >> 1] = pack2<T>(p0, p1);
+      }
+      if (n > 0) {  // O_h += P_h V of the half's tile before must be done before P_h or O_h change
+        if (!mbar_wait(bar.o_done(h), n_o & 1, p.status)) return;
+        ++n_o;
+        tc_fence_after();
+      } else if (join_pending) {  // half 0 has read this half's last accumulator
+        if (!mbar_wait(bar.join_empty(), (n_join - 1) & 1, p.status)) return;
+        join_pending = false;
+      }
+      tmem_st32(p_addr, *reinterpret_cast<uint32_t(*)[32]>(x));
+      tmem_st32(p_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+      if (n > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+        for (int c = 0; c < D_ / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_wait_ld();
+          tmem_reg_fence(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(o_addr + c * 32, o);
+        }
+      }
+      float sa[8];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) f2_unpack(sum2[a], sa[2 * a], sa[2 * a + 1]);
+      l = l * alpha + (((sa[0] + sa[1]) + (sa[2] + sa[3])) + ((sa[4] + sa[5]) + (sa[6] + sa[7])));
+      m = mn;
+      if (masked && w.keeper(j) == h) {
+        // this thread's value row of the tile: zeroed when past the unit's keys or not finite
+        const Ring vt = v0r.ahead(j, C::VST);
+        if (!mbar_wait(bar.v_full(vt.st), vt.ph, p.status)) return;
+        const uint32_t vs = v_s + vt.st * C::TILE + row * 128;
+        const int v = w.k0 + 128 * j + row;
+        bool odd = v >= w.k1;
+        if (!odd) {
+          constexpr uint32_t EX = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+#pragma unroll
+          for (int dh = 0; dh < NDH; ++dh)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint32_t e[4];
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3])
+                           : "r"(vs + dh * REG + ((c ^ (row & 7)) << 4)));
+#pragma unroll
+              for (int q = 0; q < 4; ++q) odd |= (e[q] & EX) == EX || ((e[q] >> 16) & EX) == EX;
+            }
+          if (odd && seen_by_any(p, w.g, w.vk.key(v))) poison[seq & 1] = seq;
+        }
+        if (odd) {
+#pragma unroll
+          for (int dh = 0; dh < NDH; ++dh)
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + dh * REG + c * 16), "r"(0) : "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar.p_full(h));
+    }
+    if (!mbar_wait(bar.o_done(h), n_o & 1, p.status)) return;
+    ++n_o;
+    tc_fence_after();
+    float a0 = 1.f, a1 = 0.f;  // weights of this half's and half 1's accumulators
+    if (w.dup) {
+      ++n_join;
+      if (h == 1) {
+        stats[row] = make_float2(m, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar.join_full());
+        join_pending = true;
+        continue;
+      }
+      if (!mbar_wait(bar.join_full(), (n_join - 1) & 1, p.status)) return;
+      tc_fence_after();
+      const float2 other = stats[row];
+      const float mn = fmaxf(m, other.x), b = mn == -INFINITY ? 0.f : mn;
+      a0 = ex2(m - b);
+      a1 = ex2(other.x - b);
+      l = l * a0 + other.y * a1;
+      m = mn;
+    }
+    const int n_parts = w.part >> 16;
+    const long long prow = (long long)w.g.part_row0 + (long long)(w.part & 0xffff) * w.g.ntok + tok;
+    float* rec = nullptr;
+    if (valid && n_parts > 1) {
+      if (w.g.part_row0 < 0 || prow >= p.ws_rows)
+        atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
+      else
+        rec = part_record(p, prow, w.kvh * p.G + hd);
+    }
+    if (n_parts == 1) {
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      a0 *= inv;
+      a1 *= inv;
+    }
+    T* dst = reinterpret_cast<T*>(p.out) + (long long)(w.g.q_row0 + tok) * p.out_stride + (long long)(w.kvh * p.G + hd) * D_;
+#pragma unroll
+    for (int c = 0; c < D_ / 32; ++c) {
+      uint32_t o[32];
+      tmem_ld32(o_addr + c * 32, o);
+      tmem_wait_ld();
+      tmem_reg_fence(o);
+      if (w.dup) {
+        uint32_t o1[32];
+        tmem_ld32(o_addr - C::o_col(0) + C::o_col(1) + c * 32, o1);
+        tmem_wait_ld();
+        tmem_reg_fence(o1);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          o[i] = __float_as_uint(fmaf(__uint_as_float(o1[i]), a1, __uint_as_float(o[i]) * a0));
+      } else if (n_parts == 1) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a0);
+      }
+      if (rec) {
+        float4* r4 = reinterpret_cast<float4*>(rec + c * 32);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          __stcg(r4 + i, make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
+      } else if (valid && n_parts == 1) {
+        if (out16) {
+          uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            d4[i] = make_uint4(pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])),
+                               pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3])),
+                               pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])),
+                               pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) dst[c * 32 + i] = Elem<T>::from_f(__uint_as_float(o[i]));
+        }
+      }
+    }
+    if (rec) __stcg(reinterpret_cast<float2*>(rec + D_), make_float2(m, l));
+    tc_fence_before();
+    if (w.dup) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar.join_empty());
+    }
+    if (poison[seq & 1] == seq && valid)
+      tc_row_again<T, D_>(p, w.g, w.k0, w.k1, w.part, w.kvh, tok, hd);
+  }
+}
+
+template <typename T, int D_>
+__global__ void __launch_bounds__(TcCfg<D_>::THREADS, 1)
+    masked_tc_kernel(const MaskedParams p, int TT, int q_tma, int out16, const __grid_constant__ CUtensorMap tq,
+                     const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv) {
+  using C = TcCfg<D_>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t hdr = smem_u32(base);
+  const TcBars bar(hdr);
+  const int warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  if (threadIdx.x == 32) {
+    tma_prefetch_map(&tk);
+    tma_prefetch_map(&tv);
+    if (q_tma) tma_prefetch_map(&tq);
+  }
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::KST; ++s) {
+      mbar_init(bar.k_full(s), 1);
+      mbar_init(bar.k_empty(s), 1);
+    }
+    for (int s = 0; s < C::VST; ++s) {
+      mbar_init(bar.v_full(s), 1);
+      mbar_init(bar.v_empty(s), 1);
+    }
+    for (int h = 0; h < 2; ++h) {
+      mbar_init(bar.s_full(h), 1);
+      mbar_init(bar.s_free(h), 4);
+      mbar_init(bar.p_full(h), 4);
+      mbar_init(bar.o_done(h), 1);
+    }
+    for (int s = 0; s < C::QST; ++s) {
+      mbar_init(bar.q_full(s), 1);
+      mbar_init(bar.q_empty(s), 1);
+    }
+    for (int s = 0; s < kTcItemRing; ++s) {
+      mbar_init(bar.item_full(s), 1);
+      mbar_init(bar.item_empty(s), 1 + 4 * 2);  // the MMA warp and the softmax warps
+    }
+    mbar_init(bar.join_full(), 4);
+    mbar_init(bar.join_empty(), 4);
+    fence_mbar_init();
+    reinterpret_cast<int*>(base + kTcPoison)[0] = 0;
+    reinterpret_cast<int*>(base + kTcPoison)[1] = 0;
+  }
+  if (warp == 1) tmem_alloc(hdr + kTcTmemPtr, C::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(base + kTcTmemPtr);
+  const uint32_t q_s = hdr + C::Q_OFF, k_s = hdr + C::K_OFF, v_s = hdr + C::V_OFF;
+  const int n_items = min(__ldg(p.counts + 1), p.max_items) * p.Hkv;
+  TcRing ring(bar, base);
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_CTRL));
+    if (warp == 0)
+      tc_producer<T, D_>(p, TT, q_tma, &tq, &tk, &tv, bar, q_s, k_s, v_s, n_items, ring);
+    else if (warp == 1)
+      tc_mma<D_>(p, TT, bar, tmem, q_s, k_s, v_s, std::is_same<T, __nv_bfloat16>::value, ring);
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
+    tc_softmax<T, D_>(p, TT, out16, bar, base, tmem, v_s, (warp - 4) >> 2, ring);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, C::TMEM_COLS);
+  // every ticket of every CTA is taken when the last CTA is out
+  if (threadIdx.x == 0 && atomicAdd(p.queue + 3, 1) == (int)gridDim.x - 1) {
+    p.queue[2] = 0;
+    p.queue[3] = 0;
+    __threadfence();
+  }
+}
+
+// 256 rows of whole tokens: any group of up to 64 query heads per KV head.
+int masked_tc_rows(int dtype, int Hq, int Hkv, int D, int bs) {
+  if (dtype != NF_BF16 && dtype != NF_F16) return 0;
+  if ((D != 64 && D != 128) || bs % 16) return 0;
+  const int G = Hq / Hkv;
+  return G <= 64 ? 2 * (128 / G) * G : 0;
+}
+
+template <typename T, int D_>
+static int launch_tc(const MaskedParams& p, int TT, int q_tma, int out16, const CUtensorMap& tq, const CUtensorMap& tk,
+                     const CUtensorMap& tv, cudaStream_t st, const char* what) {
+  using C = TcCfg<D_>;
+  auto kern = masked_tc_kernel<T, D_>;
+  cudaError_t e = prepare_launch(reinterpret_cast<const void*>(kern), (int)C::SMEM, C::THREADS, nullptr);
+  if (e != cudaSuccess) return fail(NF_ECUDA, "%s: smem attribute: %s", what, cudaGetErrorString(e));
+  static int regs = -1;  // a property of the binary, queried once
+  if (regs < 0) {
+    cudaFuncAttributes fa;
+    regs = cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : 0;
+  }
+  if (C::REGS_CTRL * 128 + C::REGS_SOFTMAX * 256 > regs * C::THREADS)
+    return fail(NF_EUNSUPPORTED, "%s: kernel built with %d registers per thread, the warpgroup split needs 168", what, regs);
+  long long grid = (long long)p.max_items * p.Hkv;
+  if (grid > sm_count()) grid = sm_count();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, p, TT, q_tma, out16, tq, tk, tv);
+  if (e != cudaSuccess) return fail(NF_ECUDA, "%s: launch: %s", what, cudaGetErrorString(e));
+  return check_launch(what);
+}
+
+int launch_masked_tc(const MaskedParams& p, int dtype, void* stream, const char* what) {
+  if (!masked_tc_rows(dtype, p.Hq, p.Hkv, p.D, p.bs))
+    return fail(NF_EUNSUPPORTED, "%s: no tensor-core items for this shape", what);
+  if ((reinterpret_cast<uintptr_t>(p.kp) | reinterpret_cast<uintptr_t>(p.vp)) & 15)
+    return fail(NF_EINVAL, "%s: pools must be 16-byte aligned", what);
+  if ((long long)p.max_items * p.Hkv > INT32_MAX) return fail(NF_EINVAL, "%s: too many items", what);
+  const int TT = 128 / p.G;
+  const int q_tma = reinterpret_cast<uintptr_t>(p.q) % 16 == 0 && p.q_stride % 8 == 0 && p.q_stride > 0;
+  const int out16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % 8 == 0;
+  CUtensorMap tq, tk, tv;
+  if (!encode_pool_map(&tk, p.kp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, 1, false) ||
+      !encode_pool_map(&tv, p.vp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, 1, false) ||
+      (q_tma && !encode_rows_map(&tq, p.q, dtype, p.D, p.Hq, p.rows, p.q_stride, p.G, TT)))
+    return fail(NF_ECUDA, "%s: tensor map encoding failed", what);
+  if (!q_tma) tq = tk;  // (not used)
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == NF_BF16)
+    return p.D == 64 ? launch_tc<__nv_bfloat16, 64>(p, TT, q_tma, out16, tq, tk, tv, st, what)
+                     : launch_tc<__nv_bfloat16, 128>(p, TT, q_tma, out16, tq, tk, tv, st, what);
+  return p.D == 64 ? launch_tc<__half, 64>(p, TT, q_tma, out16, tq, tk, tv, st, what)
+                   : launch_tc<__half, 128>(p, TT, q_tma, out16, tq, tk, tv, st, what);
+}
+
+}  // namespace nf

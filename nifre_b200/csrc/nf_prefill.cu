@@ -44,6 +44,7 @@
 
 #include "nf_common.cuh"
 #include "nf_internal.h"
+#include "nf_softmax.cuh"
 #include "nf_tma.cuh"
 #include "nf_umma.cuh"
 
@@ -146,32 +147,6 @@ constexpr int kPfItemRing = 4;
 
 
 // ---------------------------------------------------------------- softmax arithmetic
-// Pairs of fp32 values in one 64-bit register, for the packed fp32x2
-// instructions of sm_100 (two FMAs or adds per issue).
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
 // 2^y for a pair y <= 8 on the FMA pipe instead of the special-function
 // unit: y = j + f with j = round(y) (adding and subtracting 1.5 * 2^23), 2^f
 // on [-1/2, 1/2] by 1 + c1 f + c2 f^2 + c3 f^3 fitted for minimum relative
@@ -213,25 +188,6 @@ constexpr int kPfPolyPairs = NF_PF_POLY;
 // per turn and each warp's non-exponent work grows once the halves are out
 // of step, so by default the halves share the unit in step.
 constexpr bool kPfTurns = NF_PF_TURNS != 0;
-
-// A ring position: stage index and the parity of its current fill.
-struct Ring {
-  int st = 0;
-  uint32_t ph = 0;
-  __device__ void next(int n) {
-    if (++st == n) {
-      st = 0;
-      ph ^= 1;
-    }
-  }
-  __device__ Ring ahead(int k, int n) const {  // the position k fills later
-    Ring r;
-    const int t = st + k;
-    r.st = t % n;
-    r.ph = ph ^ ((uint32_t)(t / n) & 1u);
-    return r;
-  }
-};
 
 // Work items come from one queue shared by all CTAs: the producer warp of
 // a CTA claims the next position in the order (longest items first) when it

@@ -249,6 +249,13 @@ def test_large_scores_and_long_window():
     st.window(4000, 0, scale=2.0)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0])
+def test_scales(scale):
+    st = Step([60, 10], [1, 60], 4, 2, 64, 16, BF, seed=11, pad=1)
+    st.window(40, 3, scale=scale)
+    st.tree([np.tril(np.ones((m, m), bool)) for m in st.n], scale=scale)
+
+
 def test_dense_cache_rows():
     from nifre_b200 import KVCache
     for room in (16, 13):
