@@ -22,6 +22,7 @@
 
 #include "nf_internal.h"
 #include "nf_masked.cuh"
+#include "nf_softmax.cuh"
 #include "nf_tma.cuh"
 
 namespace nf {
@@ -46,6 +47,25 @@ struct MtLaunch {
 // Byte offset of key row r, 16-byte chunk c, in one head's staged tile.
 __device__ __forceinline__ int mt_off(int r, int c) {
   return (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+// mma.sync and movmatrix as pure functions of their registers (not volatile:
+// the scheduler may interleave independent ones with the softmax arithmetic).
+template <typename T>
+__device__ __forceinline__ void mt_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t mt_transpose(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 template <int D_>
@@ -189,95 +209,129 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
 }
 
 // A unit as its consumer warp holds it, and the running state of NT tiles of
-// 8 columns: column c = 8 j + 2 (lane % 4) (+1) of token c / G.
+// 8 columns: column c = 8 j + 2 (lane % 4) (+1) of token c / G.  m is the
+// reference the exponents are taken against, 0 while bit 2 j + e of none says
+// that the column has seen no key yet.
 template <int D_, int NT>
 struct MtState {
   static constexpr int KS = D_ / 16;
   uint32_t qf[NT][KS][2];
   float m[NT][2], l[NT][2];
   float o[KS][NT][4];
+  uint32_t none;
 };
 
-// PT staged 16-key tiles of this warp's head in one update.
-template <typename T, int D_, int NT, int PT>
+// PT staged 16-key tiles of this warp's head in one update.  With eight
+// consumer warps an SM the update's latency and instruction count bound it,
+// not its products, so the reference maximum moves only when some score
+// exceeds it by more than 8 (one vote a tile pair instead of three shuffles
+// a column, and no rescaling of O otherwise: weights stay below 2^8).
+template <typename T, int D_, int NT, int PT, bool EARLY>
 __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGroup& g, const uint32_t (&kb)[PT],
                                           const uint32_t (&vb)[PT], const int (&key0)[PT], const int (&nv)[PT],
-                                          int masked, MtState<D_, NT>& st) {
+                                          int masked, int c0, MtState<D_, NT>& st) {
   constexpr int KS = D_ / 16;
   const int lane = threadIdx.x & 31, tq = lane >> 2, n0 = 2 * (lane & 3);
   const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;
   const int vr = (lane & 7) + ((lane >> 4) & 1) * 8, vc = (lane >> 3) & 1;
   float x[PT][NT][4];
+  // fragments of both tiles (and of the values) at once where registers allow, else a tile's at a time
+  constexpr bool kEarly = EARLY;
+  uint32_t kf[kEarly ? PT : 1][KS][4];
 #pragma unroll
-  for (int t = 0; t < PT; ++t) {
+  for (int t = 0; t < PT; ++t)
 #pragma unroll
     for (int j = 0; j < NT; ++j) x[t][j][0] = x[t][j][1] = x[t][j][2] = x[t][j][3] = 0.f;
+  if constexpr (kEarly) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      uint32_t a0, a1, a2, a3;
-      ldsm_x4(kb[t] + mt_off(kr, 2 * ks + kc), a0, a1, a2, a3);
+    for (int t = 0; t < PT; ++t)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) mma16816<T>(x[t][j], a0, a1, a2, a3, st.qf[j][ks][0], st.qf[j][ks][1]);
+      for (int ks = 0; ks < KS; ++ks)
+        ldsm_x4(kb[t] + mt_off(kr, 2 * ks + kc), kf[t][ks][0], kf[t][ks][1], kf[t][ks][2], kf[t][ks][3]);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int t = 0; t < PT; ++t)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mt_mma<T>(x[t][j], kf[t][ks], st.qf[j][ks][0], st.qf[j][ks][1]);
+  } else {
+#pragma unroll
+    for (int t = 0; t < PT; ++t) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        ldsm_x4(kb[t] + mt_off(kr, 2 * ks + kc), kf[0][ks][0], kf[0][ks][1], kf[0][ks][2], kf[0][ks][3]);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mt_mma<T>(x[t][j], kf[0][ks], st.qf[j][ks][0], st.qf[j][ks][1]);
     }
+  }
+  uint32_t vf[kEarly ? PT : 1][KS][4];
+  if constexpr (kEarly) {
+#pragma unroll
+    for (int t = 0; t < PT; ++t)
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+        ldsm_x4_t(vb[t] + mt_off(vr, 2 * i + vc), vf[t][i][0], vf[t][i][1], vf[t][i][2], vf[t][i][3]);
+  }
+  // exponents against the reference; unseen keys -inf
+  const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
+  float top = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const uint64_t nm2 = f2_pack(-st.m[j][0], -st.m[j][1]);
+#pragma unroll
+    for (int t = 0; t < PT; ++t) {
+      f2_unpack(f2_fma(f2_pack(x[t][j][0], x[t][j][1]), sc2, nm2), x[t][j][0], x[t][j][1]);
+      f2_unpack(f2_fma(f2_pack(x[t][j][2], x[t][j][3]), sc2, nm2), x[t][j][2], x[t][j][3]);
+      if (masked >> t & 1) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = tq + (e >> 1) * 8, tok = min((c0 + 8 * j + n0 + (e & 1)) / p.G, g.ntok - 1);
+          if (row >= nv[t] || !sees(p, g, tok, key0[t] + row)) x[t][j][e] = -INFINITY;
+        }
+      }
+      top = fmax3(top, fmaxf(x[t][j][0], x[t][j][1]), fmaxf(x[t][j][2], x[t][j][3]));
+    }
+  }
+  if (__any_sync(0xffffffffu, top > 8.f || st.none)) {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[t][j][e] *= p.scale_log2;
-    if (masked >> t & 1) {
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(x[0][j][e], x[0][j][2 + e]);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+        for (int t = 1; t < PT; ++t) mx = fmax3(mx, x[t][j][e], x[t][j][2 + e]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = tq + (e >> 1) * 8, tok = min((8 * j + n0 + (e & 1)) / p.G, g.ntok - 1);
-          if (row >= nv[t] || !sees(p, g, tok, key0[t] + row)) x[t][j][e] = -INFINITY;
+        for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const uint32_t bit = 1u << (2 * j + e);
+        const bool first = st.none & bit;  // the first seen keys set the reference, later ones raise it
+        const float up = first ? (mx == -INFINITY ? 0.f : mx) : (mx > 8.f ? mx : 0.f);
+        const float alpha = first ? 1.f : ex2(-up);
+        if (mx != -INFINITY) st.none &= ~bit;
+        st.m[j][e] += up;
+        st.l[j][e] *= alpha;
+#pragma unroll
+        for (int t = 0; t < PT; ++t) {
+          x[t][j][e] -= up;
+          x[t][j][2 + e] -= up;
         }
-    }
-  }
-  float mx[NT][2];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    mx[j][0] = fmaxf(x[0][j][0], x[0][j][2]);
-    mx[j][1] = fmaxf(x[0][j][1], x[0][j][3]);
-#pragma unroll
-    for (int t = 1; t < PT; ++t) {
-      mx[j][0] = fmaxf(mx[j][0], fmaxf(x[t][j][0], x[t][j][2]));
-      mx[j][1] = fmaxf(mx[j][1], fmaxf(x[t][j][1], x[t][j][3]));
-    }
+        for (int i = 0; i < KS; ++i) {
+          st.o[i][j][e] *= alpha;
+          st.o[i][j][2 + e] *= alpha;
+        }
+      }
   }
 #pragma unroll
-  for (int o = 4; o < 32; o <<= 1)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      mx[j][0] = fmaxf(mx[j][0], __shfl_xor_sync(0xffffffffu, mx[j][0], o));
-      mx[j][1] = fmaxf(mx[j][1], __shfl_xor_sync(0xffffffffu, mx[j][1], o));
-    }
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const float mn0 = fmaxf(st.m[j][0], mx[j][0]), mn1 = fmaxf(st.m[j][1], mx[j][1]);
-    const float b0 = mn0 == -INFINITY ? 0.f : mn0, b1 = mn1 == -INFINITY ? 0.f : mn1;
-    const float al0 = ex2(st.m[j][0] - b0), al1 = ex2(st.m[j][1] - b1);
-    st.m[j][0] = mn0;
-    st.m[j][1] = mn1;
-    float s0 = 0.f, s1 = 0.f;
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
     for (int t = 0; t < PT; ++t) {
-      x[t][j][0] = ex2(x[t][j][0] - b0);
-      x[t][j][1] = ex2(x[t][j][1] - b1);
-      x[t][j][2] = ex2(x[t][j][2] - b0);
-      x[t][j][3] = ex2(x[t][j][3] - b1);
-      s0 += x[t][j][0] + x[t][j][2];
-      s1 += x[t][j][1] + x[t][j][3];
-    }
-    st.l[j][0] = st.l[j][0] * al0 + s0;
-    st.l[j][1] = st.l[j][1] * al1 + s1;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      st.o[i][j][0] *= al0;
-      st.o[i][j][1] *= al1;
-      st.o[i][j][2] *= al0;
-      st.o[i][j][3] *= al1;
+      for (int e = 0; e < 4; ++e) x[t][j][e] = ex2(x[t][j][e]);
+      st.l[j][0] += x[t][j][0] + x[t][j][2];
+      st.l[j][1] += x[t][j][1] + x[t][j][3];
     }
-  }
 #pragma unroll
   for (int t = 0; t < PT; ++t) {
     bool plain = true;
@@ -298,15 +352,15 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
       uint32_t pb[NT][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        pb[j][0] = movmatrix_t(pack2<T>(x[t][j][0], x[t][j][1]));
-        pb[j][1] = movmatrix_t(pack2<T>(x[t][j][2], x[t][j][3]));
+        pb[j][0] = mt_transpose(pack2<T>(x[t][j][0], x[t][j][1]));
+        pb[j][1] = mt_transpose(pack2<T>(x[t][j][2], x[t][j][3]));
       }
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        uint32_t a0, a1, a2, a3;
-        ldsm_x4_t(vb[t] + mt_off(vr, 2 * i + vc), a0, a1, a2, a3);
+        uint32_t(&f)[4] = vf[kEarly ? t : 0][i];
+        if constexpr (!kEarly) ldsm_x4_t(vb[t] + mt_off(vr, 2 * i + vc), f[0], f[1], f[2], f[3]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) mma16816<T>(st.o[i][j], a0, a1, a2, a3, pb[j][0], pb[j][1]);
+        for (int j = 0; j < NT; ++j) mt_mma<T>(st.o[i][j], f, pb[j][0], pb[j][1]);
       }
     } else {
       for (int row = 0; row < 16; ++row) {
@@ -333,11 +387,13 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
   }
 }
 
-template <typename T, int D_, int NT>
+template <typename T, int D_, int NT, int CW>
 __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned char* base) {
   constexpr int KS = D_ / 16, NDH = D_ / 64;
-  constexpr bool kPairs = NT == 1 && D_ == 64;  // two steps an update where one has little to do
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tq = lane >> 2, n0 = 2 * (lane & 3);
+  // two steps an update (128-wide heads have too few stages to hold two, two warps a head too few registers)
+  constexpr bool kPairs = D_ == 64 && CW == 1;
+  const int warp = (threadIdx.x >> 5) / CW, c0 = (threadIdx.x >> 5) % CW * (8 * NT);  // KV head, first column
+  const int lane = threadIdx.x & 31, tq = lane >> 2, n0 = 2 * (lane & 3);
   const uint32_t hdr = smem_u32(base);
   const MtStep* recs = reinterpret_cast<const MtStep*>(base + 128);
   const uint32_t stage0 = hdr + kMtHeader;
@@ -363,7 +419,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
       // 16 ks + 2 (lane % 4) (+1) and 8 further (once a unit, while the ring fills)
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int c = 8 * j + tq, tok = c / p.G;
+        const int c = c0 + 8 * j + tq, tok = c / p.G;
         const T* q = reinterpret_cast<const T*>(p.q) + (long long)(g.q_row0 + tok) * p.q_stride +
                      (long long)(kvh * p.G + (c - tok * p.G)) * D_ + n0;
 #pragma unroll
@@ -382,9 +438,10 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
             }
             st.qf[j][ks][h] = v;
           }
-        st.m[j][0] = st.m[j][1] = -INFINITY;
+        st.m[j][0] = st.m[j][1] = 0.f;
         st.l[j][0] = st.l[j][1] = 0.f;
       }
+      st.none = (1u << (2 * NT)) - 1;
 #pragma unroll
       for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -409,7 +466,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
       const uint32_t kb[2] = {sb0 + head_region, sb1 + head_region};
       const uint32_t vb[2] = {kb[0] + L.box_bytes, kb[1] + L.box_bytes};
       const int key0[2] = {r.y, r1.y}, nv[2] = {r.z, r1.z};
-      mt_update<T, D_, NT, 2>(p, g, kb, vb, key0, nv, (r.w & kMtMasked ? 1 : 0) | (r1.w & kMtMasked ? 2 : 0), st);
+      mt_update<T, D_, NT, 2, CW == 1>(p, g, kb, vb, key0, nv, (r.w & kMtMasked ? 1 : 0) | (r1.w & kMtMasked ? 2 : 0), c0, st);
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(hdr + 64 + 8 * s0);
@@ -418,7 +475,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
     } else {
       const uint32_t kb[1] = {sb0 + head_region}, vb[1] = {kb[0] + L.box_bytes};
       const int key0[1] = {r.y}, nv[1] = {r.z};
-      mt_update<T, D_, NT, 1>(p, g, kb, vb, key0, nv, r.w & kMtMasked ? 1 : 0, st);
+      mt_update<T, D_, NT, 1, false>(p, g, kb, vb, key0, nv, r.w & kMtMasked ? 1 : 0, c0, st);
       __syncwarp();
       if (lane == 0) mbar_arrive(hdr + 64 + 8 * s0);
     }
@@ -431,7 +488,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
         float l = st.l[j][e];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const int c = 8 * j + n0 + e;
+        const int c = c0 + 8 * j + n0 + e;
         if (c >= cols) continue;
         const int tok = c / p.G, head = kvh * p.G + (c - tok * p.G);
         if (n_parts == 1) {
@@ -454,14 +511,20 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
             __stcg(rec + 16 * i + tq, st.o[i][j][e]);
             __stcg(rec + 16 * i + tq + 8, st.o[i][j][2 + e]);
           }
-          if (tq == 0) __stcg(reinterpret_cast<float2*>(rec + D_), make_float2(st.m[j][e], l));
+          if (tq == 0) __stcg(reinterpret_cast<float2*>(rec + D_), make_float2(st.none >> (2 * j + e) & 1u ? -INFINITY : st.m[j][e], l));
         }
       }
   }
 }
 
-template <typename T, int D_, int NT>
-__global__ void __launch_bounds__(D_ == 64 ? 288 : 160, D_ == 64 ? 1 : 2)
+// CW: consumer warps a KV head, each with NT tiles of 8 of the group's columns.
+// Measured on 37 trees of 7 tokens over 4096 keys (1B shape, 28 columns, 310
+// MB): one warp a head with all 32 columns 115 us (latency of one update at a
+// time: 10 cycles an instruction with two warps a scheduler), the same with 232
+// registers a thread (setmaxnreg) and two steps an update 97 us, two warps a
+// head with 16 columns each 82 us (96 registers; more steps an update spill).
+template <typename T, int D_, int NT, int CW>
+__global__ void __launch_bounds__(32 * ((D_ == 64 ? 8 : 4) * CW + 1), D_ == 64 ? 1 : 2)
     masked_tma_kernel(const MaskedParams p, const MtLaunch L, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv) {
   extern __shared__ unsigned char smem_raw[];
@@ -469,21 +532,21 @@ __global__ void __launch_bounds__(D_ == 64 ? 288 : 160, D_ == 64 ? 1 : 2)
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5;
   pdl_launch_dependents();
-  if (threadIdx.x == 32 * L.HG) {
+  if (threadIdx.x == 32 * L.HG * CW) {
     tma_prefetch_map(&tk);
     tma_prefetch_map(&tv);
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < L.stages; ++s) {
       mbar_init(smem_u32(base) + 8 * s, 1);
-      mbar_init(smem_u32(base) + 64 + 8 * s, L.HG);
+      mbar_init(smem_u32(base) + 64 + 8 * s, L.HG * CW);
     }
     fence_mbar_init();
   }
   __syncthreads();
   const int total = min(__ldg(p.counts), p.max_units) * L.n_hg;
-  if (warp < L.HG)
-    mt_consumer<T, D_, NT>(p, L, base);
+  if (warp < L.HG * CW)
+    mt_consumer<T, D_, NT, CW>(p, L, base);
   else if ((threadIdx.x & 31) == 0)
     mt_producer<D_>(p, L, &tk, &tv, base, total);
   __syncthreads();
@@ -495,13 +558,20 @@ __global__ void __launch_bounds__(D_ == 64 ? 288 : 160, D_ == 64 ? 1 : 2)
   }
 }
 
-// Query rows of a group: 32 columns of a 64-wide head fit a warp's registers
-// (accumulators 64, queries 32 of them), 16 of a 128-wide one.
+// Query rows of a group: two warps a head hold 16 columns of a 64-wide head
+// each, 8 of a 128-wide one.
 int masked_tma_rows(int dtype, int Hq, int Hkv, int D, int bs) {
   if (dtype != NF_BF16 && dtype != NF_F16) return 0;
   if ((D != 64 && D != 128) || bs % 16) return 0;
   const int rows = D == 64 ? 32 : 16;
   return Hq / Hkv <= rows ? rows : 0;
+}
+
+using MtKernel = void (*)(const MaskedParams, const MtLaunch, const CUtensorMap, const CUtensorMap);
+template <typename T>
+static MtKernel mt_kernel(int D, int cols) {
+  if (D == 128) return cols <= 8 ? masked_tma_kernel<T, 128, 1, 1> : masked_tma_kernel<T, 128, 1, 2>;
+  return cols <= 8 ? masked_tma_kernel<T, 64, 1, 1> : cols <= 16 ? masked_tma_kernel<T, 64, 2, 1> : masked_tma_kernel<T, 64, 2, 2>;
 }
 
 int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char* what) {
@@ -535,20 +605,9 @@ int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char
   L.evict_first = 1;
   L.q_align4 = (reinterpret_cast<uintptr_t>(p.q) % 4 == 0) && p.q_stride % 2 == 0;
   const int cols = p.unit_tokens * p.G;
-  using Kern = void (*)(const MaskedParams, const MtLaunch, const CUtensorMap, const CUtensorMap);
-  Kern kern;
-  if (dtype == NF_BF16) {
-    using T = __nv_bfloat16;
-    kern = p.D == 64 ? (cols <= 8 ? masked_tma_kernel<T, 64, 1> : cols <= 16 ? masked_tma_kernel<T, 64, 2>
-                                                                             : masked_tma_kernel<T, 64, 4>)
-                     : (cols <= 8 ? masked_tma_kernel<T, 128, 1> : masked_tma_kernel<T, 128, 2>);
-  } else {
-    using T = __half;
-    kern = p.D == 64 ? (cols <= 8 ? masked_tma_kernel<T, 64, 1> : cols <= 16 ? masked_tma_kernel<T, 64, 2>
-                                                                             : masked_tma_kernel<T, 64, 4>)
-                     : (cols <= 8 ? masked_tma_kernel<T, 128, 1> : masked_tma_kernel<T, 128, 2>);
-  }
-  const int threads = (hg + 1) * 32, smem = kMtHeader + L.stages * L.stage_bytes + 1024;
+  const MtKernel kern = dtype == NF_BF16 ? mt_kernel<__nv_bfloat16>(p.D, cols) : mt_kernel<__half>(p.D, cols);
+  const int cw = cols <= (p.D == 64 ? 16 : 8) ? 1 : 2;
+  const int threads = (hg * cw + 1) * 32, smem = kMtHeader + L.stages * L.stage_bytes + 1024;
   int per_sm = 1;
   cudaError_t e = prepare_launch(reinterpret_cast<const void*>(kern), smem, threads, &per_sm);
   if (e != cudaSuccess) return fail(NF_ECUDA, "%s: smem attribute: %s", what, cudaGetErrorString(e));
