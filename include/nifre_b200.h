@@ -416,15 +416,14 @@ int nf_cascade_limits(int32_t dtype, int32_t num_q_heads, int32_t num_kv_heads, 
  * 256, any block size and group size.
  *
  * Work lists (device, 16-byte aligned, built by the host once per step and
- * used by every layer):
- *   groups[max_groups][8]: slot, q_row0, ntok, pos0, ctx, n_draft, mask0,
- *     part_row0 -- ntok consecutive query tokens of one sequence, whose rows
- *     of q and out start at q_row0 and whose absolute positions start at
- *     pos0.  Tree: ctx cached keys before n_draft drafted ones; the mask rows
- *     of the group's tokens (ceil(n_draft / 32) words each) start at word
- *     mask0 of `masks`.  Rows outside [0, num_rows) are neither read nor
- *     written.
- *   units[max_units][4]: group, key_begin, key_end, part | n_parts << 16 -- a
+ * used by every layer).  A group is a run of consecutive query tokens of one
+ * sequence; its fields are G = slot, q_row0, ntok, pos0, ctx, n_draft, mask0,
+ * part_row0: ntok tokens whose rows of q and out start at q_row0 and whose
+ * absolute positions start at pos0.  Tree: ctx cached keys before n_draft
+ * drafted ones; the mask rows of the group's tokens (ceil(n_draft / 32) words
+ * each) start at word mask0 of `masks`.  Groups whose rows are not in
+ * [0, num_rows) are skipped.
+ *   units[max_units][12]: key_begin, key_end, part | n_parts << 16, 0, G -- a
  *     part of the group's keys, counted without the gap that a window leaves:
  *     with lo = max(0, pos0 - window + 1) rounded down to a multiple of 16 and
  *     kept = min(sinks rounded up to a multiple of 16, lo), key v is key v of
@@ -432,16 +431,17 @@ int nf_cascade_limits(int32_t dtype, int32_t num_q_heads, int32_t num_kv_heads, 
  *     is a multiple of 16.  A group's n_parts units cover its keys once.  At
  *     most nf_masked_limits' unit_rows query rows (ntok x heads of a KV head)
  *     a group, at most unit_tokens tokens.
- *   items[max_items][4]: the same for groups of up to item_rows query rows,
+ *   items[max_items][12]: the same for groups of up to item_rows query rows,
  *     which the tensor cores take (none where item_rows is 0); key_begin a
  *     multiple of 128.
- *   merge[max_merge][4]: q_row, part_row, n_parts, step -- a token whose keys
- *     are several units: its partial rows part_row + j * step (j < n_parts)
- *     are merged into row q_row of out.  Unit j of a group writes the partial
- *     row part_row0 + j * ntok + i for token i.
- *   counts[4]: units, items, merge rows in use, 0.
- * Workspace: ws, ws_rows partial rows of num_q_heads records of head_dim
- * rounded up to a multiple of 4, plus 4, floats; queue: int32[4], zero when
+ *   merge[max_merge][12]: n_parts, first row, kind, 0, G -- four of the rows
+ *     (token x query head of a KV head) of a group whose keys are several
+ *     units (kind 0) or items (kind 1): their partial results are merged into
+ *     out.  Part j of a group uses the partial rows part_row0 + j * ntok to
+ *     part_row0 + (j + 1) * ntok - 1.
+ *   counts[4]: units, items, merge records in use, 0.
+ * Workspace: ws (16-byte aligned), ws_rows partial rows of num_q_heads *
+ * (head_dim rounded up to a multiple of 4, plus 4) floats; queue: int32[4], zero when
  * allocated, left zero by every call (calls that share it or ws must not
  * overlap).  Bad records are skipped and flagged in *status.  Up to three
  * launches, in stream order.
@@ -454,7 +454,6 @@ typedef struct NfMaskedArgs {
   const void* k_pool;
   const void* v_pool;
   const int32_t* block_tables;
-  const int32_t* groups;
   const int32_t* units;
   const int32_t* items;
   const int32_t* merge;
@@ -467,10 +466,9 @@ typedef struct NfMaskedArgs {
   int32_t* status;
   int32_t dtype, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks;
   int32_t num_slots, max_blocks_per_seq, num_rows;
-  int32_t max_groups, max_units, unit_tokens, max_items, max_merge;
+  int32_t max_units, unit_tokens, max_items, max_merge;
   int32_t window, sinks;
   float scale;
-  int32_t pad;
 } NfMaskedArgs;
 
 int nf_window_attention(const NfMaskedArgs* args, void* stream);

@@ -80,16 +80,16 @@ class NfMaskedArgs(ctypes.Structure):
     """struct NfMaskedArgs of include/nifre_b200.h (the arguments of nf_window_attention and nf_tree_attention)."""
     _fields_ = [("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64), ("q", ctypes.c_void_p),
                 ("q_row_stride", ctypes.c_int64), ("k_pool", ctypes.c_void_p), ("v_pool", ctypes.c_void_p),
-                ("block_tables", ctypes.c_void_p), ("groups", ctypes.c_void_p), ("units", ctypes.c_void_p),
+                ("block_tables", ctypes.c_void_p), ("units", ctypes.c_void_p),
                 ("items", ctypes.c_void_p), ("merge", ctypes.c_void_p), ("counts", ctypes.c_void_p),
                 ("masks", ctypes.c_void_p), ("mask_words", ctypes.c_int64), ("ws", ctypes.c_void_p),
                 ("ws_rows", ctypes.c_int64), ("queue", ctypes.c_void_p), ("status", ctypes.c_void_p),
                 ("dtype", ctypes.c_int32), ("num_q_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
                 ("head_dim", ctypes.c_int32), ("block_size", ctypes.c_int32), ("num_blocks", ctypes.c_int32),
                 ("num_slots", ctypes.c_int32), ("max_blocks_per_seq", ctypes.c_int32), ("num_rows", ctypes.c_int32),
-                ("max_groups", ctypes.c_int32), ("max_units", ctypes.c_int32), ("unit_tokens", ctypes.c_int32),
+                ("max_units", ctypes.c_int32), ("unit_tokens", ctypes.c_int32),
                 ("max_items", ctypes.c_int32), ("max_merge", ctypes.c_int32), ("window", ctypes.c_int32),
-                ("sinks", ctypes.c_int32), ("scale", ctypes.c_float), ("pad", ctypes.c_int32)]
+                ("sinks", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
 MOVE_LIST = 128  # NF_MOVE_LIST: nf_kv_move records that travel as kernel arguments

@@ -56,12 +56,8 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
        task += (long long)gridDim.x * kVecWarps) {
     const int u = (int)(task / (p.Hkv * chunks)), rest = (int)(task - (long long)u * p.Hkv * chunks);
     const int kvh = rest / chunks, c0 = (rest - kvh * chunks) * C;
-    const int4 un = __ldg(reinterpret_cast<const int4*>(p.units) + u);
-    if (un.x < 0 || un.x >= p.max_groups) {
-      if (lane == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
-      continue;
-    }
-    const MaskedGroup g = load_group(p, un.x);
+    MaskedGroup g;
+    const int4 un = load_record(p.units, u, g);
     if (!group_ok(p, g)) {
       if (lane == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
       continue;
@@ -70,7 +66,7 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
     if (c0 >= cols) continue;
     const VirtualKeys vk(p, g);
     const int* btrow = p.bt + (long long)g.slot * p.max_blocks;
-    const int v1 = min(un.z, vk.end);
+    const int v1 = min(un.y, vk.end);
     float qr[C][E];
     int tok[C];
 #pragma unroll
@@ -102,7 +98,7 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[c][e] = 0.f;
     }
-    for (int v0 = un.y; v0 < v1; v0 += KPW * U) {
+    for (int v0 = un.x; v0 < v1; v0 += KPW * U) {
       float kx[U][E], vx[U][E];
       int key[U];
       // every load of the U steps first
@@ -166,7 +162,8 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
       }
     }
     // join the lane groups
-    const int part = un.w & 0xffff, n_parts = un.w >> 16;
+    const int part = un.z & 0xffff, n_parts = un.z >> 16;
+    float* base = n_parts > 1 ? part_base(p, g, part, kvh) : nullptr;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -193,99 +190,92 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
 #pragma unroll
             for (int i = 0; i < VW; ++i) dst[e + i] = Elem<T>::from_f(acc[c][v * VW + i] * inv);
         }
-      } else {
-        const long long prow = (long long)g.part_row0 + (long long)part * g.ntok + tok[c];
-        if (g.part_row0 < 0 || prow >= p.ws_rows) {
-          if (li == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
-          continue;
-        }
-        float* rec = part_record(p, prow, head);
+      } else if (base) {
 #pragma unroll
         for (int v = 0; v < EV; ++v) {
           const int e = (v * LPK + li) * VW;
           if (e < p.D)
 #pragma unroll
-            for (int i = 0; i < VW; ++i) rec[e + i] = acc[c][v * VW + i];
+            for (int i = 0; i < VW; ++i) base[(long long)col * p.DP + e + i] = acc[c][v * VW + i];
         }
-        if (li == 0) {
-          rec[p.DP - 4] = m[c];
-          rec[p.DP - 3] = l[c];
-        }
+        if (li == 0) *reinterpret_cast<float2*>(base + (long long)col * p.DP + p.DP - 4) = make_float2(m[c], l[c]);
       }
     }
   }
 }
 
-// Merge of split-K parts: one warp per (query row, head): out = sum_j
-// 2^(m_j - M) acc_j / sum_j 2^(m_j - M) l_j, always in the order of the parts.
-// The maxima and sums of up to 32 parts come in one load, a lane each; their
-// weights are then broadcast while the accumulators stream in.
+// Merge of split-K parts: out = sum_j 2^(m_j - M) acc_j / sum_j 2^(m_j - M)
+// l_j, always in the order of the parts.  A warp takes two rows of one
+// (group, KV head): a lane holds a float4 of one of them, so a load is whole
+// 32-byte sectors, and goes over the parts PB at a time with a running maximum
+// (one round trip to L2 per PB parts).  A merge record covers four rows.
 template <typename T>
 __global__ void __launch_bounds__(256) masked_merge_kernel(const MaskedParams p) {
+  constexpr int PB = 8;
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int n = min(__ldg(p.counts + 2), p.max_merge);
+  const int D4 = p.DP / 4 - 1;
   pdl_wait();
-  const long long tasks = (long long)n * p.Hq;
+  const long long tasks = (long long)n * p.Hkv * 2;
   for (long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); task < tasks; task += (long long)gridDim.x * 8) {
-    const int r = (int)(task / p.Hq), head = (int)(task - (long long)r * p.Hq);
-    const int4 mr = __ldg(reinterpret_cast<const int4*>(p.merge) + r);
-    const long long last = mr.y + (long long)(mr.z - 1) * mr.w;
-    if (mr.x < 0 || mr.x >= p.rows || mr.y < 0 || mr.z <= 0 || mr.w <= 0 || last >= p.ws_rows) {
+    const int i = (int)(task / (p.Hkv * 2)), rest = (int)(task - (long long)i * p.Hkv * 2), kvh = rest >> 1;
+    MaskedGroup g;
+    const int4 mr = load_record(p.merge, i, g);
+    if (!group_ok(p, g) || mr.x <= 0 || mr.y < 0) {
       if (lane == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
       continue;
     }
-    const float* rec = part_record(p, mr.y, head);
-    const long long step = (long long)mr.w * p.Hq * p.DP;  // between consecutive parts
-    // the row's maximum, then its sum and weights
-    float M = -INFINITY;
-    for (int j = lane; j < mr.z; j += 32) M = fmaxf(M, __ldcg(rec + j * step + p.DP - 4));
+    const int R = g.ntok * p.G, row = mr.y + 2 * (rest & 1) + (lane & 1);
+    if (!part_base(p, g, mr.x - 1, kvh) || row >= R) continue;
+    // float4 c of the row at c * cs + at, and (m, l) as float4 D4
+    const int cs = mr.z ? R : 1, at = mr.z ? row : row * (D4 + 1);
+    const float4* base = reinterpret_cast<const float4*>(part_base(p, g, 0, kvh)) + at;
+    const long long step = (long long)g.ntok * p.Hq * (D4 + 1);  // float4s between consecutive parts
+    const int tok = row / p.G;
+    T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride +
+             (long long)(kvh * p.G + row - tok * p.G) * p.D;
+    for (int c = lane >> 1; c < D4; c += 16) {
+      float M = -INFINITY, L = 0.f;
+      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j = 0; j < mr.x; j += PB) {
+        float4 x[PB];
+        float2 ml[PB];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f, a[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = 0.f;
-    const int D2 = (p.D + 63) >> 6;  // pairs of elements a lane holds
-    for (int j0 = 0; j0 < mr.z; j0 += 32) {
-      float w = 0.f, lw = 0.f;
-      if (j0 + lane < mr.z) {
-        const float mj = __ldcg(rec + (j0 + lane) * step + p.DP - 4);
-        w = mj == -INFINITY ? 0.f : ex2(mj - base);
-        lw = w * __ldcg(rec + (j0 + lane) * step + p.DP - 3);
-        if (mj == -INFINITY) lw = 0.f;
-      }
-      // in the order of the parts, the same whatever the launch
-      const int jn = min(32, mr.z - j0);
-      for (int j = 0; j < jn; j += 4) {
-        float x[4][8], wj[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          wj[u] = j + u < jn ? __shfl_sync(0xffffffffu, w, j + u) : 0.f;
-          L += j + u < jn ? __shfl_sync(0xffffffffu, lw, j + u) : 0.f;
-          const float* pj = rec + (long long)(j0 + j + u) * step;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int e = (i * 32 + lane) * 2;  // (records are padded to whole pairs)
-            const bool in = i < D2 && e < p.D && j + u < jn && wj[u] != 0.f;
-            const float2 v = in ? __ldcg(reinterpret_cast<const float2*>(pj + e)) : make_float2(0.f, 0.f);
-            x[u][2 * i] = v.x;
-            x[u][2 * i + 1] = v.y;
+        for (int u = 0; u < PB; ++u)
+          if (j + u < mr.x) {
+            const float4* pj = base + (j + u) * step;
+            ml[u] = __ldcg(reinterpret_cast<const float2*>(pj + D4 * cs));
+            x[u] = __ldcg(pj + c * cs);
+          } else {
+            ml[u] = make_float2(-INFINITY, 0.f);
           }
-        }
+        float nm = M;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < PB; ++u) nm = fmaxf(nm, ml[u].x);
+        const float b = nm == -INFINITY ? 0.f : nm, sc = ex2(M - b);
+        A.x *= sc; A.y *= sc; A.z *= sc; A.w *= sc; L *= sc;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) a[i] = fmaf(wj[u], x[u][i], a[i]);
+        for (int u = 0; u < PB; ++u)
+          if (ml[u].x != -INFINITY) {  // (a part without seen keys)
+            const float w = ex2(ml[u].x - b);
+            A.x = fmaf(x[u].x, w, A.x); A.y = fmaf(x[u].y, w, A.y);
+            A.z = fmaf(x[u].z, w, A.z); A.w = fmaf(x[u].w, w, A.w);
+            L = fmaf(ml[u].y, w, L);
+          }
+        M = nm;
       }
-    }
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-    T* dst = reinterpret_cast<T*>(p.out) + (long long)mr.x * p.out_stride + (long long)head * p.D;
+      const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+      const float o[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
+      T* d = dst + 4 * c;
+      if (sizeof(T) == 2 && 4 * c + 4 <= p.D && (reinterpret_cast<uintptr_t>(d) & 7) == 0) {
+        if constexpr (sizeof(T) == 2)
+          *reinterpret_cast<uint2*>(d) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
+      } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = (i * 32 + lane) * 2;
-      if (e < p.D) dst[e] = Elem<T>::from_f(a[2 * i] * inv);
-      if (e + 1 < p.D) dst[e + 1] = Elem<T>::from_f(a[2 * i + 1] * inv);
+        for (int e = 0; e < 4; ++e)
+          if (4 * c + e < p.D) d[e] = Elem<T>::from_f(o[e]);
+      }
     }
   }
 }
@@ -350,12 +340,12 @@ static int masked_check(const NfMaskedArgs* a, bool tree, const char* what, Mask
     return fail(NF_EUNSUPPORTED, "%s: head_dim %d (1 to 256)", what, a->head_dim);
   if (a->block_size <= 0 || a->num_blocks <= 0 || a->max_blocks_per_seq <= 0 || a->num_slots <= 0 || a->num_rows <= 0)
     return fail(NF_EINVAL, "%s: sizes must be positive", what);
-  if (a->max_groups <= 0 || a->max_units < 0 || a->max_items < 0 || a->max_merge < 0 || a->ws_rows < 0 ||
+  if (a->max_units < 0 || a->max_items < 0 || a->max_merge < 0 || a->ws_rows < 0 ||
       a->max_units + (int64_t)a->max_items <= 0)
     return fail(NF_EINVAL, "%s: work list sizes must not be negative, and not all zero", what);
   if (a->max_units && (a->unit_tokens <= 0 || (int64_t)a->unit_tokens * a->num_q_heads > (1 << 20)))
     return fail(NF_EINVAL, "%s: unit_tokens (%d) must be positive, and at most 2^20 / num_q_heads", what, a->unit_tokens);
-  if (!a->out || !a->q || !a->k_pool || !a->v_pool || !a->block_tables || !a->groups || !a->counts || !a->queue ||
+  if (!a->out || !a->q || !a->k_pool || !a->v_pool || !a->block_tables || !a->counts || !a->queue ||
       !a->status || (a->max_units && !a->units) || (a->max_items && !a->items) || (a->max_merge && !a->merge) ||
       (a->ws_rows && !a->ws))
     return fail(NF_EINVAL, "%s: null pointer argument", what);
@@ -364,7 +354,7 @@ static int masked_check(const NfMaskedArgs* a, bool tree, const char* what, Mask
   if (!tree && (a->window <= 0 || a->sinks < 0))
     return fail(NF_EINVAL, "%s: window (%d) must be positive and sinks (%d) not negative", what, a->window, a->sinks);
   auto al = [](const void* ptr, size_t n) { return (reinterpret_cast<uintptr_t>(ptr) % n) == 0; };
-  if (!al(a->groups, 16) || !al(a->units, 16) || !al(a->items, 16) || !al(a->merge, 16) || !al(a->ws, 16) ||
+  if (!al(a->units, 16) || !al(a->items, 16) || !al(a->merge, 16) || !al(a->ws, 16) ||
       !al(a->masks, 4) || !al(a->counts, 4))
     return fail(NF_EINVAL, "%s: work lists and workspace must be 16-byte aligned", what);
   if (!al(a->q, es) || !al(a->out, es) || !al(a->k_pool, es) || !al(a->v_pool, es))
@@ -386,8 +376,6 @@ static int masked_check(const NfMaskedArgs* a, bool tree, const char* what, Mask
   p.bt = a->block_tables;
   p.num_slots = a->num_slots;
   p.max_blocks = a->max_blocks_per_seq;
-  p.groups = a->groups;
-  p.max_groups = a->max_groups;
   p.units = a->units;
   p.max_units = a->max_units;
   p.unit_tokens = a->unit_tokens;
@@ -430,7 +418,7 @@ static int masked_attention(const NfMaskedArgs* a, bool tree, const char* what, 
     if (rc) return rc;
   }
   if (p.max_merge) {
-    const long long want = ((long long)p.max_merge * p.Hq + 7) / 8, cap = (long long)sm_count() * 8;
+    const long long want = ((long long)p.max_merge * p.Hkv * 2 + 7) / 8, cap = (long long)sm_count() * 8;
     const long long blocks = want < cap ? want : cap;
     switch (a->dtype) {
       case NF_F32: return launch_masked(masked_merge_kernel<float>, blocks, 256, st, p, what);

@@ -33,21 +33,19 @@ struct MaskedParams {
   int Hq, Hkv, D, G, bs, num_blocks;
   const int* bt;
   int num_slots, max_blocks;
-  const int* groups;  // [max_groups][8]: slot, q_row0, ntok, pos0, ctx, n_draft, mask0, part_row0
-  int max_groups;
-  const int* units;  // [max_units][4]: group, key_begin, key_end (virtual), part | n_parts << 16
+  const int* units;  // [max_units][12]: key_begin, key_end (virtual), part | n_parts << 16, 0, group fields
   int max_units;
   int unit_tokens;    // the most query tokens of a unit's group
-  const int* items;   // [max_items][4]: the tensor-core path's units
+  const int* items;   // [max_items][12]: the tensor-core path's units
   int max_items;
-  const int* merge;  // [max_merge][4]: q_row, part_row0, n_parts, rows between an item's parts
+  const int* merge;  // [max_merge][12]: n_parts, first row, kind (1: items), 0, group fields
   int max_merge;
-  const int* counts;  // units, tensor-core items, merge rows, partial rows
+  const int* counts;  // units, items, merge records in use
   const uint32_t* masks;
   long long mask_words;
   int tree, window, sinks;
   float scale_log2;
-  float* ws;  // partial rows [part row][Hq][DP]: acc[D], m, l
+  float* ws;  // partial rows (see part_base): ws_rows x Hq x DP floats
   long long ws_rows;
   int DP;
   int* queue;  // work queue of the persistent kernels; zero between launches
@@ -58,10 +56,12 @@ struct MaskedGroup {
   int slot, q_row0, ntok, pos0, ctx, n_draft, mask0, part_row0;
 };
 
-__device__ __forceinline__ MaskedGroup load_group(const MaskedParams& p, int g) {
-  const int4* r = reinterpret_cast<const int4*>(p.groups) + 2 * g;
-  const int4 a = __ldg(r), b = __ldg(r + 1);
-  return MaskedGroup{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// Record i of a work list: its own four fields and its group's, in one round trip.
+__device__ __forceinline__ int4 load_record(const int* list, int i, MaskedGroup& g) {
+  const int4* r = reinterpret_cast<const int4*>(list) + 3 * (long long)i;
+  const int4 h = __ldg(r), a = __ldg(r + 1), b = __ldg(r + 2);
+  g = MaskedGroup{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  return h;
 }
 
 // The group's own bounds against the buffers that the call gave.
@@ -116,9 +116,18 @@ __device__ __forceinline__ long long key_row(const MaskedParams& p, const int* b
   return (long long)phys * p.bs + (k - lb * p.bs);
 }
 
-// Partial record of (partial row, query head).
-__device__ __forceinline__ float* part_record(const MaskedParams& p, long long row, int head) {
-  return p.ws + (row * p.Hq + head) * p.DP;
+// Partial results of part `part` of a group for one KV head, R = ntok * G rows
+// (row = token * G + query head) of DP / 4 float4s: D4 of elements, then (m, l).
+// Units store them row by row; items, whose threads hold a row each, store
+// float4 c of row r at c * R + r, so that a store is whole lines.  nullptr
+// (flagged) where the workspace ends.
+__device__ __forceinline__ float* part_base(const MaskedParams& p, const MaskedGroup& g, int part, int kvh) {
+  const long long row = (long long)g.part_row0 + (long long)part * g.ntok;
+  if (g.part_row0 < 0 || row + g.ntok > p.ws_rows) {
+    atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
+    return nullptr;
+  }
+  return p.ws + (row * p.Hq + (long long)kvh * g.ntok * p.G) * p.DP;
 }
 
 // The tensor-map path (NF_EUNSUPPORTED, nothing launched: not for this shape).

@@ -85,17 +85,22 @@ struct TcItem {
   MaskedGroup g;
   VirtualKeys vk;
   int kvh, k0, k1, part, nkt, n_half;
+  int whole0, whole1;  // tiles that every row sees wholly: [whole0, whole1)
   bool bad, dup;
-  __device__ TcItem(const MaskedParams& p, int item, int4 un, const MaskedGroup& gr, bool known, int TT)
+  __device__ TcItem(const MaskedParams& p, int item, int4 un, const MaskedGroup& gr, int TT)
       : g(gr), vk(p, gr) {
     kvh = item % p.Hkv;
-    k0 = un.y;
-    k1 = min(un.z, vk.end);
-    part = un.w;
-    bad = !known || !group_ok(p, g) || k0 < 0 || (k0 & 15) || k0 >= k1 || g.ntok > 2 * TT;
+    k0 = un.x;
+    k1 = min(un.y, vk.end);
+    part = un.z;
+    bad = !group_ok(p, g) || k0 < 0 || (k0 & 15) || k0 >= k1 || g.ntok > 2 * TT;
     nkt = bad ? 0 : (k1 - k0 + 127) >> 7;
     n_half = g.ntok > TT ? 2 : 1;
     dup = n_half == 1 && nkt > 1;
+    const int v_lo = p.tree ? 0 : max(vk.kept, g.pos0 + g.ntok - p.window - vk.gap);
+    const int v_hi = min(k1, p.tree ? g.ctx : g.pos0 + 1 - vk.gap);
+    whole0 = max(v_lo - k0 + 127, 0) >> 7;
+    whole1 = max(v_hi - k0, 0) >> 7;
   }
   __device__ __forceinline__ bool active(int h, int j) const {
     return j >= 0 && j < nkt && (dup ? (j & 1) == h : h < n_half);
@@ -104,15 +109,8 @@ struct TcItem {
   __device__ __forceinline__ int tiles(int h) const {
     return dup ? (nkt + 1 - h) >> 1 : (h < n_half ? nkt : 0);
   }
-  // whether some row of the group does not see the whole of tile j
-  __device__ __forceinline__ bool masked(const MaskedParams& p, int j) const {
-    const int v0 = k0 + 128 * j, v1 = v0 + 127;
-    if (v1 >= k1) return true;
-    if (p.tree) return v1 >= g.ctx;
-    if (v0 < vk.kept) return v1 >= vk.kept || v1 >= p.sinks;
-    const int key0 = v0 + vk.gap, key1 = v1 + vk.gap;
-    return key1 > g.pos0 || !(key0 > g.pos0 + g.ntok - 1 - p.window || key1 < p.sinks);
-  }
+  // whether some row of the group may not see the whole of tile j
+  __device__ __forceinline__ bool masked(int j) const { return j < whole0 || j >= whole1; }
   // the half that looks masked tile j's values over (it is active there)
   __device__ __forceinline__ int keeper(int j) const { return dup ? j & 1 : n_half - 1; }
 };
@@ -163,19 +161,18 @@ __device__ __noinline__ bool seen_by_any(const MaskedParams& p, const MaskedGrou
 }
 
 // The ring that hands items to the CTA's warps; a slot holds the item number
-// (-1: no more), its unit, whether its group is known, and the group.
+// (-1: no more) and the unit's record.
 struct TcRing {
   const TcBars& bar;
   unsigned char* slots;
   Ring r;
   __device__ TcRing(const TcBars& b, unsigned char* base) : bar(b), slots(base + kTcSlots) {}
   __device__ int4* slot(int st) const { return reinterpret_cast<int4*>(slots + 64 * st); }
-  __device__ bool next(int& item, int4& un, MaskedGroup& g, bool& known, int* status) {
+  __device__ bool next(int& item, int4& un, MaskedGroup& g, int* status) {
     if (!mbar_wait(bar.item_full(r.st), r.ph, status)) return false;
     const int4* sl = slot(r.st);
     const int4 a = sl[0], b = sl[1], c = sl[2], d = sl[3];
     item = a.x;
-    known = a.y != 0;
     un = b;
     g = MaskedGroup{c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w};
     __syncwarp();
@@ -186,7 +183,7 @@ struct TcRing {
 };
 
 __device__ __forceinline__ bool tc_claim(const MaskedParams& p, TcRing& ring, int n_items, int& claims, int& item,
-                                         int4& un, MaskedGroup& g, bool& known) {
+                                         int4& un, MaskedGroup& g) {
   const int lane = threadIdx.x & 31;
   int pos = blockIdx.x;  // the first item is the CTA's own, the queue hands out the rest
   if (claims > 0) {
@@ -197,16 +194,11 @@ __device__ __forceinline__ bool tc_claim(const MaskedParams& p, TcRing& ring, in
   item = pos < n_items ? pos : -1;
   un = make_int4(0, 0, 0, 0);
   g = MaskedGroup{};
-  known = false;
-  if (item >= 0) {
-    un = __ldg(reinterpret_cast<const int4*>(p.items) + item / p.Hkv);
-    known = un.x >= 0 && un.x < p.max_groups;
-    if (known) g = load_group(p, un.x);
-  }
+  if (item >= 0) un = load_record(p.items, item / p.Hkv, g);
   if (!mbar_wait(ring.bar.item_empty(ring.r.st), ring.r.ph ^ 1, p.status)) return false;
   if (lane == 0) {
     int4* sl = ring.slot(ring.r.st);
-    sl[0] = make_int4(item, known, 0, 0);
+    sl[0] = make_int4(item, 0, 0, 0);
     sl[1] = un;
     sl[2] = make_int4(g.slot, g.q_row0, g.ntok, g.pos0);
     sl[3] = make_int4(g.ctx, g.n_draft, g.mask0, g.part_row0);
@@ -288,12 +280,11 @@ __device__ void tc_producer(const MaskedParams& p, int TT, bool q_tma, const CUt
   int it, claims = 0;
   int4 un;
   MaskedGroup g;
-  bool known;
   pdl_wait();  // queries, keys and values may come from the launch before this one
-  while (tc_claim(p, ring, n_items, claims, it, un, g, known)) {
-    const TcItem w(p, it, un, g, known, TT);
+  while (tc_claim(p, ring, n_items, claims, it, un, g)) {
+    const TcItem w(p, it, un, g, TT);
     if (w.bad) {
-      if (lane == 0) atomicOr(p.status, known ? NF_STATUS_BAD_SLOT : NF_STATUS_UNIT_OVERFLOW);
+      if (lane == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
       continue;
     }
     const int* btrow = p.bt + (long long)w.g.slot * p.max_blocks;
@@ -378,9 +369,8 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
   int it;
   int4 un;
   MaskedGroup g;
-  bool known;
-  while (ring.next(it, un, g, known, p.status)) {
-    const TcItem w(p, it, un, g, known, TT);
+  while (ring.next(it, un, g, p.status)) {
+    const TcItem w(p, it, un, g, TT);
     if (w.bad) continue;
     int vprev = -1;  // V stage of tile j-1
     bool waited = false;  // tile j-1's weights were waited for already
@@ -396,7 +386,7 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
     for (int j = 0; j < w.nkt; ++j) {
       if (!mbar_wait(bar.k_full(kr.st), kr.ph, p.status)) return;
       waited = false;
-      if (C::P_ALIAS && j > 0 && !w.dup && w.masked(p, j - 1)) {
+      if (C::P_ALIAS && j > 0 && !w.dup && w.masked(j - 1)) {
         if (!wait_all(j - 1)) return;
         waited = true;
       }
@@ -420,7 +410,7 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
       if (j > 0) {
         if (!C::P_ALIAS || w.dup) {
           // (dup: half h's weights of tile j-2 in S_h were consumed before S_h of tile j was issued)
-          if (w.masked(p, j - 1)) {
+          if (w.masked(j - 1)) {
             if (!wait_all(j - 1)) return;
             waited = true;
           }
@@ -481,13 +471,11 @@ __device__ __noinline__ void tc_row_again(const MaskedParams& p, const MaskedGro
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride + (long long)head * D_;
     for (int d = 0; d < D_; ++d) dst[d] = Elem<T>::from_f(acc[d] * inv);
-  } else {
-    const long long prow = (long long)g.part_row0 + (long long)(part & 0xffff) * g.ntok + tok;
-    if (g.part_row0 < 0 || prow >= p.ws_rows) return;
-    float* rec = part_record(p, prow, head);
-    for (int d = 0; d < D_; ++d) rec[d] = acc[d];
-    rec[D_] = m;
-    rec[D_ + 1] = l;
+  } else if (float* rec = part_base(p, g, part & 0xffff, kvh)) {
+    const int R = g.ntok * p.G, r = tok * p.G + hd;
+    for (int d = 0; d < D_; ++d) rec[((d >> 2) * R + r) * 4 + (d & 3)] = acc[d];
+    rec[(D_ / 4 * R + r) * 4] = m;
+    rec[(D_ / 4 * R + r) * 4 + 1] = l;
   }
 }
 
@@ -512,9 +500,8 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
   int it, seq = 0;
   int4 un;
   MaskedGroup g;
-  bool known;
-  while (ring.next(it, un, g, known, p.status)) {
-    const TcItem w(p, it, un, g, known, TT);
+  while (ring.next(it, un, g, p.status)) {
+    const TcItem w(p, it, un, g, TT);
     if (w.bad) continue;
     ++seq;
     const Ring v0r = vr;  // V stage of the item's first tile
@@ -543,7 +530,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
 #pragma unroll
         for (int i = 0; i < 128; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * p.scale_log2);
       }
-      const bool masked = w.masked(p, j);
+      const bool masked = w.masked(j);
       if (masked) {
         uint32_t bits[4] = {0u, 0u, 0u, 0u};
         if (valid) row_bits(p, w, tok, j, bits);
@@ -664,61 +651,89 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
       l = l * a0 + other.y * a1;
       m = mn;
     }
-    const int n_parts = w.part >> 16;
-    const long long prow = (long long)w.g.part_row0 + (long long)(w.part & 0xffff) * w.g.ntok + tok;
-    float* rec = nullptr;
-    if (valid && n_parts > 1) {
-      if (w.g.part_row0 < 0 || prow >= p.ws_rows)
-        atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
-      else
-        rec = part_record(p, prow, w.kvh * p.G + hd);
-    }
+    const int n_parts = w.part >> 16, R = w.g.ntok * p.G, r = tok * p.G + hd;
+    float4* rec = nullptr;
+    // the row's place in out, in elements (-1: not a row)
+    long long at = -1;
     if (n_parts == 1) {
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       a0 *= inv;
       a1 *= inv;
+      if (valid) at = (long long)(w.g.q_row0 + tok) * p.out_stride + (long long)(w.kvh * p.G + hd) * D_;
+    } else if (valid) {
+      rec = reinterpret_cast<float4*>(part_base(p, w.g, w.part & 0xffff, w.kvh));
     }
-    T* dst = reinterpret_cast<T*>(p.out) + (long long)(w.g.q_row0 + tok) * p.out_stride + (long long)(w.kvh * p.G + hd) * D_;
 #pragma unroll
-    for (int c = 0; c < D_ / 32; ++c) {
-      uint32_t o[32];
-      tmem_ld32(o_addr + c * 32, o);
+    for (int c = 0; c < D_ / 64; ++c) {
+      uint32_t o[64];
+      tmem_ld32(o_addr + c * 64, *reinterpret_cast<uint32_t(*)[32]>(o));
+      tmem_ld32(o_addr + c * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
       tmem_wait_ld();
-      tmem_reg_fence(o);
+      tmem_reg_fence(*reinterpret_cast<uint32_t(*)[32]>(o));
+      tmem_reg_fence(*reinterpret_cast<uint32_t(*)[32]>(o + 32));
       if (w.dup) {
-        uint32_t o1[32];
-        tmem_ld32(o_addr - C::o_col(0) + C::o_col(1) + c * 32, o1);
-        tmem_wait_ld();
-        tmem_reg_fence(o1);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          o[i] = __float_as_uint(fmaf(__uint_as_float(o1[i]), a1, __uint_as_float(o[i]) * a0));
+        for (int b = 0; b < 2; ++b) {
+          uint32_t o1[32];
+          tmem_ld32(o_addr - C::o_col(0) + C::o_col(1) + c * 64 + b * 32, o1);
+          tmem_wait_ld();
+          tmem_reg_fence(o1);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            o[32 * b + i] = __float_as_uint(fmaf(__uint_as_float(o1[i]), a1, __uint_as_float(o[32 * b + i]) * a0));
+        }
       } else if (n_parts == 1) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a0);
+        for (int i = 0; i < 64; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * a0);
       }
-      if (rec) {
-        float4* r4 = reinterpret_cast<float4*>(rec + c * 32);
+      if (n_parts > 1) {
+        if (rec) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          __stcg(r4 + i, make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                     __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
-      } else if (valid && n_parts == 1) {
+          for (int i = 0; i < 16; ++i)  // lanes are rows: 512 contiguous bytes a store
+            __stcg(rec + (c * 16 + i) * R + r, make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                          __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3])));
+        }
+        continue;
+      }
+      // eight lanes exchange 16-byte pieces (an 8 x 8 transpose in three steps), so that they store one row's 128
+      // bytes together instead of a piece of eight rows each
+      uint32_t v[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = pack2<T>(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+#pragma unroll
+      for (int st = 1; st < 8; st <<= 1) {
+        const bool up = lane & st;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (q & st) continue;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t &lo = v[4 * q + e], &hi = v[4 * (q ^ st) + e];
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, st);
+            if (up)
+              lo = got;
+            else
+              hi = got;
+          }
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const long long row_at = __shfl_sync(0xffffffffu, at, (lane & ~7) + q);
+        if (row_at < 0) continue;
+        T* d = reinterpret_cast<T*>(p.out) + row_at + c * 64 + (lane & 7) * 8;
         if (out16) {
-          uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            d4[i] = make_uint4(pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])),
-                               pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3])),
-                               pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])),
-                               pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
+          *reinterpret_cast<uint4*>(d) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) dst[c * 32 + i] = Elem<T>::from_f(__uint_as_float(o[i]));
+          for (int e = 0; e < 4; ++e) {
+            reinterpret_cast<unsigned short*>(d)[2 * e] = v[4 * q + e] & 0xffff;
+            reinterpret_cast<unsigned short*>(d)[2 * e + 1] = v[4 * q + e] >> 16;
+          }
         }
       }
     }
-    if (rec) __stcg(reinterpret_cast<float2*>(rec + D_), make_float2(m, l));
+    if (rec) __stcg(reinterpret_cast<float2*>(rec + D_ / 4 * R + r), make_float2(m, l));
     tc_fence_before();
     if (w.dup) {
       __syncwarp();

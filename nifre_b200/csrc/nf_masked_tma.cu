@@ -70,68 +70,50 @@ __device__ __forceinline__ uint32_t mt_transpose(uint32_t x) {
 
 template <int D_>
 __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUtensorMap* tk, const CUtensorMap* tv,
-                            unsigned char* base, int total) {
+                            unsigned char* base) {
   constexpr int NDH = D_ / 64;
   const uint32_t hdr = smem_u32(base);
   auto full = [&](int s) { return hdr + 8 * s; };
   auto empty = [&](int s) { return hdr + 64 + 8 * s; };
   MtStep* recs = reinterpret_cast<MtStep*>(base + 128);
   const uint32_t stage0 = hdr + kMtHeader;
-  // the switch to the next unit needs four dependent round trips (ticket,
-  // unit, group, block id): each is asked for kGap steps after the one before
+  // the switch to the next unit needs three dependent round trips (ticket,
+  // record, block id): each is asked for kGap steps after the one before
   constexpr int kGap = 2, kAhead = 4 * kGap;
   const uint64_t pol = L.evict_first ? l2_evict_first() : l2_evict_last();
-  const int4* units = reinterpret_cast<const int4*>(p.units);
   int k = 0, s = 0;
   uint32_t pe = 1;
   bool ok = true;
   int w = blockIdx.x;
-  int4 un = make_int4(0, 0, 0, 0);
-  MaskedGroup g{};
-  bool good = false;
-  auto fetch_group = [&](const int4& unit, MaskedGroup& gr) {
-    const bool in = unit.x >= 0 && unit.x < p.max_groups;
-    if (in) gr = load_group(p, unit.x);
-    return in;
-  };
-  if (w < total) {
-    un = __ldg(units + w / L.n_hg);
-    good = fetch_group(un, g);
-  }
+  MaskedGroup g;
+  int4 un = load_record(p.units, min(w / L.n_hg, p.max_units - 1), g);  // (before the count is known: no matter)
+  const int total = min(__ldg(p.counts), p.max_units) * L.n_hg;
   pdl_wait();
   while (w < total) {
     const int u = w / L.n_hg, hg = w - u * L.n_hg, h0 = hg * L.HG;
-    if (!good || !group_ok(p, g)) {
-      atomicOr(p.status, good ? NF_STATUS_BAD_SLOT : NF_STATUS_UNIT_OVERFLOW);
+    if (!group_ok(p, g)) {
+      atomicOr(p.status, NF_STATUS_BAD_SLOT);
       w = (int)gridDim.x + atomicAdd(p.queue, 1);
-      if (w < total) {
-        un = __ldg(units + w / L.n_hg);
-        good = fetch_group(un, g);
-      }
+      if (w < total) un = load_record(p.units, w / L.n_hg, g);
       continue;
     }
     const VirtualKeys vk(p, g);
-    const int v1 = min(un.z, vk.end);
+    const int v1 = min(un.y, vk.end);
     const int* btrow = p.bt + (long long)g.slot * p.max_blocks;
-    const int nsteps = max(1, (v1 - un.y + 15) >> 4);  // (a unit without keys still ends in an epilogue)
+    const int nsteps = max(1, (v1 - un.x + 15) >> 4);  // (a unit without keys still ends in an epilogue)
     const int ask = nsteps - 1 - min(kAhead, nsteps - 1);
     int wn = total;
     int4 nu = make_int4(0, 0, 0, 0);
     MaskedGroup ng{};
-    bool ngood = false;
-    int have = 0;  // what is known of the next unit: 1 ticket, 2 unit, 3 group
-    for (int i = 0, v = un.y; i < nsteps; ++i, v += 16, ++k) {
+    bool have = false;  // the next unit's record is here
+    for (int i = 0, v = un.x; i < nsteps; ++i, v += 16, ++k) {
       if (i == ask) {
         wn = (int)gridDim.x + atomicAdd(p.queue, 1);
-        have = 1;
       } else if (i == ask + kGap && wn < total) {
-        nu = __ldg(units + wn / L.n_hg);
-        have = 2;
-      } else if (i == ask + 2 * kGap && wn < total) {
-        ngood = fetch_group(nu, ng);
-        have = 3;
-      } else if (i == ask + 3 * kGap && wn < total && ngood && ng.slot >= 0 && ng.slot < p.num_slots) {
-        const int lb = VirtualKeys(p, ng).key(nu.y) / p.bs;
+        nu = load_record(p.units, wn / L.n_hg, ng);
+        have = true;
+      } else if (i == ask + 2 * kGap && wn < total && ng.slot >= 0 && ng.slot < p.num_slots) {
+        const int lb = VirtualKeys(p, ng).key(nu.x) / p.bs;
         if (lb >= 0 && lb < p.max_blocks)
           asm volatile("prefetch.global.L1 [%0];" ::"l"(p.bt + (long long)ng.slot * p.max_blocks + lb));
       }
@@ -156,7 +138,7 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
           make_int4(u, key0, nv, (i == 0 ? kMtFirst : 0) | (i == nsteps - 1 ? kMtLast : 0) | (whole ? 0 : kMtMasked));
       if (i == 0) {
         reinterpret_cast<int4*>(&r)[1] = make_int4(g.q_row0, g.ntok, g.pos0, g.ctx);
-        reinterpret_cast<int4*>(&r)[2] = make_int4(g.n_draft, g.mask0, g.part_row0, un.w);
+        reinterpret_cast<int4*>(&r)[2] = make_int4(g.n_draft, g.mask0, g.part_row0, un.z);
         r.hg = hg;
       }
       const int off = key0 - lb * p.bs;
@@ -190,14 +172,10 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
       }
     }
     if (!ok) break;
-    if (wn < total) {  // a short unit: what the steps did not get to
-      if (have < 2) nu = __ldg(units + wn / L.n_hg);
-      if (have < 3) ngood = fetch_group(nu, ng);
-    }
+    if (wn < total && !have) nu = load_record(p.units, wn / L.n_hg, ng);  // a short unit
     w = wn;
     un = nu;
     g = ng;
-    good = ngood;
   }
   if (ok && mbar_wait(empty(s), pe, p.status)) {
     recs[s].u = -1;
@@ -481,6 +459,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
     }
     if (!last) continue;
     const int cols = g.ntok * p.G, n_parts = part >> 16;
+    float* rec = n_parts > 1 ? part_base(p, g, part & 0xffff, kvh) : nullptr;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -499,19 +478,16 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
             dst[16 * i] = Elem<T>::from_f(st.o[i][j][e] * inv);
             dst[16 * i + 8] = Elem<T>::from_f(st.o[i][j][2 + e] * inv);
           }
-        } else {
-          const long long row = (long long)g.part_row0 + (long long)(part & 0xffff) * g.ntok + tok;
-          if (g.part_row0 < 0 || row >= p.ws_rows) {
-            atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
-            continue;
-          }
-          float* rec = part_record(p, row, head);
+        } else if (rec) {
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
-            __stcg(rec + 16 * i + tq, st.o[i][j][e]);
-            __stcg(rec + 16 * i + tq + 8, st.o[i][j][2 + e]);
+            const int d = 16 * i + tq;
+            __stcg(rec + c * (D_ + 4) + d, st.o[i][j][e]);
+            __stcg(rec + c * (D_ + 4) + d + 8, st.o[i][j][2 + e]);
           }
-          if (tq == 0) __stcg(reinterpret_cast<float2*>(rec + D_), make_float2(st.none >> (2 * j + e) & 1u ? -INFINITY : st.m[j][e], l));
+          if (tq == 0)
+            __stcg(reinterpret_cast<float2*>(rec + c * (D_ + 4) + D_),
+                   make_float2(st.none >> (2 * j + e) & 1u ? -INFINITY : st.m[j][e], l));
         }
       }
   }
@@ -544,11 +520,10 @@ __global__ void __launch_bounds__(32 * ((D_ == 64 ? 8 : 4) * CW + 1), D_ == 64 ?
     fence_mbar_init();
   }
   __syncthreads();
-  const int total = min(__ldg(p.counts), p.max_units) * L.n_hg;
   if (warp < L.HG * CW)
     mt_consumer<T, D_, NT, CW>(p, L, base);
   else if ((threadIdx.x & 31) == 0)
-    mt_producer<D_>(p, L, &tk, &tv, base, total);
+    mt_producer<D_>(p, L, &tk, &tv, base);
   __syncthreads();
   // the last CTA out rewinds the queue (every ticket of every CTA is taken)
   if (threadIdx.x == 0 && atomicAdd(p.queue + 1, 1) == (int)gridDim.x - 1) {

@@ -83,35 +83,36 @@ def even_shares(keys, share: int, align: int, least: int):
 
 
 class WorkLists:
-    """Groups, units, tensor-core items and merge rows of one step, and their place in one int32 buffer."""
+    """Units, tensor-core items and merge records of one step (each record with its group's fields), the mask words,
+    and their place in one int32 buffer."""
 
-    def __init__(self, groups, units, items, merge, part_rows: int, unit_tokens: int, masks):
-        self.groups, self.units, self.items, self.merge, self.masks = groups, units, items, merge, masks
+    def __init__(self, units, items, merge, masks, part_rows: int, unit_tokens: int):
+        self.units, self.items, self.merge, self.masks = units, items, merge, masks
         self.part_rows, self.unit_tokens = part_rows, unit_tokens
 
     def sizes(self):
         """Entries of each list, the partial rows and the tokens of the largest unit's group."""
-        return (len(self.groups), len(self.units), len(self.items), len(self.merge), len(self.masks), self.part_rows,
-                self.unit_tokens)
+        return (len(self.units), len(self.items), len(self.merge), len(self.masks), self.part_rows, self.unit_tokens)
 
     @staticmethod
     def room(sizes):
         """Capacities for lists of these sizes: whole multiples of 64 entries, so that the next steps' lists of the
         same batch fit as well (the launches are sized by the capacities)."""
-        up = [-(-n // 64) * 64 for n in sizes[:6]]
-        return (*up, sizes[6])
+        return (*(-(-n // 64) * 64 for n in sizes[:5]), sizes[5])
 
     @staticmethod
     def offsets(room):
         """Start of each list in the buffer and its length."""
-        at = np.cumsum([HEAD, 8 * room[0], 4 * room[1], 4 * room[2], 4 * room[3], -(-room[4] // 4) * 4]).tolist()
-        return at[:5], at[5]
+        at = [HEAD]
+        for n in (12 * room[0], 12 * room[1], 12 * room[2], -(-room[3] // 4) * 4):
+            at.append(at[-1] + n)
+        return at[:4], at[4]
 
     def pack(self, room) -> np.ndarray:
         at, total = self.offsets(room)
         host = np.zeros(total, dtype=np.int32)
-        host[:4] = (len(self.units), len(self.items), len(self.merge), 0)
-        for start, part in zip(at, (self.groups, self.units, self.items, self.merge, self.masks)):
+        host[:3] = (len(self.units), len(self.items), len(self.merge))
+        for start, part in zip(at, (self.units, self.items, self.merge, self.masks)):
             host[start:start + part.size] = part.reshape(-1)
         return host
 
@@ -169,15 +170,16 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
         n = np.bincount(g, minlength=len(seq))
         first[:] = np.cumsum(n) - n
         j = np.arange(len(g)) - first[g]
-        u = np.stack([g, k0, k1, j | parts[g] << 16], axis=1)
+        u = np.concatenate([np.stack([k0, k1, j | parts[g] << 16, 0 * j], axis=1), groups[g]], axis=1)
         return u[np.argsort(k0 - k1, kind="stable")].astype(np.int32)
 
     split_groups = np.flatnonzero(parts > 1)
-    m = np.repeat(split_groups, ntok[split_groups])
-    t = np.arange(len(m)) - np.repeat(np.cumsum(ntok[split_groups]) - ntok[split_groups], ntok[split_groups])
-    merge = np.stack([groups[m, 1] + t, part0[m] + t, parts[m], ntok[m]], axis=1).astype(np.int32)
-    return WorkLists(groups.astype(np.int32), listed(*cuts[0]), listed(*cuts[1]), merge,
-                     int(rows.sum()), int(ntok[~on_items].max()) if (~on_items).any() else 0, masks)
+    fours = -(-ntok[split_groups] * group // 4)  # a merge record covers four rows
+    m = np.repeat(split_groups, fours)
+    t = np.arange(len(m)) - np.repeat(np.cumsum(fours) - fours, fours)
+    merge = np.concatenate([np.stack([parts[m], 4 * t, on_items[m], 0 * t], axis=1), groups[m]], axis=1).astype(np.int32)
+    return WorkLists(listed(*cuts[0]), listed(*cuts[1]), merge, masks, int(rows.sum()),
+                     int(ntok[~on_items].max()) if (~on_items).any() else 0)
 
 
 def unit_share_for(keys: np.ndarray, workers: int, kv_heads: int) -> int:
@@ -308,17 +310,17 @@ class MaskedAttentionOps:
             return view
         view.buf = host.to(self.device, non_blocking=True)
         D, room = self.head_dim, view.room
-        view.ws = torch.empty(room[5] * q_heads * (-(-D // 4) * 4 + 4), dtype=torch.float32, device=self.device)
+        view.ws = torch.empty(room[4] * q_heads * (-(-D // 4) * 4 + 4), dtype=torch.float32, device=self.device)
         at, _ = lists.offsets(room)
         base = view.buf.data_ptr()
         ptr = lambda i: base + 4 * at[i] if room[i] else None  # noqa: E731
         view.args = _lib.NfMaskedArgs(
-            block_tables=self._bt_ptr, groups=ptr(0), units=ptr(1), items=ptr(2), merge=ptr(3), counts=base,
-            masks=ptr(4), mask_words=room[4], ws=view.ws.data_ptr() if room[5] else None, ws_rows=room[5],
-            queue=base + 16, status=self._status_ptr, dtype=self._dt_code, num_q_heads=q_heads,
-            num_kv_heads=self.n_heads, head_dim=D, block_size=self.block_size, num_blocks=self.num_blocks,
-            num_slots=self.batch_size, max_blocks_per_seq=self.max_blocks_per_seq, max_groups=room[0],
-            max_units=room[1], unit_tokens=room[6], max_items=room[2], max_merge=room[3], window=window, sinks=sinks)
+            block_tables=self._bt_ptr, units=ptr(0), items=ptr(1), merge=ptr(2), counts=base, masks=ptr(3),
+            mask_words=room[3], ws=view.ws.data_ptr() if room[4] else None, ws_rows=room[4], queue=base + 16,
+            status=self._status_ptr, dtype=self._dt_code, num_q_heads=q_heads, num_kv_heads=self.n_heads, head_dim=D,
+            block_size=self.block_size, num_blocks=self.num_blocks, num_slots=self.batch_size,
+            max_blocks_per_seq=self.max_blocks_per_seq, max_units=room[0], unit_tokens=room[5], max_items=room[1],
+            max_merge=room[2], window=window, sinks=sinks)
         view.args_ptr = ctypes.addressof(view.args)
         lib = _lib.load()
         view.fn = lib.nf_tree_attention if kind == "tree" else lib.nf_window_attention

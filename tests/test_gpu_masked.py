@@ -299,7 +299,7 @@ def test_bad_records_are_flagged_not_followed():
     view = st.cache.plan_window(st.plan, 30, 0, q_heads=4)
     at, _ = __import__("nifre_b200.masked", fromlist=["WorkLists"]).WorkLists.offsets(view.room)
     good = view.buf.clone()
-    for index, value, bit in ((at[0], 99, "bad slot=1"), (at[0] + 1, 77, "bad slot=1"), (at[1], 1 << 20, "unit overflow=1")):
+    for index, value, bit in ((at[0] + 4, 99, "bad slot=1"), (at[0] + 5, 77, "bad slot=1"), (at[0] + 6, -1, "bad slot=1")):
         view.buf.copy_(good)
         view.buf[index] = value
         out = torch.full((2, 256), 7, dtype=F32, device=DEV)

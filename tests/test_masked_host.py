@@ -13,18 +13,16 @@ from nifre_b200.masked import WorkLists, build_lists, even_shares, mask_words, t
 from oracle.masked import window_seen
 
 
-def _keys_of(lists, g, window, sinks):
-    """The keys that the units of group g read, in order."""
-    _, _, ntok, pos0, ctx, n_draft, _, _ = lists.groups[g].tolist()
-    kept, gap, count = virtual_keys(np.asarray([pos0]), np.asarray([ntok]), window, sinks)
-    return int(kept[0]), int(gap[0]), int(count[0])
+def _keys_of(pos0, ntok, window, sinks):
+    """kept, gap and count of the virtual keys of a group."""
+    return [int(x[0]) for x in virtual_keys(np.asarray([pos0]), np.asarray([ntok]), window, sinks)]
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (7, 1), (16, 16), (100, 4), (1000, 40), (1 << 30, 0), (33, 1 << 30)])
 @pytest.mark.parametrize("rows", [(16, 0), (8, 256), (32, 128)])
 def test_units_cover_each_tokens_keys_once(window, sinks, rows):
     """Every key a token sees is read exactly once by its group's units, every token is in one group, parts are
-    numbered in order, and the merge rows name exactly the tokens with several parts."""
+    numbered in order, and the merge records cover exactly the rows of groups with several parts."""
     rng = np.random.default_rng(window + sinks)
     S = 9
     n = rng.integers(1, 90, size=S)
@@ -37,40 +35,37 @@ def test_units_cover_each_tokens_keys_once(window, sinks, rows):
     group = 4
     lists = build_lists(slots, n, starts, ctx, group, unit_rows, item_rows, workers=8, kv_heads=2, window=window,
                         sinks=sinks, unit_share=64, item_share=256)
-    cover = {}
-    for g, rec in enumerate(lists.groups.tolist()):
-        slot, q0, ntok, pos0, c, nd, _, part0 = rec
+    units, cover = {}, {}
+    for kind, recs in (("unit", lists.units), ("item", lists.items)):
+        for k0, k1, pp, zero, *g in recs.tolist():
+            assert k0 % (128 if kind == "item" else 16) == 0 and k0 < k1 and zero == 0
+            units.setdefault(tuple(g), []).append((pp & 0xffff, k0, k1, pp >> 16, kind))
+    merged = {tuple(r) for r in lists.merge.tolist()}
+    n_merge = 0
+    taken = np.zeros(lists.part_rows, dtype=int)
+    for g, us in units.items():
+        slot, q0, ntok, pos0, c, nd, _, part0 = g
         s = slots.tolist().index(slot)
         assert c == ctx[s] and nd == n[s] and q0 - starts[s] == pos0 - ctx[s]
         for t in range(ntok):
             assert (s, pos0 + t) not in cover
             cover[(s, pos0 + t)] = g
-    assert len(cover) == n.sum()
-    units = {}
-    for kind, recs in (("unit", lists.units), ("item", lists.items)):
-        for g, k0, k1, pp in recs.tolist():
-            assert k0 % (128 if kind == "item" else 16) == 0 and k0 < k1
-            units.setdefault(g, []).append((pp & 0xffff, k0, k1, pp >> 16, kind))
-    merged = {tuple(r) for r in lists.merge.tolist()}
-    n_merge = 0
-    taken = np.zeros(lists.part_rows, dtype=int)
-    for g, rec in enumerate(lists.groups.tolist()):
-        _, q0, ntok, pos0, c, nd, _, part0 = rec
-        us = sorted(units[g])
-        kept, gap, count = _keys_of(lists, g, window, sinks)
+        us = sorted(us)
+        kept, gap, count = _keys_of(pos0, ntok, window, sinks)
         assert [u[0] for u in us] == list(range(len(us))) and {u[3] for u in us} == {len(us)}
         assert us[0][1] == 0 and us[-1][2] == count and all(a[2] == b[1] for a, b in zip(us, us[1:]))
         limit = item_rows if us[0][4] == "item" else max(unit_rows, group)
-        assert ntok * group <= limit
+        assert ntok * group <= limit and len({u[4] for u in us}) == 1
         read = [v if v < kept else v + gap for v in range(count)]
         assert len(set(read)) == len(read)
         seen = window_seen(int(pos0), int(ntok), window, sinks)
         assert set(seen.any(0).nonzero().squeeze(1).tolist()) <= set(read)
         if len(us) > 1:
             taken[part0:part0 + len(us) * ntok] += 1
-            for t in range(ntok):
-                assert (q0 + t, part0 + t, len(us), ntok) in merged
+            for row in range(0, ntok * group, 4):
+                assert (len(us), row, int(us[0][4] == "item"), 0, *g) in merged
                 n_merge += 1
+    assert len(cover) == n.sum()
     assert n_merge == len(merged) == len(lists.merge) and (taken == 1).all()
 
 
@@ -78,7 +73,7 @@ def test_tree_lists_carry_every_mask_row():
     parents = [[-1, 0, 0, 1], [-1] * 40, [-1]]
     words = [mask_words(tree_visibility(p)) for p in parents]
     lists = build_lists([2, 0, 1], [4, 40, 1], [0, 4, 44], [100, 0, 5], 8, 16, 0, 8, 1, words=words, unit_share=64)
-    for slot, q0, ntok, pos0, ctx, nd, mask0, _ in lists.groups.tolist():
+    for _, _, _, _, slot, q0, ntok, pos0, ctx, nd, mask0, _ in lists.units.tolist():
         s = [2, 0, 1].index(slot)
         seen = tree_visibility(parents[s])
         w = (nd + 31) // 32
@@ -122,12 +117,12 @@ def test_even_shares_cover_every_group_in_order():
 def test_packed_lists_and_room():
     lists = build_lists([0, 1], [1, 40], [0, 1], [500, 20], 4, 16, 0, 4, 1, window=300, sinks=3, unit_share=64)
     room = lists.room(lists.sizes())
-    assert all(r >= n and r % 64 == 0 for r, n in zip(room[:6], lists.sizes()[:6]))
+    assert all(r >= n and r % 64 == 0 for r, n in zip(room[:5], lists.sizes()[:5]))
     host = lists.pack(room)
     at, total = WorkLists.offsets(room)
     assert len(host) == total and all(a % 4 == 0 for a in at)
     assert host[:8].tolist() == [len(lists.units), 0, len(lists.merge), 0, 0, 0, 0, 0]
-    assert host[at[1]:at[1] + lists.units.size].tolist() == lists.units.reshape(-1).tolist()
+    assert host[at[0]:at[0] + lists.units.size].tolist() == lists.units.reshape(-1).tolist()
 
 
 def test_too_many_parts_are_refused():
@@ -155,10 +150,10 @@ def test_masked_arguments_struct_matches_the_header(tmp_path):
 
 
 def _args(**kw):
-    base = dict(out=256, q=256, k_pool=256, v_pool=256, block_tables=256, groups=256, units=256, items=256, merge=256,
+    base = dict(out=256, q=256, k_pool=256, v_pool=256, block_tables=256, units=256, items=256, merge=256,
                 counts=256, masks=256, mask_words=4, ws=256, ws_rows=4, queue=256, status=256, dtype=2, num_q_heads=8,
                 num_kv_heads=2, head_dim=64, block_size=16, num_blocks=4, num_slots=1, max_blocks_per_seq=4, num_rows=1,
-                max_groups=1, max_units=1, unit_tokens=1, max_items=0, max_merge=0, window=4, sinks=0, scale=1.0)
+                max_units=1, unit_tokens=1, max_items=0, max_merge=0, window=4, sinks=0, scale=1.0)
     base.update(kw)
     return _lib.NfMaskedArgs(**base)
 
@@ -169,7 +164,7 @@ def _args(**kw):
     (dict(block_size=0), "sizes"), (dict(num_rows=0), "sizes"), (dict(max_units=-1), "work list"),
     (dict(max_units=0), "work list"), (dict(unit_tokens=0), "unit_tokens"), (dict(unit_tokens=1 << 20), "unit_tokens"),
     (dict(q=None), "null"), (dict(units=None), "null"), (dict(ws=None), "null"), (dict(status=None), "null"),
-    (dict(q_row_stride=-1), "stride"), (dict(groups=260), "aligned"), (dict(q=257), "aligned"),
+    (dict(q_row_stride=-1), "stride"), (dict(units=260), "aligned"), (dict(q=257), "aligned"),
     (dict(window=0), "window"), (dict(sinks=-1), "sinks")])
 def test_window_entry_point_refuses(change, match):
     """Host-side checks: nothing is launched."""
