@@ -439,7 +439,10 @@ int nf_cascade_limits(int32_t dtype, int32_t num_q_heads, int32_t num_kv_heads, 
  *     units (kind 0) or items (kind 1): their partial results are merged into
  *     out.  Part j of a group uses the partial rows part_row0 + j * ntok to
  *     part_row0 + (j + 1) * ntok - 1.
- *   counts[4]: units, items, merge records in use, 0.
+ *   unit_shares, item_shares: the runs of units (items) that a worker takes for
+ *     one KV head: share i is records shares[i] to shares[i + 1] - 1, at most
+ *     max_units (max_items) shares.
+ *   counts[4]: unit shares, item shares, merge records and units in use.
  * Workspace: ws (16-byte aligned), ws_rows partial rows of num_q_heads *
  * (head_dim rounded up to a multiple of 4, plus 4) floats; queue: int32[4], zero when
  * allocated, left zero by every call (calls that share it or ws must not
@@ -457,6 +460,8 @@ typedef struct NfMaskedArgs {
   const int32_t* units;
   const int32_t* items;
   const int32_t* merge;
+  const int32_t* unit_shares;
+  const int32_t* item_shares;
   const int32_t* counts;
   const uint32_t* masks;
   int64_t mask_words;

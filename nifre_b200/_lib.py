@@ -81,7 +81,8 @@ class NfMaskedArgs(ctypes.Structure):
     _fields_ = [("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64), ("q", ctypes.c_void_p),
                 ("q_row_stride", ctypes.c_int64), ("k_pool", ctypes.c_void_p), ("v_pool", ctypes.c_void_p),
                 ("block_tables", ctypes.c_void_p), ("units", ctypes.c_void_p),
-                ("items", ctypes.c_void_p), ("merge", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+                ("items", ctypes.c_void_p), ("merge", ctypes.c_void_p), ("unit_shares", ctypes.c_void_p),
+                ("item_shares", ctypes.c_void_p), ("counts", ctypes.c_void_p),
                 ("masks", ctypes.c_void_p), ("mask_words", ctypes.c_int64), ("ws", ctypes.c_void_p),
                 ("ws_rows", ctypes.c_int64), ("queue", ctypes.c_void_p), ("status", ctypes.c_void_p),
                 ("dtype", ctypes.c_int32), ("num_q_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),

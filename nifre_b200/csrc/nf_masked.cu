@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
   constexpr int E = EV * VW;
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, li = lane % LPK, lg = lane / LPK;
-  const int n_units = min(__ldg(p.counts), p.max_units);
+  const int n_units = min(__ldg(p.counts + 3), p.max_units);
   pdl_wait();
   const T* q = reinterpret_cast<const T*>(p.q);
   const T* kp = reinterpret_cast<const T*>(p.kp);
@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
 // 32-byte sectors, and goes over the parts PB at a time with a running maximum
 // (one round trip to L2 per PB parts).  A merge record covers four rows.
 template <typename T>
-__global__ void __launch_bounds__(256) masked_merge_kernel(const MaskedParams p) {
-  constexpr int PB = 8;
+__global__ void __launch_bounds__(256, 4) masked_merge_kernel(const MaskedParams p) {
+  constexpr int PB = 4;
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int n = min(__ldg(p.counts + 2), p.max_merge);
@@ -346,7 +346,8 @@ static int masked_check(const NfMaskedArgs* a, bool tree, const char* what, Mask
   if (a->max_units && (a->unit_tokens <= 0 || (int64_t)a->unit_tokens * a->num_q_heads > (1 << 20)))
     return fail(NF_EINVAL, "%s: unit_tokens (%d) must be positive, and at most 2^20 / num_q_heads", what, a->unit_tokens);
   if (!a->out || !a->q || !a->k_pool || !a->v_pool || !a->block_tables || !a->counts || !a->queue ||
-      !a->status || (a->max_units && !a->units) || (a->max_items && !a->items) || (a->max_merge && !a->merge) ||
+      !a->status || (a->max_units && (!a->units || !a->unit_shares)) ||
+      (a->max_items && (!a->items || !a->item_shares)) || (a->max_merge && !a->merge) ||
       (a->ws_rows && !a->ws))
     return fail(NF_EINVAL, "%s: null pointer argument", what);
   if (a->q_row_stride < 0 || a->out_row_stride < 0) return fail(NF_EINVAL, "%s: negative row stride", what);
@@ -355,7 +356,8 @@ static int masked_check(const NfMaskedArgs* a, bool tree, const char* what, Mask
     return fail(NF_EINVAL, "%s: window (%d) must be positive and sinks (%d) not negative", what, a->window, a->sinks);
   auto al = [](const void* ptr, size_t n) { return (reinterpret_cast<uintptr_t>(ptr) % n) == 0; };
   if (!al(a->units, 16) || !al(a->items, 16) || !al(a->merge, 16) || !al(a->ws, 16) ||
-      !al(a->masks, 4) || !al(a->counts, 4))
+      !al(a->masks, 4) || !al(a->counts, 4) ||
+      !al(a->unit_shares, 4) || !al(a->item_shares, 4))
     return fail(NF_EINVAL, "%s: work lists and workspace must be 16-byte aligned", what);
   if (!al(a->q, es) || !al(a->out, es) || !al(a->k_pool, es) || !al(a->v_pool, es))
     return fail(NF_EINVAL, "%s: tensors must be aligned to their elements", what);
@@ -383,6 +385,8 @@ static int masked_check(const NfMaskedArgs* a, bool tree, const char* what, Mask
   p.max_items = a->max_items;
   p.merge = a->merge;
   p.max_merge = a->max_merge;
+  p.unit_shares = a->unit_shares;
+  p.item_shares = a->item_shares;
   p.counts = a->counts;
   p.masks = a->masks;
   p.mask_words = tree ? a->mask_words : 0;

@@ -40,7 +40,9 @@ struct MaskedParams {
   int max_items;
   const int* merge;  // [max_merge][12]: n_parts, first row, kind (1: items), 0, group fields
   int max_merge;
-  const int* counts;  // units, items, merge records in use
+  const int* unit_shares;  // share i: records [i] to [i + 1] - 1
+  const int* item_shares;
+  const int* counts;  // unit shares, item shares, merge records, units in use
   const uint32_t* masks;
   long long mask_words;
   int tree, window, sinks;
@@ -62,6 +64,11 @@ __device__ __forceinline__ int4 load_record(const int* list, int i, MaskedGroup&
   const int4 h = __ldg(r), a = __ldg(r + 1), b = __ldg(r + 2);
   g = MaskedGroup{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
   return h;
+}
+
+// Units of share i, within the list.
+__device__ __forceinline__ int2 load_share(const int* shares, int i, int max_records) {
+  return make_int2(max(0, __ldg(shares + i)), min(__ldg(shares + i + 1), max_records));
 }
 
 // The group's own bounds against the buffers that the call gave.

@@ -2,7 +2,7 @@
 // on fifth-generation tensor cores (tcgen05, tensor memory), for 16-bit pools
 // with head_dim 64 or 128 and a block size that is a multiple of 16.
 //
-// An item is (unit, KV head): up to 256 query rows (row = token * G + query
+// An item is (unit, KV head), a task (share of units, KV head).  Up to 256 query rows (row = token * G + query
 // head), as two 128-row halves, against the unit's part of the group's
 // virtual keys in tiles of 128.  Each 16-key block of a tile has its own
 // place in the pools, so the gap between a window's sinks and its last keys
@@ -89,7 +89,7 @@ struct TcItem {
   bool bad, dup;
   __device__ TcItem(const MaskedParams& p, int item, int4 un, const MaskedGroup& gr, int TT)
       : g(gr), vk(p, gr) {
-    kvh = item % p.Hkv;
+    kvh = item;
     k0 = un.x;
     k1 = min(un.y, vk.end);
     part = un.z;
@@ -111,8 +111,6 @@ struct TcItem {
   }
   // whether some row of the group may not see the whole of tile j
   __device__ __forceinline__ bool masked(int j) const { return j < whole0 || j >= whole1; }
-  // the half that looks masked tile j's values over (it is active there)
-  __device__ __forceinline__ int keeper(int j) const { return dup ? j & 1 : n_half - 1; }
 };
 
 // Bits [lo, hi) of word w of a 128-bit row.
@@ -160,7 +158,7 @@ __device__ __noinline__ bool seen_by_any(const MaskedParams& p, const MaskedGrou
   return false;
 }
 
-// The ring that hands items to the CTA's warps; a slot holds the item number
+// The ring that hands items to the CTA's warps; a slot holds the KV head
 // (-1: no more) and the unit's record.
 struct TcRing {
   const TcBars& bar;
@@ -168,33 +166,49 @@ struct TcRing {
   Ring r;
   __device__ TcRing(const TcBars& b, unsigned char* base) : bar(b), slots(base + kTcSlots) {}
   __device__ int4* slot(int st) const { return reinterpret_cast<int4*>(slots + 64 * st); }
-  __device__ bool next(int& item, int4& un, MaskedGroup& g, int* status) {
-    if (!mbar_wait(bar.item_full(r.st), r.ph, status)) return false;
-    const int4* sl = slot(r.st);
+  // the item in slot st (until release)
+  __device__ TcItem item(const MaskedParams& p, int st, int TT) const {
+    const int4* sl = slot(st);
     const int4 a = sl[0], b = sl[1], c = sl[2], d = sl[3];
-    item = a.x;
-    un = b;
-    g = MaskedGroup{c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w};
+    return TcItem(p, a.x, b, MaskedGroup{c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w}, TT);
+  }
+  __device__ int kv_head(int st) const { return slot(st)->x; }
+  // waits for the next item: its slot (-1 at the end, or when the wait ran out)
+  __device__ int next(int* status) {
+    if (!mbar_wait(bar.item_full(r.st), r.ph, status)) return -1;
+    return kv_head(r.st) < 0 ? -1 : r.st;
+  }
+  __device__ void release() {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar.item_empty(r.st));
     r.next(kTcItemRing);
-    return item >= 0;
   }
 };
 
-__device__ __forceinline__ bool tc_claim(const MaskedParams& p, TcRing& ring, int n_items, int& claims, int& item,
+// The producer's side: the next unit of the (share, KV head) task at work, or
+// the next task's first.
+struct TcClaim {
+  int task = -1, u = 0;
+  int2 sh = make_int2(0, 0);
+};
+__device__ __forceinline__ bool tc_claim(const MaskedParams& p, TcRing& ring, int tasks, TcClaim& cl, int& item,
                                          int4& un, MaskedGroup& g) {
   const int lane = threadIdx.x & 31;
-  int pos = blockIdx.x;  // the first item is the CTA's own, the queue hands out the rest
-  if (claims > 0) {
-    if (lane == 0) pos = (int)gridDim.x + atomicAdd(p.queue + 2, 1);
-    pos = __shfl_sync(0xffffffffu, pos, 0);
+  while (++cl.u >= cl.sh.y && cl.task < tasks) {
+    int pos = blockIdx.x;  // the first task is the CTA's own, the queue hands out the rest
+    if (cl.task >= 0) {
+      if (lane == 0) pos = (int)gridDim.x + atomicAdd(p.queue + 2, 1);
+      pos = __shfl_sync(0xffffffffu, pos, 0);
+    }
+    cl.task = pos;
+    if (pos >= tasks) break;
+    cl.sh = load_share(p.item_shares, pos / p.Hkv, p.max_items);
+    cl.u = cl.sh.x - 1;
   }
-  ++claims;
-  item = pos < n_items ? pos : -1;
+  item = cl.task < tasks ? cl.task % p.Hkv : -1;  // (the KV head)
   un = make_int4(0, 0, 0, 0);
   g = MaskedGroup{};
-  if (item >= 0) un = load_record(p.items, item / p.Hkv, g);
+  if (item >= 0) un = load_record(p.items, cl.u, g);
   if (!mbar_wait(ring.bar.item_empty(ring.r.st), ring.r.ph ^ 1, p.status)) return false;
   if (lane == 0) {
     int4* sl = ring.slot(ring.r.st);
@@ -271,17 +285,18 @@ __device__ void tc_load_queries(const MaskedParams& p, const TcItem& w, int TT, 
 template <typename T, int D_>
 __device__ void tc_producer(const MaskedParams& p, int TT, bool q_tma, const CUtensorMap* tq, const CUtensorMap* tk,
                             const CUtensorMap* tv, const TcBars& bar, uint32_t q_s, uint32_t k_s, uint32_t v_s,
-                            int n_items, TcRing& ring) {
+                            int tasks, TcRing& ring) {
   using C = TcCfg<D_>;
   constexpr int NDH = D_ / 64;
   const int lane = threadIdx.x & 31;
   const uint64_t pol = l2_evict_last(), pol_q = l2_evict_first();
   Ring qr, kr, vr;
-  int it, claims = 0;
+  int it;
+  TcClaim claim;
   int4 un;
   MaskedGroup g;
   pdl_wait();  // queries, keys and values may come from the launch before this one
-  while (tc_claim(p, ring, n_items, claims, it, un, g)) {
+  while (tc_claim(p, ring, tasks, claim, it, un, g)) {
     const TcItem w(p, it, un, g, TT);
     if (w.bad) {
       if (lane == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
@@ -366,76 +381,87 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
     }
     __syncwarp();
   };
-  int it;
-  int4 un;
-  MaskedGroup g;
-  while (ring.next(it, un, g, p.status)) {
-    const TcItem w(p, it, un, g, TT);
+  for (int slot; (slot = ring.next(p.status)) >= 0;) {
+    const TcItem w = ring.item(p, slot, TT);
+    ring.release();
     if (w.bad) continue;
-    int vprev = -1;  // V stage of tile j-1
-    bool waited = false;  // tile j-1's weights were waited for already
-    auto first_of = [&](int j) { return w.dup ? j < 2 : j == 0; };  // a half's first tile overwrites O_h
-    // both halves' weights of a masked tile must be in before either P V: the keeper half may zero value rows
-    auto wait_all = [&](int j) -> bool {
+    // P V runs `lag` tiles behind S: one, or two where the halves take tiles in turn (a half's next S is then issued
+    // while the other half's weights are still to come)
+    const int lag = w.dup ? 2 : 1;
+    int v1 = -1, v2 = -1;  // V stages of the last tile loaded and the one before
+    auto pv = [&](int j, int vst) -> bool {  // P V of tile j from V stage vst
+      bool waited = false;
+      if (w.masked(j)) {
+        // both halves' weights of a masked tile must be in before either P V: the keeper half may zero value rows
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (w.active(h, j) && !wait_p(h)) return false;
+        for (int h = 0; h < 2; ++h)
+          if (w.active(h, j) && !wait_p(h)) return false;
+        waited = true;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (!w.active(h, j)) continue;
+        if (!waited && !wait_p(h)) return false;
+        issue_pv(h, vst, j < lag);  // (a half's first tile overwrites O_h)
+      }
       return true;
     };
     if (!mbar_wait(bar.q_full(qr.st), qr.ph, p.status)) return;
     for (int j = 0; j < w.nkt; ++j) {
       if (!mbar_wait(bar.k_full(kr.st), kr.ph, p.status)) return;
-      waited = false;
-      if (C::P_ALIAS && j > 0 && !w.dup && w.masked(j - 1)) {
-        if (!wait_all(j - 1)) return;
-        waited = true;
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (C::P_ALIAS && !w.dup && w.active(h, j - 1)) {
-          // P_h of tile j-1 sits in S_h: consume it before S_h is rewritten
-          if (!waited && !wait_p(h)) return;
-          issue_pv(h, vprev, first_of(j - 1));
-        }
-        if (!w.active(h, j)) continue;
-        if (!C::P_ALIAS) {
-          if (!mbar_wait(bar.s_free(h), (n_s[h] & 1) ^ 1, p.status)) return;
-          ++n_s[h];
-        }
-        tc_fence_after();
-        issue_s(h, w.dup ? 0 : h, kr.st);
-      }
-      if (leader) umma_commit(bar.k_empty(kr.st));
-      kr.next(C::KST);
-      if (j > 0) {
-        if (!C::P_ALIAS || w.dup) {
-          // (dup: half h's weights of tile j-2 in S_h were consumed before S_h of tile j was issued)
-          if (w.masked(j - 1)) {
-            if (!wait_all(j - 1)) return;
+      const int jp = j - lag, vst = lag == 1 ? v1 : v2;
+      if (C::P_ALIAS) {
+        // P_h sits in S_h: it is consumed before S_h is rewritten
+        if (w.dup) {
+          if (jp >= 0 && !pv(jp, vst)) return;
+          tc_fence_after();
+          issue_s(j & 1, 0, kr.st);
+        } else {
+          bool waited = false;
+          if (jp >= 0 && w.masked(jp)) {
+            for (int h = 0; h < w.n_half; ++h)
+              if (!wait_p(h)) return;
             waited = true;
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (!w.active(h, j - 1)) continue;
-            if (!waited && !wait_p(h)) return;
-            issue_pv(h, vprev, first_of(j - 1));
+            if (h >= w.n_half) continue;
+            if (jp >= 0) {
+              if (!waited && !wait_p(h)) return;
+              issue_pv(h, vst, jp == 0);
+            }
+            tc_fence_after();
+            issue_s(h, h, kr.st);
           }
         }
-        if (leader) umma_commit(bar.v_empty(vprev));
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!w.active(h, j)) continue;
+          if (!mbar_wait(bar.s_free(h), (n_s[h] & 1) ^ 1, p.status)) return;
+          ++n_s[h];
+          tc_fence_after();
+          issue_s(h, w.dup ? 0 : h, kr.st);
+        }
       }
+      if (leader) umma_commit(bar.k_empty(kr.st));
+      kr.next(C::KST);
+      if (!C::P_ALIAS && jp >= 0 && !pv(jp, vst)) return;
+      if (jp >= 0 && leader) umma_commit(bar.v_empty(vst));
       if (!mbar_wait(bar.v_full(vr.st), vr.ph, p.status)) return;
-      vprev = vr.st;
+      v2 = v1;
+      v1 = vr.st;
       vr.next(C::VST);
     }
     // every S of the item is issued: the Q stage is free once they complete
     if (leader) umma_commit(bar.q_empty(qr.st));
     qr.next(C::QST);
-    const int jl = w.nkt - 1;
-    if (!wait_all(jl)) return;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (w.active(h, jl)) issue_pv(h, vprev, first_of(jl));
-    if (leader) umma_commit(bar.v_empty(vprev));
+    if (lag == 2) {  // (such an item has two tiles or more)
+      if (!pv(w.nkt - 2, v2)) return;
+      if (leader) umma_commit(bar.v_empty(v2));
+    }
+    if (!pv(w.nkt - 1, v1)) return;
+    if (leader) umma_commit(bar.v_empty(v1));
   }
 }
 
@@ -497,77 +523,104 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
   const float scale = p.scale_log2 > 0.f ? p.scale_log2 : 1.f;
   bool join_pending = false;  // half 1: its accumulator is still to be read by half 0
   Ring vr;
-  int it, seq = 0;
-  int4 un;
-  MaskedGroup g;
-  while (ring.next(it, un, g, p.status)) {
-    const TcItem w(p, it, un, g, TT);
-    if (w.bad) continue;
-    ++seq;
-    const Ring v0r = vr;  // V stage of the item's first tile
-    vr = vr.ahead(w.nkt, C::VST);
-    if (w.tiles(h) == 0) continue;
-    const int tok = (w.dup ? 0 : h * TT) + row / p.G, hd = row % p.G;
-    const bool valid = row < TT * p.G && tok < w.g.ntok;
-    float m = -INFINITY, l = 0.f;
+  int seq = 0;
+  // The item itself stays in its slot of shared memory while the tiles run (its fields would cost the tile loop the
+  // registers of the scores); what masked tiles and the epilogue need is read there again.
+  for (int slot; (slot = ring.next(p.status)) >= 0; ring.release()) {
+    Ring v0r;  // V stage of the item's first tile
+    int nkt, whole0, whole1;
+    bool dup, keep;  // keep: this half looks the values of masked tiles over (where the halves share them)
+    bool valid;
+    {
+      const TcItem w = ring.item(p, slot, TT);
+      if (w.bad) continue;
+      ++seq;
+      v0r = vr;
+      vr = vr.ahead(w.nkt, C::VST);
+      if (w.tiles(h) == 0) continue;
+      nkt = w.nkt;
+      whole0 = w.whole0;
+      whole1 = w.whole1;
+      dup = w.dup;
+      keep = w.dup || h == w.n_half - 1;
+      valid = row < TT * p.G && (dup ? 0 : h * TT) + row / p.G < w.g.ntok;
+    }
+    float m = 0.f, l = 0.f;  // the reference of the exponents, and the sum of the weights
+    bool none = true;        // the row has seen no key yet
     int n = 0;  // tiles done
-    for (int j = w.dup ? h : 0; j < w.nkt; j += w.dup ? 2 : 1, ++n) {
+    for (int j = dup ? h : 0; j < nkt; j += dup ? 2 : 1, ++n) {
       if (!mbar_wait(bar.s_full(h), n_s & 1, p.status)) return;
       ++n_s;
       tc_fence_after();
+      const bool masked = j < whole0 || j >= whole1;
       uint32_t x[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
-      tmem_wait_ld();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_reg_fence(*reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
-      if (!C::P_ALIAS) {  // S_h is in registers: the next S_h may be computed
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar.s_free(h));
-      }
-      if (p.scale_log2 <= 0.f) {
-#pragma unroll
-        for (int i = 0; i < 128; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * p.scale_log2);
-      }
-      const bool masked = w.masked(j);
-      if (masked) {
-        uint32_t bits[4] = {0u, 0u, 0u, 0u};
-        if (valid) row_bits(p, w, tok, j, bits);
-#pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (!(bits[i >> 5] >> (i & 31) & 1u)) x[i] = 0xff800000u;
-      }
-      float acc[8];
-#pragma unroll
-      for (int a = 0; a < 8; ++a) acc[a] = fmaxf(__uint_as_float(x[a]), __uint_as_float(x[a + 8]));
-#pragma unroll
-      for (int i = 16; i < 128; i += 16)
-#pragma unroll
-        for (int a = 0; a < 8; ++a) acc[a] = fmax3(acc[a], __uint_as_float(x[i + a]), __uint_as_float(x[i + 8 + a]));
-      float mt = fmaxf(fmaxf(fmaxf(acc[0], acc[1]), fmaxf(acc[2], acc[3])),
-                       fmaxf(fmaxf(acc[4], acc[5]), fmaxf(acc[6], acc[7])));
-      mt *= scale;
-      // lazy rescaling: the reference max moves only when the tile's max exceeds it by more than 8
-      const bool grow = mt > m + 8.f;
-      const float mn = grow ? mt : m;
-      const float alpha = grow ? ex2(m - mn) : 1.f;
-      const float nbase = mn == -INFINITY ? 0.f : -mn;
-      const uint64_t sc2 = f2_pack(scale, scale), nb2 = f2_pack(nbase, nbase);
+      float alpha = 1.f;
       uint64_t sum2[4];
+      // the tile's scores into registers, unseen ones -inf
+      auto scores = [&]() {
 #pragma unroll
-      for (int a = 0; a < 4; ++a) sum2[a] = 0ull;
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+        tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 128; i += 2) {
-        const uint64_t y2 = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, nb2);
-        float y0, y1;
-        f2_unpack(y2, y0, y1);
-        const float p0 = ex2(y0), p1 = ex2(y1);
-        sum2[(i >> 1) & 3] = f2_add(sum2[(i >> 1) & 3], f2_pack(p0, p1));
-        x[i >> 1] = pack2<T>(p0, p1);
+        for (int c = 0; c < 4; ++c) tmem_reg_fence(*reinterpret_cast<uint32_t(*)[32]>(x + 32 * c));
+        if (!C::P_ALIAS) {  // S_h is in registers: the next S_h may be computed
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar.s_free(h));
+        }
+        if (p.scale_log2 <= 0.f) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * p.scale_log2);
+        }
+        if (masked) {
+          uint32_t bits[4] = {0u, 0u, 0u, 0u};
+          if (valid) {
+            const TcItem w = ring.item(p, slot, TT);
+            row_bits(p, w, (dup ? 0 : h * TT) + row / p.G, j, bits);
+          }
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (!(bits[i >> 5] >> (i & 31) & 1u)) x[i] = 0xff800000u;
+        }
+      };
+      // weights against the reference m in the low half of x, and their sums
+      auto weights = [&]() {
+        const uint64_t sc2 = f2_pack(scale, scale), nb2 = f2_pack(-m, -m);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) sum2[a] = 0ull;
+#pragma unroll
+        for (int i = 0; i < 128; i += 2) {
+          const uint64_t y2 = f2_fma(f2_pack(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), sc2, nb2);
+          float y0, y1;
+          f2_unpack(y2, y0, y1);
+          const float p0 = ex2(y0), p1 = ex2(y1);
+          sum2[(i >> 1) & 3] = f2_add(sum2[(i >> 1) & 3], f2_pack(p0, p1));
+          x[i >> 1] = pack2<T>(p0, p1);
+        }
+      };
+      // lazy rescaling: the reference moves only to a row's first seen scores, and when a score exceeds it by more
+      // than 8 (weights stay below 2^8)
+      {
+        scores();
+        float acc[8];
+#pragma unroll
+        for (int a = 0; a < 8; ++a) acc[a] = fmaxf(__uint_as_float(x[a]), __uint_as_float(x[a + 8]));
+#pragma unroll
+        for (int i = 16; i < 128; i += 16)
+#pragma unroll
+          for (int a = 0; a < 8; ++a) acc[a] = fmax3(acc[a], __uint_as_float(x[i + a]), __uint_as_float(x[i + 8 + a]));
+        const float mt = scale * fmaxf(fmaxf(fmaxf(acc[0], acc[1]), fmaxf(acc[2], acc[3])),
+                                       fmaxf(fmaxf(acc[4], acc[5]), fmaxf(acc[6], acc[7])));
+        if (none ? mt > -INFINITY : mt > m + 8.f) {
+          if (!none) alpha = ex2(m - mt);
+          m = mt;
+          none = false;
+        }
+        weights();
       }
       if (n > 0) {  // O_h += P_h V of the half's tile before must be done before P_h or O_h change
-        if (!mbar_wait(bar.o_done(h), n_o & 1, p.status)) return;
+        // (with P_h in S_h it was issued before this tile's S_h, which is complete)
+        if (!C::P_ALIAS && !mbar_wait(bar.o_done(h), n_o & 1, p.status)) return;
         ++n_o;
         tc_fence_after();
       } else if (join_pending) {  // half 0 has read this half's last accumulator
@@ -592,8 +645,8 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
 #pragma unroll
       for (int a = 0; a < 4; ++a) f2_unpack(sum2[a], sa[2 * a], sa[2 * a + 1]);
       l = l * alpha + (((sa[0] + sa[1]) + (sa[2] + sa[3])) + ((sa[4] + sa[5]) + (sa[6] + sa[7])));
-      m = mn;
-      if (masked && w.keeper(j) == h) {
+      if (masked && keep) {
+        const TcItem w = ring.item(p, slot, TT);
         // this thread's value row of the tile: zeroed when past the unit's keys or not finite
         const Ring vt = v0r.ahead(j, C::VST);
         if (!mbar_wait(bar.v_full(vt.st), vt.ph, p.status)) return;
@@ -631,6 +684,9 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
     if (!mbar_wait(bar.o_done(h), n_o & 1, p.status)) return;
     ++n_o;
     tc_fence_after();
+    if (none) m = -INFINITY;
+    const TcItem w = ring.item(p, slot, TT);
+    const int tok = (w.dup ? 0 : h * TT) + row / p.G, hd = row % p.G;
     float a0 = 1.f, a1 = 0.f;  // weights of this half's and half 1's accumulators
     if (w.dup) {
       ++n_join;
@@ -795,12 +851,12 @@ __global__ void __launch_bounds__(TcCfg<D_>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(base + kTcTmemPtr);
   const uint32_t q_s = hdr + C::Q_OFF, k_s = hdr + C::K_OFF, v_s = hdr + C::V_OFF;
-  const int n_items = min(__ldg(p.counts + 1), p.max_items) * p.Hkv;
+  const int tasks = min(__ldg(p.counts + 1), p.max_items) * p.Hkv;
   TcRing ring(bar, base);
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_CTRL));
     if (warp == 0)
-      tc_producer<T, D_>(p, TT, q_tma, &tq, &tk, &tv, bar, q_s, k_s, v_s, n_items, ring);
+      tc_producer<T, D_>(p, TT, q_tma, &tq, &tk, &tv, bar, q_s, k_s, v_s, tasks, ring);
     else if (warp == 1)
       tc_mma<D_>(p, TT, bar, tmem, q_s, k_s, v_s, std::is_same<T, __nv_bfloat16>::value, ring);
   } else {

@@ -2,8 +2,8 @@
 // drafts), for 16-bit pools with head_dim 64 or 128 and a block size that is
 // a multiple of 16.  Bound by the key and value bytes.
 //
-// A CTA owns HG KV heads.  Its producer thread takes (unit, head group) pairs
-// from a queue and issues, for each 16-key step of a unit, one tensor copy for
+// A CTA owns HG KV heads.  Its producer thread takes (share, head group) tasks
+// from a queue and, for the share's units, issues, for each 16-key step of a unit, one tensor copy for
 // K and one for V: 16 tokens of one block x HG heads x head_dim, landing
 // head-major and 128-byte swizzled.  Steps skip the gap between a window's
 // sinks and its last keys, so a group reads its visible keys (rounded to 16)
@@ -77,24 +77,35 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
   auto empty = [&](int s) { return hdr + 64 + 8 * s; };
   MtStep* recs = reinterpret_cast<MtStep*>(base + 128);
   const uint32_t stage0 = hdr + kMtHeader;
-  // the switch to the next unit needs three dependent round trips (ticket,
+  // the switch to another task needs four dependent round trips (ticket, share,
   // record, block id): each is asked for kGap steps after the one before
   constexpr int kGap = 2, kAhead = 4 * kGap;
   const uint64_t pol = L.evict_first ? l2_evict_first() : l2_evict_last();
   int k = 0, s = 0;
   uint32_t pe = 1;
   bool ok = true;
+  // a task: (share, head group); u: the share's unit at work
   int w = blockIdx.x;
-  MaskedGroup g;
-  int4 un = load_record(p.units, min(w / L.n_hg, p.max_units - 1), g);  // (before the count is known: no matter)
+  int2 sh = load_share(p.unit_shares, min(w / L.n_hg, p.max_units - 1), p.max_units);
   const int total = min(__ldg(p.counts), p.max_units) * L.n_hg;
+  int u = sh.x;
+  MaskedGroup g;
+  int4 un = load_record(p.units, min(u, p.max_units - 1), g);
   pdl_wait();
   while (w < total) {
-    const int u = w / L.n_hg, hg = w - u * L.n_hg, h0 = hg * L.HG;
-    if (!group_ok(p, g)) {
-      atomicOr(p.status, NF_STATUS_BAD_SLOT);
-      w = (int)gridDim.x + atomicAdd(p.queue, 1);
-      if (w < total) un = load_record(p.units, w / L.n_hg, g);
+    const int hg = w % L.n_hg, h0 = hg * L.HG;
+    const bool more = u + 1 < sh.y;  // the next unit is this share's
+    if (u >= sh.y || !group_ok(p, g)) {
+      if (u < sh.y) atomicOr(p.status, NF_STATUS_BAD_SLOT);
+      if (more) {
+        ++u;
+      } else {
+        w = (int)gridDim.x + atomicAdd(p.queue, 1);
+        if (w >= total) break;
+        sh = load_share(p.unit_shares, w / L.n_hg, p.max_units);
+        u = sh.x;
+      }
+      un = load_record(p.units, min(u, p.max_units - 1), g);
       continue;
     }
     const VirtualKeys vk(p, g);
@@ -102,17 +113,23 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
     const int* btrow = p.bt + (long long)g.slot * p.max_blocks;
     const int nsteps = max(1, (v1 - un.x + 15) >> 4);  // (a unit without keys still ends in an epilogue)
     const int ask = nsteps - 1 - min(kAhead, nsteps - 1);
-    int wn = total;
+    int wn = more ? w : total, nu_at = u + 1;
+    int2 nsh = sh;
     int4 nu = make_int4(0, 0, 0, 0);
     MaskedGroup ng{};
-    bool have = false;  // the next unit's record is here
+    int have = more ? 2 : 0;  // what is known of the next unit: 1 its task, 2 its place, 3 its record
     for (int i = 0, v = un.x; i < nsteps; ++i, v += 16, ++k) {
-      if (i == ask) {
+      if (i == ask && have == 0) {
         wn = (int)gridDim.x + atomicAdd(p.queue, 1);
-      } else if (i == ask + kGap && wn < total) {
-        nu = load_record(p.units, wn / L.n_hg, ng);
-        have = true;
-      } else if (i == ask + 2 * kGap && wn < total && ng.slot >= 0 && ng.slot < p.num_slots) {
+        have = 1;
+      } else if (i == ask + kGap && have == 1 && wn < total) {
+        nsh = load_share(p.unit_shares, wn / L.n_hg, p.max_units);
+        nu_at = nsh.x;
+        have = 2;
+      } else if (i == ask + 2 * kGap && have == 2) {
+        nu = load_record(p.units, min(nu_at, p.max_units - 1), ng);
+        have = 3;
+      } else if (i == ask + 3 * kGap && have == 3 && ng.slot >= 0 && ng.slot < p.num_slots) {
         const int lb = VirtualKeys(p, ng).key(nu.x) / p.bs;
         if (lb >= 0 && lb < p.max_blocks)
           asm volatile("prefetch.global.L1 [%0];" ::"l"(p.bt + (long long)ng.slot * p.max_blocks + lb));
@@ -172,8 +189,16 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
       }
     }
     if (!ok) break;
-    if (wn < total && !have) nu = load_record(p.units, wn / L.n_hg, ng);  // a short unit
+    if (wn < total && have < 3) {  // a short unit
+      if (have < 2) {
+        nsh = load_share(p.unit_shares, wn / L.n_hg, p.max_units);
+        nu_at = nsh.x;
+      }
+      nu = load_record(p.units, min(nu_at, p.max_units - 1), ng);
+    }
     w = wn;
+    sh = nsh;
+    u = nu_at;
     un = nu;
     g = ng;
   }

@@ -16,7 +16,7 @@ import torch
 from nifre_b200 import _lib
 
 MAX_PARTS = 32767  # parts of one group (a unit record's 15 bits)
-HEAD = 8  # counts (4) and the kernels' work queue (4, zero) at the start of the buffer
+HEAD = 8  # counts (4) and the kernels' work queues (4, zero) at the start of the buffer
 
 
 def tree_visibility(parents) -> np.ndarray:
@@ -53,41 +53,37 @@ def virtual_keys(pos0, ntok, window: int, sinks: int):
 
 
 def even_shares(keys, share: int, align: int, least: int):
-    """Cut groups of ``keys`` keys into units by laying them end to end and cutting every ``share`` keys (then every
-    worker's share is one or two units, whatever the groups' lengths, and no group has more parts than it needs).
+    """Cut groups of ``keys`` keys into shares of about ``share`` keys by laying them end to end (then every worker has
+    the same to do whatever the groups' lengths, and no group has more parts than that needs).
 
-    Cuts sit at multiples of ``align`` of their group and at least ``least``
-    keys from its ends.  Returns per unit (group, first key, end), in order.
+    A share is a run of units: the end of one group, whole groups, the start of
+    another.  Cuts sit at multiples of ``align`` of their group and at least
+    ``least`` keys from its ends, else at its nearer end.  Returns per unit
+    (group, first key, end), in order, and the shares' first units (and the
+    number of units).
     """
     keys = np.asarray(keys, dtype=np.int64)
     end = np.cumsum(keys)
     start = end - keys
-    cuts = np.arange(share, int(end[-1]), share) if len(keys) else np.zeros(0, dtype=np.int64)
+    cuts = np.arange(share, int(end[-1]), share)
     g = np.searchsorted(end, cuts, side="right")
     at = (cuts - start[g] + align // 2) // align * align
-    keep = (at >= least) & (keys[g] - at >= least)
-    g, at = g[keep], at[keep]
-    group = np.concatenate([np.arange(len(keys)), g])
-    first = np.concatenate([np.zeros(len(keys), dtype=np.int64), at])
-    order = np.lexsort((first, group))
-    group, first = group[order], first[order]
-    distinct = np.ones(len(group), dtype=bool)
-    distinct[1:] = (group[1:] != group[:-1]) | (first[1:] != first[:-1])
-    group, first = group[distinct], first[distinct]
-    last = np.ones(len(group), dtype=bool)
-    last[:-1] = group[1:] != group[:-1]
-    stop = np.empty_like(first)
-    stop[:-1] = first[1:]
-    stop[last] = keys[group[last]]
-    return group, first, stop
+    low, high = at < least, keys[g] - at < least
+    at = np.where(low & (~high | (2 * at <= keys[g])), 0, np.where(high, keys[g], at))
+    where = np.unique(np.concatenate([[0], start[g] + at, [int(end[-1])]]))  # the shares' bounds
+    bounds = np.unique(np.concatenate([start, where]))  # every unit's start (and the end)
+    first, stop = bounds[:-1], bounds[1:]
+    group = np.searchsorted(end, first, side="right")
+    return group, first - start[group], stop - start[group], np.searchsorted(bounds, where)
 
 
 class WorkLists:
-    """Units, tensor-core items and merge records of one step (each record with its group's fields), the mask words,
-    and their place in one int32 buffer."""
+    """Units, tensor-core items and merge records of one step (each record with its group's fields), the shares of
+    units and items that workers take, the mask words, and their place in one int32 buffer."""
 
-    def __init__(self, units, items, merge, masks, part_rows: int, unit_tokens: int):
+    def __init__(self, units, items, merge, masks, unit_shares, item_shares, part_rows: int, unit_tokens: int):
         self.units, self.items, self.merge, self.masks = units, items, merge, masks
+        self.unit_shares, self.item_shares = unit_shares, item_shares
         self.part_rows, self.unit_tokens = part_rows, unit_tokens
 
     def sizes(self):
@@ -102,23 +98,26 @@ class WorkLists:
 
     @staticmethod
     def offsets(room):
-        """Start of each list in the buffer and its length."""
+        """Start of units, items, merge records, masks and the units' and items' shares (there are at most as many
+        shares as units), and the length."""
         at = [HEAD]
-        for n in (12 * room[0], 12 * room[1], 12 * room[2], -(-room[3] // 4) * 4):
-            at.append(at[-1] + n)
-        return at[:4], at[4]
+        for n in (12 * room[0], 12 * room[1], 12 * room[2], room[3], room[0] + 1, room[1] + 1):
+            at.append(at[-1] + -(-n // 4) * 4)
+        return at[:6], at[6]
 
     def pack(self, room) -> np.ndarray:
         at, total = self.offsets(room)
         host = np.zeros(total, dtype=np.int32)
-        host[:3] = (len(self.units), len(self.items), len(self.merge))
-        for start, part in zip(at, (self.units, self.items, self.merge, self.masks)):
+        host[:4] = (max(0, len(self.unit_shares) - 1), max(0, len(self.item_shares) - 1), len(self.merge),
+                    len(self.units))
+        for start, part in zip(at, (self.units, self.items, self.merge, self.masks, self.unit_shares,
+                                    self.item_shares)):
             host[start:start + part.size] = part.reshape(-1)
         return host
 
 
 def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_rows: int, workers: int, kv_heads: int,
-                window=None, sinks: int = 0, words=None, unit_share=None, item_share=None) -> WorkLists:
+                head_dim: int = 64, window=None, sinks: int = 0, words=None, unit_share=None, item_share=None) -> WorkLists:
     """Work lists of a step whose sequences get ``q_lens`` new tokens behind ``ctx`` cached ones.
 
     ``window``/``sinks``, or ``words``: each sequence's mask rows (``mask_words``).
@@ -146,15 +145,23 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
         mask0 = start[:-1][seq] + tok0 * np.asarray([w.shape[1] for w in words], dtype=np.int64)[seq]
         masks = np.concatenate([w.reshape(-1) for w in words])
     on_items = routed[seq]
-    cuts = []  # (group, first key, end) of every unit and of every item
-    for on, share, align, share_for in ((~on_items, unit_share, 16, unit_share_for),
-                                        (on_items, item_share, 128, item_share_for)):
+    cuts = []  # (group, first key, end) of every unit and of every item, and the shares of them
+    for on, share, align, least, share_for in ((~on_items, unit_share, 16, 64, unit_share_for),
+                                               (on_items, item_share, 128, 128, item_share_for)):
         mine = np.flatnonzero(on)
-        g, k0, k1 = even_shares(keys[mine], share or share_for(keys[mine], workers, kv_heads), align, 4 * align) \
-            if len(mine) else (mine, mine, mine)
-        cuts.append((mine[g], k0, k1))
+        if not len(mine):
+            cuts.append((mine, mine, mine, mine))
+            continue
+        k = keys[mine]
+        share = share or share_for(k, ntok[mine] * group, workers, kv_heads, head_dim)
+        if share:
+            g, k0, k1, at = even_shares(k, share, align, least)
+        else:  # whole groups, the longest first
+            g = np.argsort(-k, kind="stable")
+            k0, k1, at = 0 * k, k[g], np.arange(len(k) + 1)
+        cuts.append((mine[g], k0, k1, at))
     parts = np.zeros(len(seq), dtype=np.int64)
-    for g, _, _ in cuts:
+    for g, *_ in cuts:
         parts += np.bincount(g, minlength=len(seq))
     if parts.max() > MAX_PARTS:
         raise ValueError(f"a sequence's keys are cut into {int(parts.max())} parts, at most {MAX_PARTS}")
@@ -164,36 +171,49 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
     if groups.max() >= 1 << 31:
         raise ValueError("the step's work lists exceed 32-bit indices")
 
-    def listed(g, k0, k1):
-        """Unit records, the largest first (a queue over the list then ends on short ones)."""
-        first = np.zeros(len(seq), dtype=np.int64)
-        n = np.bincount(g, minlength=len(seq))
-        first[:] = np.cumsum(n) - n
-        j = np.arange(len(g)) - first[g]
-        u = np.concatenate([np.stack([k0, k1, j | parts[g] << 16, 0 * j], axis=1), groups[g]], axis=1)
-        return u[np.argsort(k0 - k1, kind="stable")].astype(np.int32)
+    def listed(g, k0, k1, _):
+        """Unit records, a group's parts numbered in the order of their keys."""
+        j = np.arange(len(g)) - np.searchsorted(g, g) if len(g) and (np.diff(g) >= 0).all() else 0 * g
+        return np.concatenate([np.stack([k0, k1, j | parts[g] << 16, 0 * g], axis=1), groups[g]], axis=1).astype(np.int32)
 
     split_groups = np.flatnonzero(parts > 1)
     fours = -(-ntok[split_groups] * group // 4)  # a merge record covers four rows
     m = np.repeat(split_groups, fours)
     t = np.arange(len(m)) - np.repeat(np.cumsum(fours) - fours, fours)
     merge = np.concatenate([np.stack([parts[m], 4 * t, on_items[m], 0 * t], axis=1), groups[m]], axis=1).astype(np.int32)
-    return WorkLists(listed(*cuts[0]), listed(*cuts[1]), merge, masks, int(rows.sum()),
+    return WorkLists(listed(*cuts[0]), listed(*cuts[1]), merge, masks, cuts[0][3], cuts[1][3], int(rows.sum()),
                      int(ntok[~on_items].max()) if (~on_items).any() else 0)
 
 
-def unit_share_for(keys: np.ndarray, workers: int, kv_heads: int) -> int:
-    """Keys per unit: one share a worker (a partial row costs about as much as 4 keys to write and merge), up to four
-    where shares stay at 512 keys or more (then the queue evens out the workers' speeds); 64 keys at least."""
+def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
+    """Keys per share of units: one share a worker, up to four where shares stay at 512 keys or more (then the queue
+    evens out the workers' speeds); 64 keys at least."""
     total = int(keys.sum())
+    workers = max(1, workers * 8 // kv_heads)  # eight KV heads at a time an SM
     waves = min(4, max(1, total // (workers * 512)))
     return max(64, -(-total // (workers * waves * 16)) * 16)
 
 
-def item_share_for(keys: np.ndarray, workers: int, kv_heads: int) -> int:
-    """Keys per tensor-core item (one per KV head): one item per worker, at least 256 keys each."""
-    want = max(1, int(keys.sum()) * kv_heads // workers)
-    return max(256, -(-want // 128) * 128)
+def item_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
+    """Keys per share of tensor-core items, 0 for whole groups.
+
+    Whole groups need no merge, but the workers end unevenly; equal shares cost
+    partial results (written and read: 4 (head_dim + 4) bytes a row and part)
+    and the merge's launch.  Both are estimated in microseconds from a tile's
+    time (256 rows x 128 keys 1.8 at head_dim 64, 2.0 at 128; 128 rows 1.2), 2
+    an item, 4 a merge and 3 TB/s, which fit the measured cases within a fifth.
+    """
+    tiles = -(-keys // 128)
+    cost = np.where(rows <= 128, 1.2, 1.8 if head_dim == 64 else 2.0)
+    each = tiles * cost + 2.0
+    whole = max(float(each.max()), -(-len(keys) * kv_heads // workers) * float(each.mean()))
+    shares = max(1, workers // kv_heads)
+    share = max(256, -(-int(keys.sum()) // (shares * 128)) * 128)
+    cuts = int(keys.sum()) // share
+    parts = cuts + min(cuts, len(keys))  # partial results: two at a group's first cut, one more at each further
+    cut = max(float((tiles * cost).sum()) / shares, 2 * float(cost.min())) + 8.0 + \
+        parts * float(rows.mean()) * kv_heads * 4 * (head_dim + 4) * 2 / 3e6
+    return share if cut < whole else 0
 
 
 class MaskedPlan:
@@ -289,7 +309,7 @@ class MaskedAttentionOps:
             raise IndexError(f"cache slot out of range [0, {self.batch_size})")
         unit_rows, item_rows = self.masked_limits(q_heads)
         lists = build_lists(plan.slots, plan.q_lens, plan.q_starts, plan.ctx_before, q_heads // self.n_heads, unit_rows,
-                            item_rows, self.masked_workers, self.n_heads, window, sinks, words)
+                            item_rows, self.sm_count, self.n_heads, self.head_dim, window, sinks, words)
         sizes = lists.sizes()
         if into is None:
             view = MaskedPlan(kind, window, sinks, q_heads, plan.rows_needed)
@@ -316,6 +336,7 @@ class MaskedAttentionOps:
         ptr = lambda i: base + 4 * at[i] if room[i] else None  # noqa: E731
         view.args = _lib.NfMaskedArgs(
             block_tables=self._bt_ptr, units=ptr(0), items=ptr(1), merge=ptr(2), counts=base, masks=ptr(3),
+            unit_shares=base + 4 * at[4], item_shares=base + 4 * at[5],
             mask_words=room[3], ws=view.ws.data_ptr() if room[4] else None, ws_rows=room[4], queue=base + 16,
             status=self._status_ptr, dtype=self._dt_code, num_q_heads=q_heads, num_kv_heads=self.n_heads, head_dim=D,
             block_size=self.block_size, num_blocks=self.num_blocks, num_slots=self.batch_size,
@@ -329,13 +350,6 @@ class MaskedAttentionOps:
         view.ready.record(torch.cuda.current_stream(self.device))
         view.streams = {self._stream()}
         return view
-
-    @property
-    def masked_workers(self) -> int:
-        """Units at work at once that a step's keys are cut for: the tensor-map kernel keeps eight KV heads an SM on
-        the go, the per-warp kernel (other types and shapes) about 32."""
-        heads = 8 if self.dtype != torch.float32 and self.head_dim in (64, 128) and self.block_size % 16 == 0 else 32
-        return max(1, self.sm_count * heads // self.n_heads)
 
     def window_attention_step(self, layer_id: int, q: torch.Tensor, view: MaskedPlan, out: torch.Tensor,
                               scale: float | None = None) -> torch.Tensor:

@@ -65,6 +65,8 @@ def test_units_cover_each_tokens_keys_once(window, sinks, rows):
             for row in range(0, ntok * group, 4):
                 assert (len(us), row, int(us[0][4] == "item"), 0, *g) in merged
                 n_merge += 1
+    for recs, shares in ((lists.units, lists.unit_shares), (lists.items, lists.item_shares)):
+        assert not len(recs) or (shares[0] == 0 and shares[-1] == len(recs) and (np.diff(shares) > 0).all())
     assert len(cover) == n.sum()
     assert n_merge == len(merged) == len(lists.merge) and (taken == 1).all()
 
@@ -102,16 +104,18 @@ def test_even_shares_cover_every_group_in_order():
     rng = np.random.default_rng(1)
     for n, most, share, align in ((1, 5, 64, 16), (9, 3000, 448, 16), (40, 200, 64, 16), (5, 9000, 256, 128), (64, 1041, 464, 16)):
         keys = rng.integers(1, most, size=n)
-        g, k0, k1 = even_shares(keys, share, align, 4 * align)
+        least = 4 * align
+        g, k0, k1, at = even_shares(keys, share, align, least)
         assert (k0 < k1).all() and (k0 % align == 0).all()
         assert (np.diff(g) >= 0).all() and set(g.tolist()) == set(range(n))
         for i in range(n):
             mine = g == i
             assert k0[mine][0] == 0 and k1[mine][-1] == keys[i] and (k1[mine][:-1] == k0[mine][1:]).all()
             if mine.sum() > 1:
-                assert (k1[mine] - k0[mine]).min() >= min(4 * align, share - align)
-        # a share, the pieces next to a cut that was left out, and the rounding
-        assert (k1 - k0).max() <= 2 * share + 8 * align + align
+                assert (k1[mine] - k0[mine]).min() >= min(least, share - align)
+        assert at[0] == 0 and at[-1] == len(g) and (np.diff(at) > 0).all()
+        sizes = np.add.reduceat(k1 - k0, at[:-1])
+        assert sizes.max() <= share + 2 * least + align  # each bound moves by less than least
 
 
 def test_packed_lists_and_room():
@@ -121,7 +125,8 @@ def test_packed_lists_and_room():
     host = lists.pack(room)
     at, total = WorkLists.offsets(room)
     assert len(host) == total and all(a % 4 == 0 for a in at)
-    assert host[:8].tolist() == [len(lists.units), 0, len(lists.merge), 0, 0, 0, 0, 0]
+    assert host[:8].tolist() == [len(lists.unit_shares) - 1, 0, len(lists.merge), len(lists.units), 0, 0, 0, 0]
+    assert host[at[4]:at[4] + len(lists.unit_shares)].tolist() == lists.unit_shares.tolist()
     assert host[at[0]:at[0] + lists.units.size].tolist() == lists.units.reshape(-1).tolist()
 
 
@@ -151,7 +156,7 @@ def test_masked_arguments_struct_matches_the_header(tmp_path):
 
 def _args(**kw):
     base = dict(out=256, q=256, k_pool=256, v_pool=256, block_tables=256, units=256, items=256, merge=256,
-                counts=256, masks=256, mask_words=4, ws=256, ws_rows=4, queue=256, status=256, dtype=2, num_q_heads=8,
+                unit_shares=256, item_shares=256, counts=256, masks=256, mask_words=4, ws=256, ws_rows=4, queue=256, status=256, dtype=2, num_q_heads=8,
                 num_kv_heads=2, head_dim=64, block_size=16, num_blocks=4, num_slots=1, max_blocks_per_seq=4, num_rows=1,
                 max_units=1, unit_tokens=1, max_items=0, max_merge=0, window=4, sinks=0, scale=1.0)
     base.update(kw)
