@@ -6,11 +6,11 @@
 
 namespace nf {
 
-// Columns (token, query head of the KV head) that one warp task carries.
+// Columns (token, query head of the KV head) that one CTA task carries.
 constexpr int kVecCols = 4;
 // Query rows of a per-warp group (at least one token).
 constexpr int kVecRows = 16;
-constexpr int kVecWarps = 4;
+constexpr int kVecWarps = 8;
 
 template <typename T, int VW> struct VecLoad;
 template <> struct VecLoad<float, 4> {
@@ -31,19 +31,23 @@ template <typename H> struct VecLoad<H, 1> {
   static __device__ __forceinline__ void load(const H* p, float (&x)[1]) { x[0] = Elem<H>::to_f(*p); }
 };
 
-// One warp computes C columns of one (unit, KV head): LPK lanes hold a key's
-// row (VW elements a load, EV loads), so 32 / LPK keys are worked on at once,
-// each lane group with its own running maximum, sum and output; they are
-// joined by shuffles at the end.  Bound by the key and value bytes (each
-// column chunk of a group reads them again, from L2 where there are several)
-// and, for short key ranges, by the latency of the dependent loads.
+// A CTA computes C columns of one (unit, KV head): its warps take the unit's
+// keys in turn, KPW at a time a step (LPK lanes hold a key's row, VW elements
+// a load, EV loads; every lane group has a running maximum, sum and output of
+// its own), and are joined through shared memory at the end.  Bound by the
+// key and value bytes (column chunks of a group read them again, from L2) and,
+// for short key ranges, by the latency of the dependent loads: eight warps on
+// a unit make that two or three steps, and one unit a sequence needs no merge
+// (8 float32 decodes of 12 heads over 130 keys: 41 us with a warp a unit of 64
+// keys and a merge).
 template <typename T, int VW, int LPK, int EV, int C>
 __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const MaskedParams p) {
   constexpr int KPW = 32 / LPK;  // keys per step of the warp
   constexpr int U = EV * VW >= 8 ? 2 : 4;  // steps in flight
   constexpr int E = EV * VW;
+  extern __shared__ float joined[];  // [kVecWarps][C][D + 2]
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31, li = lane % LPK, lg = lane / LPK;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, li = lane % LPK, lg = lane / LPK;
   const int n_units = min(__ldg(p.counts + 3), p.max_units);
   pdl_wait();
   const T* q = reinterpret_cast<const T*>(p.q);
@@ -52,14 +56,13 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
   const long long row_elems = (long long)p.Hkv * p.D;
   const int chunks = (p.unit_tokens * p.G + C - 1) / C;  // of the largest group; a smaller one's last tasks are empty
   const long long tasks = (long long)n_units * p.Hkv * chunks;
-  for (long long task = (long long)blockIdx.x * kVecWarps + (threadIdx.x >> 5); task < tasks;
-       task += (long long)gridDim.x * kVecWarps) {
+  for (long long task = blockIdx.x; task < tasks; task += gridDim.x) {
     const int u = (int)(task / (p.Hkv * chunks)), rest = (int)(task - (long long)u * p.Hkv * chunks);
     const int kvh = rest / chunks, c0 = (rest - kvh * chunks) * C;
     MaskedGroup g;
     const int4 un = load_record(p.units, u, g);
     if (!group_ok(p, g)) {
-      if (lane == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
+      if (threadIdx.x == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
       continue;
     }
     const int cols = g.ntok * p.G;
@@ -78,16 +81,9 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
 #pragma unroll
       for (int v = 0; v < EV; ++v) {
         const int e = (v * LPK + li) * VW;
-        float x[VW];
 #pragma unroll
-        for (int i = 0; i < VW; ++i) x[i] = 0.f;
-        if (e < p.D) {
-          // queries may start at any element of their row's allocation: element loads
-#pragma unroll
-          for (int i = 0; i < VW; ++i) x[i] = Elem<T>::to_f(qrow[e + i]);
-        }
-#pragma unroll
-        for (int i = 0; i < VW; ++i) qr[c][v * VW + i] = x[i] * p.scale_log2;
+        for (int i = 0; i < VW; ++i)  // queries may start at any element of their row's allocation: element loads
+          qr[c][v * VW + i] = e < p.D ? Elem<T>::to_f(qrow[e + i]) * p.scale_log2 : 0.f;
       }
     }
     float m[C], l[C], acc[C][E];
@@ -98,24 +94,28 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[c][e] = 0.f;
     }
-    for (int v0 = un.x; v0 < v1; v0 += KPW * U) {
+    for (int v0 = un.x + warp * (KPW * U); v0 < v1; v0 += kVecWarps * KPW * U) {
       float kx[U][E], vx[U][E];
       int key[U];
+      long long row[U];
       // every load of the U steps first
 #pragma unroll
       for (int s = 0; s < U; ++s) {
         const int v = v0 + s * KPW + lg;
         key[s] = v < v1 ? vk.key(v) : -1;
-        const long long row = key[s] >= 0 ? key_row(p, btrow, key[s]) : -1;
-        if (row < 0) key[s] = -1;
+        row[s] = key[s] >= 0 ? key_row(p, btrow, key[s]) : -1;
+        if (row[s] < 0) key[s] = -1;
+      }
+#pragma unroll
+      for (int s = 0; s < U; ++s)
 #pragma unroll
         for (int w = 0; w < EV; ++w) {
           const int e = (w * LPK + li) * VW;
           float a[VW], b[VW];
 #pragma unroll
           for (int i = 0; i < VW; ++i) a[i] = b[i] = 0.f;
-          if (row >= 0 && e < p.D) {
-            const long long off = row * row_elems + (long long)kvh * p.D + e;
+          if (row[s] >= 0 && e < p.D) {
+            const long long off = row[s] * row_elems + (long long)kvh * p.D + e;
             VecLoad<T, VW>::load(kp + off, a);
             VecLoad<T, VW>::load(vp + off, b);
           }
@@ -125,7 +125,6 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
             vx[s][w * VW + i] = b[i];
           }
         }
-      }
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float x[U];
@@ -161,9 +160,9 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
         }
       }
     }
-    // join the lane groups
-    const int part = un.z & 0xffff, n_parts = un.z >> 16;
-    float* base = n_parts > 1 ? part_base(p, g, part, kvh) : nullptr;
+    // join the lane groups, then the warps
+    const int DJ = p.D + 2;
+    __syncthreads();  // (the task before has read the joined states)
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -177,28 +176,48 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
           acc[c][e] = acc[c][e] * a + __shfl_xor_sync(0xffffffffu, acc[c][e], o) * b;
         m[c] = mn;
       }
-      const int col = c0 + c;
-      if (col >= cols || lg != 0) continue;
-      const int head = kvh * p.G + (col - tok[c] * p.G);
+      if (lg != 0) continue;
+      float* st = joined + (warp * C + c) * DJ;
+#pragma unroll
+      for (int v = 0; v < EV; ++v) {
+        const int e = (v * LPK + li) * VW;
+        if (e < p.D)
+#pragma unroll
+          for (int i = 0; i < VW; ++i) st[e + i] = acc[c][v * VW + i];
+      }
+      if (li == 0) {
+        st[p.D] = m[c];
+        st[p.D + 1] = l[c];
+      }
+    }
+    __syncthreads();
+    const int part = un.z & 0xffff, n_parts = un.z >> 16;
+    float* rec = n_parts > 1 ? part_base(p, g, part, kvh) : nullptr;
+    const int n = min(C, cols - c0) * p.D;
+    for (int i = threadIdx.x; i < n; i += kVecWarps * 32) {
+      const int c = i / p.D, e = i - c * p.D, col = c0 + c;
+      float M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+      for (int w = 0; w < kVecWarps; ++w) M = fmaxf(M, joined[(w * C + c) * DJ + p.D]);
+      const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int w = 0; w < kVecWarps; ++w) {
+        const float* st = joined + (w * C + c) * DJ;
+        const float f = ex2(st[p.D] - base);
+        if (st[p.D] != -INFINITY) {  // (a warp whose keys the column does not see)
+          A = fmaf(st[e], f, A);
+          L = fmaf(st[p.D + 1], f, L);
+        }
+      }
       if (n_parts == 1) {
-        const float inv = l[c] > 0.f ? 1.f / l[c] : (l[c] == 0.f ? 0.f : l[c]);
-        T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok[c]) * p.out_stride + (long long)head * p.D;
-#pragma unroll
-        for (int v = 0; v < EV; ++v) {
-          const int e = (v * LPK + li) * VW;
-          if (e < p.D)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) dst[e + i] = Elem<T>::from_f(acc[c][v * VW + i] * inv);
-        }
-      } else if (base) {
-#pragma unroll
-        for (int v = 0; v < EV; ++v) {
-          const int e = (v * LPK + li) * VW;
-          if (e < p.D)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) base[(long long)col * p.DP + e + i] = acc[c][v * VW + i];
-        }
-        if (li == 0) *reinterpret_cast<float2*>(base + (long long)col * p.DP + p.DP - 4) = make_float2(m[c], l[c]);
+        const int t = col / p.G, head = kvh * p.G + (col - t * p.G);
+        const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+        reinterpret_cast<T*>(p.out)[(long long)(g.q_row0 + t) * p.out_stride + (long long)head * p.D + e] =
+            Elem<T>::from_f(A * inv);
+      } else if (rec) {
+        float* r = rec + (long long)col * p.DP;
+        r[e] = A;
+        if (e == 0) *reinterpret_cast<float2*>(r + p.DP - 4) = make_float2(M, L);
       }
     }
   }
@@ -284,10 +303,11 @@ __global__ void __launch_bounds__(256, 4) masked_merge_kernel(const MaskedParams
 // one before it ahead of its first read of what that writes).
 template <typename K>
 static int launch_masked(K kern, long long blocks, int threads, cudaStream_t st, const MaskedParams& p,
-                         const char* what) {
+                         const char* what, int smem = 0) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks < 1 ? 1 : blocks));
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -301,15 +321,15 @@ static int launch_masked(K kern, long long blocks, int threads, cudaStream_t st,
 
 template <typename T, int VW, int LPK, int EV>
 static int launch_vec(const MaskedParams& p, cudaStream_t st, const char* what) {
-  // one column per warp task where no group has more (decodes of a model without grouped heads), else four
+  // one column where no group has more (decodes of a model without grouped heads), else four
   const bool one = p.unit_tokens * p.G == 1;
   const int C = one ? 1 : kVecCols;
-  const long long chunks = (p.unit_tokens * p.G + C - 1) / C;
-  long long blocks = ((long long)p.max_units * p.Hkv * chunks + kVecWarps - 1) / kVecWarps;
+  long long blocks = (long long)p.max_units * p.Hkv * ((p.unit_tokens * p.G + C - 1) / C);
   const long long cap = (long long)sm_count() * 8;
   if (blocks > cap) blocks = cap;
-  return one ? launch_masked(masked_vec_kernel<T, VW, LPK, EV, 1>, blocks, kVecWarps * 32, st, p, what)
-             : launch_masked(masked_vec_kernel<T, VW, LPK, EV, kVecCols>, blocks, kVecWarps * 32, st, p, what);
+  const int smem = kVecWarps * C * (p.D + 2) * 4;  // 32 KB at most
+  return one ? launch_masked(masked_vec_kernel<T, VW, LPK, EV, 1>, blocks, kVecWarps * 32, st, p, what, smem)
+             : launch_masked(masked_vec_kernel<T, VW, LPK, EV, kVecCols>, blocks, kVecWarps * 32, st, p, what, smem);
 }
 
 template <typename T>

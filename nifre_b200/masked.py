@@ -187,8 +187,12 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
 
 def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
     """Keys per share of units: one share a worker, up to four where shares stay at 512 keys or more (then the queue
-    evens out the workers' speeds); 64 keys at least."""
+    evens out the workers' speeds); 64 keys at least.  ``head_dim`` 0: the kernel of other types and shapes, a CTA a
+    (unit, KV head, four rows), eight an SM, which is quick on 256 keys and would rather not merge."""
     total = int(keys.sum())
+    if not head_dim:
+        tasks = max(1, workers * 8 // (kv_heads * max(1, -(-int(rows.max()) // 4))))
+        return max(256, -(-total // (tasks * 16)) * 16)
     workers = max(1, workers * 8 // kv_heads)  # eight KV heads at a time an SM
     waves = min(4, max(1, total // (workers * 512)))
     return max(64, -(-total // (workers * waves * 16)) * 16)
@@ -309,7 +313,8 @@ class MaskedAttentionOps:
             raise IndexError(f"cache slot out of range [0, {self.batch_size})")
         unit_rows, item_rows = self.masked_limits(q_heads)
         lists = build_lists(plan.slots, plan.q_lens, plan.q_starts, plan.ctx_before, q_heads // self.n_heads, unit_rows,
-                            item_rows, self.sm_count, self.n_heads, self.head_dim, window, sinks, words)
+                            item_rows, self.sm_count, self.n_heads, self.head_dim if item_rows else 0, window,
+                            sinks, words)
         sizes = lists.sizes()
         if into is None:
             view = MaskedPlan(kind, window, sinks, q_heads, plan.rows_needed)

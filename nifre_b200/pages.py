@@ -11,6 +11,8 @@ sequence that would append into one gets a copy first.
 
 from __future__ import annotations
 
+from array import array
+
 import numpy as np
 import torch
 
@@ -60,37 +62,43 @@ class PageOps:
     def _copy_ids(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         if not src.numel():
             return
-        with torch.cuda.device(self._dev_index):
-            _lib.check(_lib.load().nf_copy_blocks(
-                self._k_ptr[0], self._v_ptr[0], self._layer_bytes, self.num_layers, self.block_size * self._row_bytes,
-                self.num_blocks, src.data_ptr(), dst.data_ptr(), src.numel(), self._status_ptr, self._stream()),
-                "nf_copy_blocks")
+        args = (self._k_ptr[0], self._v_ptr[0], self._layer_bytes, self.num_layers, self.block_size * self._row_bytes,
+                self.num_blocks, src.data_ptr(), dst.data_ptr(), src.numel(), self._status_ptr, self._stream())
+        if torch.cuda.current_device() == self._dev_index:
+            rc = _lib.load().nf_copy_blocks(*args)
+        else:
+            with torch.cuda.device(self._dev_index):
+                rc = _lib.load().nf_copy_blocks(*args)
+        if rc:
+            _lib.check(rc, "nf_copy_blocks")
 
     def _move_rows(self, moves, pos) -> None:
         """One launch of row moves (source row, destination row, rows, continues) and position records (slot, value)."""
         if not moves and not pos:
             return
-        m = np.asarray(moves, dtype=np.int32).reshape(-1, 4)
-        v = np.asarray(pos, dtype=np.int32).reshape(-1, 2)
-        most = int(m[:, 2].max()) if len(m) else 0
-        if max(len(m), len(v)) <= _lib.MOVE_LIST:
-            mp, vp, on_device = m.ctypes.data, v.ctypes.data, 0
+        most = max((m[2] for m in moves), default=0)
+        flat = array("i", [x for rec in moves for x in rec])
+        flat.extend([x for rec in pos for x in rec])
+        if max(len(moves), len(pos)) <= _lib.MOVE_LIST:  # read before the call returns
+            mp, on_device = flat.buffer_info()[0], 0
         else:
-            both = torch.from_numpy(np.concatenate([m.reshape(-1), v.reshape(-1)])).pin_memory()
-            keep = both.to(self.device, non_blocking=True)
+            keep = torch.frombuffer(flat, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
             mp, on_device = keep.data_ptr(), 1
-            vp = mp + 16 * len(m)
-        with torch.cuda.device(self._dev_index):
-            _lib.check(_lib.load().nf_kv_move(
-                self._k_ptr[0], self._v_ptr[0], self._layer_bytes, self.num_layers, self._row_bytes, self._pool_rows,
-                mp if len(m) else None, len(m), most, vp if len(v) else None, len(v), self._pos_ptr, self.batch_size,
-                on_device, self._status_ptr, self._stream()), "nf_kv_move")
+        args = (self._k_ptr[0], self._v_ptr[0], self._layer_bytes, self.num_layers, self._row_bytes, self._pool_rows,
+                mp if moves else None, len(moves), most, mp + 16 * len(moves) if pos else None, len(pos),
+                self._pos_ptr, self.batch_size, on_device, self._status_ptr, self._stream())
+        if torch.cuda.current_device() == self._dev_index:
+            rc = _lib.load().nf_kv_move(*args)
+        else:
+            with torch.cuda.device(self._dev_index):
+                rc = _lib.load().nf_kv_move(*args)
+        if rc:
+            _lib.check(rc, "nf_kv_move")
 
     def _slots(self, slots, what: str) -> list[int]:
         got = [int(s) for s in slots]
-        for s in got:
-            if not 0 <= s < self.batch_size:
-                raise IndexError(f"{what} {s} out of range [0, {self.batch_size})")
+        if got and (min(got) < 0 or max(got) >= self.batch_size):
+            raise IndexError(f"{what} out of range [0, {self.batch_size}): {got}")
         return got
 
     def _refuse_open(self, slots, what: str) -> None:
@@ -120,35 +128,35 @@ class PageOps:
             return
         self._refuse_open(dst, "fork")
         bs, tables, alloc = self.block_size, self.block_tables, self.block_allocator
-        todo = []
+        length, counts = self.pos_host.tolist(), alloc._refcount
+        holes = bool(self._hole_end.any())
+        todo, changed = [], []
         for s, d in zip(src, dst):
-            n = int(self.pos_host[s])
-            full, tail = n // bs, n % bs
+            n = length[s]
+            full, tail = divmod(n, bs)
             have, want = tables[d]._physical_blocks, tables[s]._physical_blocks
+            todo.append((s, d, n, full, tail))
             # a slot forked before from the same blocks keeps them
-            same = len(have) == full + (tail > 0) and have[:full] == want[:full] and \
-                (not tail or alloc._refcount[have[full]] == 1)
-            todo.append((s, d, n, full, tail, same))
-        changed = [t for t in todo if not t[5]]
+            if not (len(have) == full + (tail > 0) and have[:full] == want[:full]
+                    and (not tail or counts[have[full]] == 1)):
+                changed.append(todo[-1])
         for _, d, *_ in reversed(changed):  # the last released block is the next one allocated
             tables[d].clear()
             self.pos_host[d] = 0
             self._clear_hole(d)
-        if sum(t[4] > 0 for t in changed) > alloc.free_count:
+        need = sum(t[4] > 0 for t in changed)
+        if need > alloc.free_count:
             self._move_rows([], [(t[1], 0) for t in changed])
-            raise BlockPoolExhaustedError(f"need {sum(t[4] > 0 for t in changed)} blocks, only {alloc.free_count} free")
-        for s, d, n, full, tail, _ in changed:
+            raise BlockPoolExhaustedError(f"need {need} blocks, only {alloc.free_count} free")
+        for s, d, n, full, tail in changed:
             tables[d].share(tables[s]._physical_blocks[:full])
             if tail:
                 tables[d].ensure_capacity(n)
-        moves, pos = [], []
-        for s, d, n, full, tail, _ in todo:
-            if tail:
-                moves.append((tables[s]._physical_blocks[full] * bs, tables[d]._physical_blocks[full] * bs, tail, 0))
-            self.pos_host[d] = n
-            self._copy_hole(s, d)
-            pos.append((d, n))
-        self._move_rows(moves, pos)
+        self.pos_host[dst] = self.pos_host[src]
+        if holes:
+            self._hole_first[dst], self._hole_end[dst] = self._hole_first[src], self._hole_end[src]
+        self._move_rows([(tables[s]._physical_blocks[full] * bs, tables[d]._physical_blocks[full] * bs, tail, 0)
+                         for s, d, _, full, tail in todo if tail], [(d, n) for _, d, n, _, _ in todo])
 
     # ------------------------------------------------------------------ drafted tokens
     def keep_tokens(self, plan, paths) -> None:
@@ -269,9 +277,6 @@ class PageOps:
 
     def _clear_hole(self, slot: int) -> None:
         self._hole_first[slot] = self._hole_end[slot] = 0
-
-    def _copy_hole(self, src: int, dst: int) -> None:
-        self._hole_first[dst], self._hole_end[dst] = self._hole_first[src], self._hole_end[src]
 
     def _holes_of(self, slots) -> bool:
         return bool(self._hole_end[slots].any())
