@@ -235,12 +235,16 @@ __global__ void __launch_bounds__(256, 4) masked_merge_kernel(const MaskedParams
   const int lane = threadIdx.x & 31;
   const int n = min(__ldg(p.counts + 2), p.max_merge);
   const int D4 = p.DP / 4 - 1;
-  pdl_wait();
   const long long tasks = (long long)n * p.Hkv * 2;
-  for (long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); task < tasks; task += (long long)gridDim.x * 8) {
+  // the first task's record is not of the launch before this one: it is read while that one ends
+  MaskedGroup g;
+  long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  int4 mr = load_record(p.merge, (int)min(task / (p.Hkv * 2), (long long)p.max_merge - 1), g);
+  const long long first = task;
+  pdl_wait();
+  for (; task < tasks; task += (long long)gridDim.x * 8) {
     const int i = (int)(task / (p.Hkv * 2)), rest = (int)(task - (long long)i * p.Hkv * 2), kvh = rest >> 1;
-    MaskedGroup g;
-    const int4 mr = load_record(p.merge, i, g);
+    if (task != first) mr = load_record(p.merge, i, g);
     if (!group_ok(p, g) || mr.x <= 0 || mr.y < 0) {
       if (lane == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
       continue;

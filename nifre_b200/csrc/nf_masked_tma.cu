@@ -91,6 +91,11 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
   int u = sh.x;
   MaskedGroup g;
   int4 un = load_record(p.units, min(u, p.max_units - 1), g);
+  if (w < total && g.slot >= 0 && g.slot < p.num_slots) {  // the block tables are the step's pack's, before that launch
+    const int lb = VirtualKeys(p, g).key(un.x) / p.bs;
+    if (lb >= 0 && lb < p.max_blocks)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.bt + (long long)g.slot * p.max_blocks + lb));
+  }
   pdl_wait();
   while (w < total) {
     const int hg = w % L.n_hg, h0 = hg * L.HG;

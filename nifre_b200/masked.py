@@ -186,16 +186,16 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
 
 
 def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
-    """Keys per share of units: one share a worker, up to four where shares stay at 512 keys or more (then the queue
-    evens out the workers' speeds); 64 keys at least.  ``head_dim`` 0: the kernel of other types and shapes, a CTA a
-    (unit, KV head, four rows), eight an SM, which is quick on 256 keys and would rather not merge."""
+    """Keys per share of units: one a worker, and 64 at least.  (Finer shares and a queue over them cost more in
+    partial results than they even out: 64 windows of 4096 keys, 296 CTAs, 165 us in 127 shares, 175 in 444, 178 in
+    592.)  ``head_dim`` 0: the kernel of other types and shapes, a CTA a (unit, KV head, four rows), eight an SM,
+    which is quick on 256 keys and would rather not merge."""
     total = int(keys.sum())
     if not head_dim:
         tasks = max(1, workers * 8 // (kv_heads * max(1, -(-int(rows.max()) // 4))))
         return max(256, -(-total // (tasks * 16)) * 16)
     workers = max(1, workers * 8 // kv_heads)  # eight KV heads at a time an SM
-    waves = min(4, max(1, total // (workers * 512)))
-    return max(64, -(-total // (workers * waves * 16)) * 16)
+    return max(64, -(-total // (workers * 16)) * 16)
 
 
 def item_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
@@ -204,12 +204,12 @@ def item_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> in
     Whole groups need no merge, but the workers end unevenly; equal shares cost
     partial results (written and read: 4 (head_dim + 4) bytes a row and part)
     and the merge's launch.  Both are estimated in microseconds from a tile's
-    time (256 rows x 128 keys 1.8 at head_dim 64, 2.0 at 128; 128 rows 1.2), 2
+    time (256 rows x 128 keys 1.8 at head_dim 64, 2.0 at 128; 128 rows 1.2), 4
     an item, 4 a merge and 3 TB/s, which fit the measured cases within a fifth.
     """
     tiles = -(-keys // 128)
     cost = np.where(rows <= 128, 1.2, 1.8 if head_dim == 64 else 2.0)
-    each = tiles * cost + 2.0
+    each = tiles * cost + 4.0
     whole = max(float(each.max()), -(-len(keys) * kv_heads // workers) * float(each.mean()))
     shares = max(1, workers // kv_heads)
     share = max(256, -(-int(keys.sum()) // (shares * 128)) * 128)

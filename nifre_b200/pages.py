@@ -72,20 +72,20 @@ class PageOps:
         if rc:
             _lib.check(rc, "nf_copy_blocks")
 
-    def _move_rows(self, moves, pos) -> None:
-        """One launch of row moves (source row, destination row, rows, continues) and position records (slot, value)."""
+    def _move_rows(self, moves, pos, most: int) -> None:
+        """One launch of row moves (flat: source row, destination row, rows -- at most ``most`` --, continues) and
+        position records (flat: slot, value)."""
         if not moves and not pos:
             return
-        most = max((m[2] for m in moves), default=0)
-        flat = array("i", [x for rec in moves for x in rec])
-        flat.extend([x for rec in pos for x in rec])
-        if max(len(moves), len(pos)) <= _lib.MOVE_LIST:  # read before the call returns
+        n_moves, n_pos = len(moves) // 4, len(pos) // 2
+        flat = array("i", moves + pos)
+        if n_moves <= _lib.MOVE_LIST and n_pos <= _lib.MOVE_LIST:  # read before the call returns
             mp, on_device = flat.buffer_info()[0], 0
         else:
             keep = torch.frombuffer(flat, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
             mp, on_device = keep.data_ptr(), 1
         args = (self._k_ptr[0], self._v_ptr[0], self._layer_bytes, self.num_layers, self._row_bytes, self._pool_rows,
-                mp if moves else None, len(moves), most, mp + 16 * len(moves) if pos else None, len(pos),
+                mp if moves else None, n_moves, most, mp + 16 * n_moves if pos else None, n_pos,
                 self._pos_ptr, self.batch_size, on_device, self._status_ptr, self._stream())
         if torch.cuda.current_device() == self._dev_index:
             rc = _lib.load().nf_kv_move(*args)
@@ -129,34 +129,50 @@ class PageOps:
         self._refuse_open(dst, "fork")
         bs, tables, alloc = self.block_size, self.block_tables, self.block_allocator
         length, counts = self.pos_host.tolist(), alloc._refcount
-        holes = bool(self._hole_end.any())
-        todo, changed = [], []
+        held = {}  # per source: length, full blocks, tokens of the last block, its full blocks, its last block
+        for s in src:
+            if s not in held:
+                full, tail = divmod(length[s], bs)
+                blocks = tables[s]._physical_blocks
+                held[s] = (length[s], full, tail, blocks[:full], blocks[full] * bs if tail else 0)
+        changed = []
         for s, d in zip(src, dst):
-            n = length[s]
-            full, tail = divmod(n, bs)
-            have, want = tables[d]._physical_blocks, tables[s]._physical_blocks
-            todo.append((s, d, n, full, tail))
             # a slot forked before from the same blocks keeps them
-            if not (len(have) == full + (tail > 0) and have[:full] == want[:full]
-                    and (not tail or counts[have[full]] == 1)):
-                changed.append(todo[-1])
-        for _, d, *_ in reversed(changed):  # the last released block is the next one allocated
+            _, full, tail, want, _ = held[s]
+            have = tables[d]._physical_blocks
+            if tail:
+                if len(have) != full + 1 or counts[have[full]] != 1 or have[:full] != want:
+                    changed.append((s, d))
+            elif have != want:
+                changed.append((s, d))
+        if changed:
+            self._refork(changed, held)
+        self.pos_host[dst] = [held[s][0] for s in src]
+        if self._hole_end.any():
+            self._hole_first[dst], self._hole_end[dst] = self._hole_first[src], self._hole_end[src]
+        moves, pos = [], []
+        for s, d in zip(src, dst):
+            n, full, tail, _, row = held[s]
+            if tail:
+                moves += (row, tables[d]._physical_blocks[full] * bs, tail, 0)
+            pos += (d, n)
+        self._move_rows(moves, pos, bs)
+
+    def _refork(self, pairs, held) -> None:
+        """Give the destination slots of the pairs their sources' full blocks and a last block of their own."""
+        tables, alloc = self.block_tables, self.block_allocator
+        for _, d in reversed(pairs):  # the last released block is the next one allocated
             tables[d].clear()
             self.pos_host[d] = 0
             self._clear_hole(d)
-        need = sum(t[4] > 0 for t in changed)
+        need = sum(held[s][2] > 0 for s, _ in pairs)
         if need > alloc.free_count:
-            self._move_rows([], [(t[1], 0) for t in changed])
+            self._move_rows([], [x for _, d in pairs for x in (d, 0)], 0)
             raise BlockPoolExhaustedError(f"need {need} blocks, only {alloc.free_count} free")
-        for s, d, n, full, tail in changed:
-            tables[d].share(tables[s]._physical_blocks[:full])
-            if tail:
-                tables[d].ensure_capacity(n)
-        self.pos_host[dst] = self.pos_host[src]
-        if holes:
-            self._hole_first[dst], self._hole_end[dst] = self._hole_first[src], self._hole_end[src]
-        self._move_rows([(tables[s]._physical_blocks[full] * bs, tables[d]._physical_blocks[full] * bs, tail, 0)
-                         for s, d, _, full, tail in todo if tail], [(d, n) for _, d, n, _, _ in todo])
+        for s, d in pairs:
+            tables[d].share(held[s][3])
+            if held[s][2]:
+                tables[d].ensure_capacity(held[s][0])
 
     # ------------------------------------------------------------------ drafted tokens
     def keep_tokens(self, plan, paths) -> None:
@@ -196,16 +212,15 @@ class PageOps:
                 if t == j:
                     continue
                 a, b = c + t, c + j
-                row = (blocks[a // bs] * bs + a % bs, blocks[b // bs] * bs + b % bs)
-                last = moves[-1] if started else None
-                if last and row[0] == last[0] + last[2] and row[1] == last[1] + last[2]:
-                    moves[-1] = (last[0], last[1], last[2] + 1, last[3])
+                src, dst = blocks[a // bs] * bs + a % bs, blocks[b // bs] * bs + b % bs
+                if started and src == moves[-4] + moves[-2] and dst == moves[-3] + moves[-2]:
+                    moves[-2] += 1  # one run of rows
                 else:
-                    moves.append((*row, 1, started))
+                    moves += (src, dst, 1, started)
                     started = 1
             self.pos_host[s] = c + len(path)
-            pos.append((s, c + len(path)))
-        self._move_rows(moves, pos)
+            pos += (s, c + len(path))
+        self._move_rows(moves, pos, bs)
 
     def _own_blocks(self, slot: int, first: int, end: int) -> None:
         """Replace blocks first .. end-1 of the slot's table that others hold too by copies of its own."""
