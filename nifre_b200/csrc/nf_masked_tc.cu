@@ -875,12 +875,11 @@ __global__ void __launch_bounds__(TcCfg<D_>::THREADS, 1)
   }
 }
 
-// 256 rows of whole tokens: any group of up to 64 query heads per KV head.
+// 256 rows of whole tokens, for the shapes whose small groups the tensor-map kernel takes.
 int masked_tc_rows(int dtype, int Hq, int Hkv, int D, int bs) {
-  if (dtype != NF_BF16 && dtype != NF_F16) return 0;
-  if ((D != 64 && D != 128) || bs % 16) return 0;
+  if (!masked_tma_rows(dtype, Hq, Hkv, D, bs)) return 0;
   const int G = Hq / Hkv;
-  return G <= 64 ? 2 * (128 / G) * G : 0;
+  return 2 * (128 / G) * G;
 }
 
 template <typename T, int D_>

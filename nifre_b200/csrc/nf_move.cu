@@ -4,7 +4,9 @@
 //
 // Bound by HBM: each byte is read once and written once.  A CTA takes tiles
 // of kTileCols 16-byte columns of a record's rows, every thread with four
-// loads in flight before its stores.  Records that continue a run are ordered
+// loads in flight before its stores; a CTA a tile (1000 blocks of 16 layers, 1.05
+// GB: 161 us, the measured copy bandwidth; a grid of eight CTAs an SM that walk
+// the tiles 183 us, cache hints and eight loads no better).  Records that continue a run are ordered
 // after the ones before them: the CTA that holds the run's tile walks its
 // records row by row, each thread on its own column, so rows may move onto
 // rows that the run has read already (no other thread touches the column).
@@ -123,8 +125,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_cons
 template <typename V, typename L>
 static int launch_move(const MoveParams& p, const L& lists, cudaStream_t st) {
   long long blocks = (long long)p.n_moves * p.layers * 2 * p.n_tiles;
-  const long long cap = (long long)sm_count() * 8;
-  if (blocks > cap) blocks = cap;
+  if (blocks > (1 << 30)) blocks = 1 << 30;
   if (blocks < 1) blocks = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);

@@ -250,8 +250,9 @@ class MaskedAttentionOps:
         ``q_heads``: query heads of the attention calls (default: those of
         ``plan``).  ``into``: a plan of the same window from an earlier step of
         the batch, whose device buffers are filled again, so that a CUDA graph
-        captured with it reads the new step; ValueError where the new lists do
-        not fit them (then capture again with a new plan).
+        captured with it reads the new step (refill on the stream that
+        replays it); ValueError where the new lists do not fit them (then
+        capture again with a new plan).
         """
         if int(window) != window or window <= 0:
             raise ValueError(f"window must be a positive whole number, got {window}")
@@ -311,6 +312,8 @@ class MaskedAttentionOps:
             raise ValueError(f"q_heads must be a positive multiple of the cache's {self.n_heads} heads, got {q_heads}")
         if int(plan.slots.max()) >= self.batch_size:
             raise IndexError(f"cache slot out of range [0, {self.batch_size})")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("plans are made outside a CUDA graph capture (and refilled with into=)")
         unit_rows, item_rows = self.masked_limits(q_heads)
         lists = build_lists(plan.slots, plan.q_lens, plan.q_starts, plan.ctx_before, q_heads // self.n_heads, unit_rows,
                             item_rows, self.sm_count, self.n_heads, self.head_dim if item_rows else 0, window,
@@ -331,7 +334,7 @@ class MaskedAttentionOps:
         view.upload_bytes = host.numel() * 4
         if into is not None:
             view.buf.copy_(host, non_blocking=True)
-            view.ready.record()
+            view.ready.record(torch.cuda.current_stream(self.device))
             return view
         view.buf = host.to(self.device, non_blocking=True)
         D, room = self.head_dim, view.room

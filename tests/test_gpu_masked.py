@@ -119,7 +119,7 @@ SHAPES = [(32, 8, 64, 16, BF), (8, 8, 64, 32, HF), (8, 1, 128, 16, HF), (16, 4, 
 IDS = [f"{a}q{b}kv{c}d{d}b{str(e)[6:]}" for a, b, c, d, e in SHAPES]
 
 
-@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 1), (64, 4), (130, 33), (1000, 0), (1 << 30, 0)])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (5, 1), (64, 4), (130, 33), (1000, 0), (3, 1 << 30)])
 @pytest.mark.parametrize("shape", SHAPES, ids=IDS)
 def test_window_attention(shape, window, sinks):
     """Empty and short contexts, block and tile edges, decodes, short chunks and prefill chunks in one step."""
@@ -256,9 +256,43 @@ def test_scales(scale):
     st.tree([np.tril(np.ones((m, m), bool)) for m in st.n], scale=scale)
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(16, 8, 128), (8, 8, 96)])
+def test_pools_past_32_bit_offsets(hq, hkv, d):
+    """Blocks whose elements lie more than 2^31 past the pool's start, decodes, a chunk and a tree."""
+    from nifre_b200 import PagedKVCache
+    bs, per = 16, 16 * hkv * d
+    blocks = (1 << 31) // per + 64
+    cache = PagedKVCache(1, 1024, hkv, d, device=DEV, dtype=HF, block_size=bs, enable_prefix_cache=False, num_blocks=blocks)
+    cache.init_batch(2)  # blocks are handed out from the last one down
+    g = torch.Generator().manual_seed(16)
+    st = Step.__new__(Step)
+    st.cache, st.g, st.dtype, st.hq, st.hkv, st.d = cache, g, HF, hq, hkv, d
+    st.k = [torch.empty(1, 0, hkv, d, dtype=HF, device=DEV) for _ in range(2)]
+    st.v = [t.clone() for t in st.k]
+    st.ctx, st.n, st.start, st.rows = [300, 200], [1, 40], [0, 1], 41
+    st._append([0, 1], st.ctx)
+    st.plan = st._append([0, 1], st.n, st.start, 41, q_heads=hq)
+    assert min(b for t in cache.block_tables for b in t.physical_blocks()) * per > 1 << 31
+    st.q = st.rand(1, 41, hq * d)
+    st.window(150, 20)
+    st.tree([np.tril(np.ones((m, m), bool)) for m in st.n])
+    src = cache.block_tables[0].physical_blocks()[0]
+    cache.copy_blocks([src], [3])
+    assert torch.equal(cache.k[0][3], cache.k[0][src]) and torch.equal(cache.v[0][3], cache.v[0][src])
+
+
+def test_plans_are_not_made_inside_a_capture():
+    st = Step([20], [1], 4, 2, 64, 16, HF, seed=17)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="capture"):
+            st.cache.plan_window(st.plan, 4, q_heads=4)
+        st.q.add_(0)
+
+
 def test_dense_cache_rows():
     from nifre_b200 import KVCache
-    for room in (16, 13):
+    for room in (9, 13):  # rows of 128 and of 132 tokens
         st = Step([30, 100], [1, 19], 4, 4, 64, None, HF, seed=10, cls=KVCache, room=room)
         st.window(50, 3)
         st.tree([np.tril(np.ones((m, m), bool)) for m in st.n])
