@@ -472,8 +472,10 @@ typedef struct NfMaskedArgs {
   int32_t dtype, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks;
   int32_t num_slots, max_blocks_per_seq, num_rows;
   int32_t max_units, unit_tokens, max_items, max_merge;
+  int32_t max_parts; /* the most parts of a merge record (a hint: 0 is none) */
   int32_t window, sinks;
   float scale;
+  int32_t pad;
 } NfMaskedArgs;
 
 int nf_window_attention(const NfMaskedArgs* args, void* stream);

@@ -89,8 +89,8 @@ class NfMaskedArgs(ctypes.Structure):
                 ("head_dim", ctypes.c_int32), ("block_size", ctypes.c_int32), ("num_blocks", ctypes.c_int32),
                 ("num_slots", ctypes.c_int32), ("max_blocks_per_seq", ctypes.c_int32), ("num_rows", ctypes.c_int32),
                 ("max_units", ctypes.c_int32), ("unit_tokens", ctypes.c_int32),
-                ("max_items", ctypes.c_int32), ("max_merge", ctypes.c_int32), ("window", ctypes.c_int32),
-                ("sinks", ctypes.c_int32), ("scale", ctypes.c_float)]
+                ("max_items", ctypes.c_int32), ("max_merge", ctypes.c_int32), ("max_parts", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("sinks", ctypes.c_int32), ("scale", ctypes.c_float), ("pad", ctypes.c_int32)]
 
 
 MOVE_LIST = 128  # NF_MOVE_LIST: nf_kv_move records that travel as kernel arguments

@@ -41,7 +41,7 @@ template <typename H> struct VecLoad<H, 1> {
 // (8 float32 decodes of 12 heads over 130 keys: 41 us with a warp a unit of 64
 // keys and a merge).
 template <typename T, int VW, int LPK, int EV, int C>
-__global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const MaskedParams p) {
+__global__ void __launch_bounds__(kVecWarps * 32, C == 1 ? 3 : 2) masked_vec_kernel(const MaskedParams p) {
   constexpr int KPW = 32 / LPK;  // keys per step of the warp
   constexpr int U = EV * VW >= 8 ? 2 : 4;  // steps in flight
   constexpr int E = EV * VW;
@@ -227,70 +227,102 @@ __global__ void __launch_bounds__(kVecWarps * 32) masked_vec_kernel(const Masked
 // l_j, always in the order of the parts.  A warp takes two rows of one
 // (group, KV head): a lane holds a float4 of one of them, so a load is whole
 // 32-byte sectors, and goes over the parts PB at a time with a running maximum
-// (one round trip to L2 per PB parts).  A merge record covers four rows.
-template <typename T>
+// (one round trip to L2 per PB parts).  A merge record covers four rows.  WAYS
+// warps share the parts of a task (joined through shared memory): 48 parts of a
+// long context would be twelve round trips for one.
+template <typename T, int WAYS>
 __global__ void __launch_bounds__(256, 4) masked_merge_kernel(const MaskedParams p) {
-  constexpr int PB = 4;
+  constexpr int PB = 4, PER = 8 / WAYS;  // tasks a CTA
+  __shared__ float4 join_a[WAYS > 1 ? 8 : 1][32];
+  __shared__ float2 join_s[WAYS > 1 ? 8 : 1][32];
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % WAYS;
   const int n = min(__ldg(p.counts + 2), p.max_merge);
   const int D4 = p.DP / 4 - 1;
   const long long tasks = (long long)n * p.Hkv * 2;
   // the first task's record is not of the launch before this one: it is read while that one ends
   MaskedGroup g;
-  long long task = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  long long task = (long long)blockIdx.x * PER + warp / WAYS;
   int4 mr = load_record(p.merge, (int)min(task / (p.Hkv * 2), (long long)p.max_merge - 1), g);
   const long long first = task;
   pdl_wait();
-  for (; task < tasks; task += (long long)gridDim.x * 8) {
+  // (a CTA's warps go through the loop together: they join inside)
+  for (; task - warp / WAYS < tasks; task += (long long)gridDim.x * PER) {
     const int i = (int)(task / (p.Hkv * 2)), rest = (int)(task - (long long)i * p.Hkv * 2), kvh = rest >> 1;
-    if (task != first) mr = load_record(p.merge, i, g);
-    if (!group_ok(p, g) || mr.x <= 0 || mr.y < 0) {
-      if (lane == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
-      continue;
+    if (task != first && task < tasks) mr = load_record(p.merge, i, g);
+    bool ok = task < tasks;
+    if (ok && (!group_ok(p, g) || mr.x <= 0 || mr.y < 0)) {
+      if (lane == 0 && way == 0) atomicOr(p.status, NF_STATUS_UNIT_OVERFLOW);
+      ok = false;
     }
     const int R = g.ntok * p.G, row = mr.y + 2 * (rest & 1) + (lane & 1);
-    if (!part_base(p, g, mr.x - 1, kvh) || row >= R) continue;
+    const float4* base = nullptr;
     // float4 c of the row at c * cs + at, and (m, l) as float4 D4
     const int cs = mr.z ? R : 1, at = mr.z ? row : row * (D4 + 1);
-    const float4* base = reinterpret_cast<const float4*>(part_base(p, g, 0, kvh)) + at;
+    if (ok && row < R && part_base(p, g, mr.x - 1, kvh))
+      base = reinterpret_cast<const float4*>(part_base(p, g, 0, kvh)) + at;
     const long long step = (long long)g.ntok * p.Hq * (D4 + 1);  // float4s between consecutive parts
-    const int tok = row / p.G;
-    T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride +
-             (long long)(kvh * p.G + row - tok * p.G) * p.D;
-    for (int c = lane >> 1; c < D4; c += 16) {
+    for (int c0 = 0; c0 < D4; c0 += 16) {
+      const int c = c0 + (lane >> 1);
       float M = -INFINITY, L = 0.f;
       float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int j = 0; j < mr.x; j += PB) {
-        float4 x[PB];
-        float2 ml[PB];
+      if (base && c < D4)
+        for (int j = way * PB; j < mr.x; j += WAYS * PB) {
+          float4 x[PB];
+          float2 ml[PB];
 #pragma unroll
-        for (int u = 0; u < PB; ++u)
-          if (j + u < mr.x) {
-            const float4* pj = base + (j + u) * step;
-            ml[u] = __ldcg(reinterpret_cast<const float2*>(pj + D4 * cs));
-            x[u] = __ldcg(pj + c * cs);
-          } else {
-            ml[u] = make_float2(-INFINITY, 0.f);
+          for (int u = 0; u < PB; ++u)
+            if (j + u < mr.x) {
+              const float4* pj = base + (j + u) * step;
+              ml[u] = __ldcg(reinterpret_cast<const float2*>(pj + D4 * cs));
+              x[u] = __ldcg(pj + c * cs);
+            } else {
+              ml[u] = make_float2(-INFINITY, 0.f);
+            }
+          float nm = M;
+#pragma unroll
+          for (int u = 0; u < PB; ++u) nm = fmaxf(nm, ml[u].x);
+          const float b = nm == -INFINITY ? 0.f : nm, sc = ex2(M - b);
+          A.x *= sc; A.y *= sc; A.z *= sc; A.w *= sc; L *= sc;
+#pragma unroll
+          for (int u = 0; u < PB; ++u)
+            if (ml[u].x != -INFINITY) {  // (a part without seen keys)
+              const float w = ex2(ml[u].x - b);
+              A.x = fmaf(x[u].x, w, A.x); A.y = fmaf(x[u].y, w, A.y);
+              A.z = fmaf(x[u].z, w, A.z); A.w = fmaf(x[u].w, w, A.w);
+              L = fmaf(ml[u].y, w, L);
+            }
+          M = nm;
+        }
+      if constexpr (WAYS > 1) {
+        __syncthreads();  // (the join before has been read)
+        join_a[warp][lane] = A;
+        join_s[warp][lane] = make_float2(M, L);
+        __syncthreads();
+        if (way == 0) {
+          float nm = M;
+#pragma unroll
+          for (int w = 1; w < WAYS; ++w) nm = fmaxf(nm, join_s[warp + w][lane].x);
+          const float b = nm == -INFINITY ? 0.f : nm, f0 = ex2(M - b);
+          A.x *= f0; A.y *= f0; A.z *= f0; A.w *= f0; L *= f0;
+#pragma unroll
+          for (int w = 1; w < WAYS; ++w) {
+            const float2 s = join_s[warp + w][lane];
+            const float4 x = join_a[warp + w][lane];
+            if (s.x != -INFINITY) {
+              const float f = ex2(s.x - b);
+              A.x = fmaf(x.x, f, A.x); A.y = fmaf(x.y, f, A.y); A.z = fmaf(x.z, f, A.z); A.w = fmaf(x.w, f, A.w);
+              L = fmaf(s.y, f, L);
+            }
           }
-        float nm = M;
-#pragma unroll
-        for (int u = 0; u < PB; ++u) nm = fmaxf(nm, ml[u].x);
-        const float b = nm == -INFINITY ? 0.f : nm, sc = ex2(M - b);
-        A.x *= sc; A.y *= sc; A.z *= sc; A.w *= sc; L *= sc;
-#pragma unroll
-        for (int u = 0; u < PB; ++u)
-          if (ml[u].x != -INFINITY) {  // (a part without seen keys)
-            const float w = ex2(ml[u].x - b);
-            A.x = fmaf(x[u].x, w, A.x); A.y = fmaf(x[u].y, w, A.y);
-            A.z = fmaf(x[u].z, w, A.z); A.w = fmaf(x[u].w, w, A.w);
-            L = fmaf(ml[u].y, w, L);
-          }
-        M = nm;
+        }
       }
+      if (way != 0 || !base || c >= D4) continue;
       const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
       const float o[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
-      T* d = dst + 4 * c;
+      const int tok = row / p.G;
+      T* d = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride +
+             (long long)(kvh * p.G + row - tok * p.G) * p.D + 4 * c;
       if (sizeof(T) == 2 && 4 * c + 4 <= p.D && (reinterpret_cast<uintptr_t>(d) & 7) == 0) {
         if constexpr (sizeof(T) == 2)
           *reinterpret_cast<uint2*>(d) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
@@ -323,6 +355,16 @@ static int launch_masked(K kern, long long blocks, int threads, cudaStream_t st,
   return check_launch(what);
 }
 
+template <typename T>
+static int launch_merge(const MaskedParams& p, int max_parts, cudaStream_t st, const char* what) {
+  const int ways = max_parts <= 8 ? 1 : max_parts <= 16 ? 2 : 8;
+  const long long want = ((long long)p.max_merge * p.Hkv * 2 * ways + 7) / 8, cap = (long long)sm_count() * 8;
+  const long long blocks = want < cap ? want : cap;
+  if (ways == 1) return launch_masked(masked_merge_kernel<T, 1>, blocks, 256, st, p, what);
+  if (ways == 2) return launch_masked(masked_merge_kernel<T, 2>, blocks, 256, st, p, what);
+  return launch_masked(masked_merge_kernel<T, 8>, blocks, 256, st, p, what);
+}
+
 template <typename T, int VW, int LPK, int EV>
 static int launch_vec(const MaskedParams& p, cudaStream_t st, const char* what) {
   // one column where no group has more (decodes of a model without grouped heads), else four
@@ -342,11 +384,16 @@ static int dispatch_vec(const MaskedParams& p, cudaStream_t st, const char* what
   const bool vec = p.D % VW == 0 &&
                    ((reinterpret_cast<uintptr_t>(p.kp) | reinterpret_cast<uintptr_t>(p.vp)) & 15) == 0;
   if (!vec) return launch_vec<T, 1, 32, 8>(p, st, what);
+  // eight lanes a key where registers allow (three shuffles a score, four keys at a time)
   const int n = p.D / VW;
   if (n <= 8) return launch_vec<T, VW, 8, 1>(p, st, what);
+  if constexpr (sizeof(T) == 4) {
+    if (n <= 16) return launch_vec<T, VW, 8, 2>(p, st, what);
+    if (n <= 32) return launch_vec<T, VW, 16, 2>(p, st, what);
+    return launch_vec<T, VW, 32, 2>(p, st, what);
+  }
   if (n <= 16) return launch_vec<T, VW, 16, 1>(p, st, what);
   if (n <= 32) return launch_vec<T, VW, 32, 1>(p, st, what);
-  if constexpr (sizeof(T) == 4) return launch_vec<T, VW, 32, 2>(p, st, what);
   return fail(NF_EUNSUPPORTED, "%s: head_dim %d > 256", what, p.D);
 }
 
@@ -446,12 +493,10 @@ static int masked_attention(const NfMaskedArgs* a, bool tree, const char* what, 
     if (rc) return rc;
   }
   if (p.max_merge) {
-    const long long want = ((long long)p.max_merge * p.Hkv * 2 + 7) / 8, cap = (long long)sm_count() * 8;
-    const long long blocks = want < cap ? want : cap;
     switch (a->dtype) {
-      case NF_F32: return launch_masked(masked_merge_kernel<float>, blocks, 256, st, p, what);
-      case NF_F16: return launch_masked(masked_merge_kernel<__half>, blocks, 256, st, p, what);
-      default: return launch_masked(masked_merge_kernel<__nv_bfloat16>, blocks, 256, st, p, what);
+      case NF_F32: return launch_merge<float>(p, a->max_parts, st, what);
+      case NF_F16: return launch_merge<__half>(p, a->max_parts, st, what);
+      default: return launch_merge<__nv_bfloat16>(p, a->max_parts, st, what);
     }
   }
   return ok();

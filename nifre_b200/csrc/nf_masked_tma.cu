@@ -131,10 +131,10 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
         nsh = load_share(p.unit_shares, wn / L.n_hg, p.max_units);
         nu_at = nsh.x;
         have = 2;
-      } else if (i == ask + 2 * kGap && have == 2) {
+      } else if (have == 2 && (more || i == ask + 2 * kGap)) {
         nu = load_record(p.units, min(nu_at, p.max_units - 1), ng);
         have = 3;
-      } else if (i == ask + 3 * kGap && have == 3 && ng.slot >= 0 && ng.slot < p.num_slots) {
+      } else if (have == 3 && i == (more ? 1 : ask + 3 * kGap) && ng.slot >= 0 && ng.slot < p.num_slots) {
         const int lb = VirtualKeys(p, ng).key(nu.x) / p.bs;
         if (lb >= 0 && lb < p.max_blocks)
           asm volatile("prefetch.global.L1 [%0];" ::"l"(p.bt + (long long)ng.slot * p.max_blocks + lb));
@@ -227,6 +227,7 @@ struct MtState {
   float m[NT][2], l[NT][2];
   float o[KS][NT][4];
   uint32_t none;
+  uint32_t tok[NT];  // the tokens of columns 8 j + 2 (lane % 4) (low half) and the next (high half)
 };
 
 // PT staged 16-key tiles of this warp's head in one update.  With eight
@@ -237,7 +238,7 @@ struct MtState {
 template <typename T, int D_, int NT, int PT, bool EARLY>
 __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGroup& g, const uint32_t (&kb)[PT],
                                           const uint32_t (&vb)[PT], const int (&key0)[PT], const int (&nv)[PT],
-                                          int masked, int c0, MtState<D_, NT>& st) {
+                                          int masked, MtState<D_, NT>& st) {
   constexpr int KS = D_ / 16;
   const int lane = threadIdx.x & 31, tq = lane >> 2, n0 = 2 * (lane & 3);
   const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;
@@ -295,7 +296,7 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
       if (masked >> t & 1) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int row = tq + (e >> 1) * 8, tok = min((c0 + 8 * j + n0 + (e & 1)) / p.G, g.ntok - 1);
+          const int row = tq + (e >> 1) * 8, tok = e & 1 ? st.tok[j] >> 16 : st.tok[j] & 0xffff;
           if (row >= nv[t] || !sees(p, g, tok, key0[t] + row)) x[t][j][e] = -INFINITY;
         }
       }
@@ -446,6 +447,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
             }
             st.qf[j][ks][h] = v;
           }
+        st.tok[j] = min((c0 + 8 * j + n0) / p.G, g.ntok - 1) | min((c0 + 8 * j + n0 + 1) / p.G, g.ntok - 1) << 16;
         st.m[j][0] = st.m[j][1] = 0.f;
         st.l[j][0] = st.l[j][1] = 0.f;
       }
@@ -474,7 +476,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
       const uint32_t kb[2] = {sb0 + head_region, sb1 + head_region};
       const uint32_t vb[2] = {kb[0] + L.box_bytes, kb[1] + L.box_bytes};
       const int key0[2] = {r.y, r1.y}, nv[2] = {r.z, r1.z};
-      mt_update<T, D_, NT, 2, CW == 1>(p, g, kb, vb, key0, nv, (r.w & kMtMasked ? 1 : 0) | (r1.w & kMtMasked ? 2 : 0), c0, st);
+      mt_update<T, D_, NT, 2, CW == 1>(p, g, kb, vb, key0, nv, (r.w & kMtMasked ? 1 : 0) | (r1.w & kMtMasked ? 2 : 0), st);
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(hdr + 64 + 8 * s0);
@@ -483,7 +485,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
     } else {
       const uint32_t kb[1] = {sb0 + head_region}, vb[1] = {kb[0] + L.box_bytes};
       const int key0[1] = {r.y}, nv[1] = {r.z};
-      mt_update<T, D_, NT, 1, false>(p, g, kb, vb, key0, nv, r.w & kMtMasked ? 1 : 0, c0, st);
+      mt_update<T, D_, NT, 1, false>(p, g, kb, vb, key0, nv, r.w & kMtMasked ? 1 : 0, st);
       __syncwarp();
       if (lane == 0) mbar_arrive(hdr + 64 + 8 * s0);
     }

@@ -52,22 +52,25 @@ def virtual_keys(pos0, ntok, window: int, sinks: int):
     return kept, gap, pos0 + ntok - gap
 
 
-def even_shares(keys, share: int, align: int, least: int):
+def even_shares(keys, share: int, align: int, least: int, each: int = 0):
     """Cut groups of ``keys`` keys into shares of about ``share`` keys by laying them end to end (then every worker has
     the same to do whatever the groups' lengths, and no group has more parts than that needs).
 
     A share is a run of units: the end of one group, whole groups, the start of
-    another.  Cuts sit at multiples of ``align`` of their group and at least
-    ``least`` keys from its ends, else at its nearer end.  Returns per unit
-    (group, first key, end), in order, and the shares' first units (and the
-    number of units).
+    another.  A group counts ``each`` keys more than it has (what a unit costs
+    besides its keys).  Cuts sit at multiples of ``align`` of their group and
+    at least ``least`` keys from its ends, else at its nearer end.  Returns per
+    unit (group, first key, end), in order, and the shares' first units (and
+    the number of units).
     """
     keys = np.asarray(keys, dtype=np.int64)
     end = np.cumsum(keys)
     start = end - keys
-    cuts = np.arange(share, int(end[-1]), share)
-    g = np.searchsorted(end, cuts, side="right")
-    at = (cuts - start[g] + align // 2) // align * align
+    cost = np.cumsum(keys + each)
+    cuts = np.arange(share, int(cost[-1]), share)
+    g = np.searchsorted(cost, cuts, side="right")
+    at = cuts - (cost[g] - keys[g])  # below 0: among what the group costs besides
+    at = (np.maximum(at, 0) + align // 2) // align * align
     low, high = at < least, keys[g] - at < least
     at = np.where(low & (~high | (2 * at <= keys[g])), 0, np.where(high, keys[g], at))
     where = np.unique(np.concatenate([[0], start[g] + at, [int(end[-1])]]))  # the shares' bounds
@@ -81,20 +84,22 @@ class WorkLists:
     """Units, tensor-core items and merge records of one step (each record with its group's fields), the shares of
     units and items that workers take, the mask words, and their place in one int32 buffer."""
 
-    def __init__(self, units, items, merge, masks, unit_shares, item_shares, part_rows: int, unit_tokens: int):
+    def __init__(self, units, items, merge, masks, unit_shares, item_shares, part_rows: int, unit_tokens: int,
+                 max_parts: int):
         self.units, self.items, self.merge, self.masks = units, items, merge, masks
         self.unit_shares, self.item_shares = unit_shares, item_shares
-        self.part_rows, self.unit_tokens = part_rows, unit_tokens
+        self.part_rows, self.unit_tokens, self.max_parts = part_rows, unit_tokens, max_parts
 
     def sizes(self):
-        """Entries of each list, the partial rows and the tokens of the largest unit's group."""
-        return (len(self.units), len(self.items), len(self.merge), len(self.masks), self.part_rows, self.unit_tokens)
+        """Entries of each list, the partial rows, the tokens of the largest unit's group and the most parts."""
+        return (len(self.units), len(self.items), len(self.merge), len(self.masks), self.part_rows, self.unit_tokens,
+                self.max_parts)
 
     @staticmethod
     def room(sizes):
         """Capacities for lists of these sizes: whole multiples of 64 entries, so that the next steps' lists of the
         same batch fit as well (the launches are sized by the capacities)."""
-        return (*(-(-n // 64) * 64 for n in sizes[:5]), sizes[5])
+        return (*(-(-n // 64) * 64 for n in sizes[:5]), sizes[5], -(-sizes[6] // 4) * 4)
 
     @staticmethod
     def offsets(room):
@@ -146,8 +151,8 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
         masks = np.concatenate([w.reshape(-1) for w in words])
     on_items = routed[seq]
     cuts = []  # (group, first key, end) of every unit and of every item, and the shares of them
-    for on, share, align, least, share_for in ((~on_items, unit_share, 16, 64, unit_share_for),
-                                               (on_items, item_share, 128, 128, item_share_for)):
+    for on, share, align, least, each, share_for in ((~on_items, unit_share, 16, 64, 48, unit_share_for),
+                                                     (on_items, item_share, 128, 128, 256, item_share_for)):
         mine = np.flatnonzero(on)
         if not len(mine):
             cuts.append((mine, mine, mine, mine))
@@ -155,7 +160,7 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
         k = keys[mine]
         share = share or share_for(k, ntok[mine] * group, workers, kv_heads, head_dim)
         if share:
-            g, k0, k1, at = even_shares(k, share, align, least)
+            g, k0, k1, at = even_shares(k, share, align, least, each)
         else:  # whole groups, the longest first
             g = np.argsort(-k, kind="stable")
             k0, k1, at = 0 * k, k[g], np.arange(len(k) + 1)
@@ -182,7 +187,7 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
     t = np.arange(len(m)) - np.repeat(np.cumsum(fours) - fours, fours)
     merge = np.concatenate([np.stack([parts[m], 4 * t, on_items[m], 0 * t], axis=1), groups[m]], axis=1).astype(np.int32)
     return WorkLists(listed(*cuts[0]), listed(*cuts[1]), merge, masks, cuts[0][3], cuts[1][3], int(rows.sum()),
-                     int(ntok[~on_items].max()) if (~on_items).any() else 0)
+                     int(ntok[~on_items].max()) if (~on_items).any() else 0, int(parts.max()))
 
 
 def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
@@ -190,12 +195,12 @@ def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> in
     partial results than they even out: 64 windows of 4096 keys, 296 CTAs, 165 us in 127 shares, 175 in 444, 178 in
     592.)  ``head_dim`` 0: the kernel of other types and shapes, a CTA a (unit, KV head, four rows), eight an SM,
     which is quick on 256 keys and would rather not merge."""
-    total = int(keys.sum())
     if not head_dim:
-        tasks = max(1, workers * 8 // (kv_heads * max(1, -(-int(rows.max()) // 4))))
-        return max(256, -(-total // (tasks * 16)) * 16)
+        each = kv_heads * max(1, -(-int(rows.max()) // 4))  # CTAs a unit
+        return max(256 if len(keys) * each >= 48 else 128,
+                   -(-int(keys.sum()) * each // (workers * 8 * 16)) * 16)
     workers = max(1, workers * 8 // kv_heads)  # eight KV heads at a time an SM
-    return max(64, -(-total // (workers * 16)) * 16)
+    return max(64, -(-int(keys.sum() + 48 * len(keys)) // (workers * 16)) * 16)
 
 
 def item_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
@@ -205,19 +210,24 @@ def item_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> in
     partial results (written and read: 4 (head_dim + 4) bytes a row and part)
     and the merge's launch.  Both are estimated in microseconds from a tile's
     time (256 rows x 128 keys 1.8 at head_dim 64, 2.0 at 128; 128 rows 1.2), 4
-    an item, 4 a merge and 3 TB/s, which fit the measured cases within a fifth.
+    an item, 4 a merge, 0.3 a part of the longest group and 3 TB/s, which fit the
+    measured cases within a fifth.
     """
     tiles = -(-keys // 128)
     cost = np.where(rows <= 128, 1.2, 1.8 if head_dim == 64 else 2.0)
     each = tiles * cost + 4.0
-    whole = max(float(each.max()), -(-len(keys) * kv_heads // workers) * float(each.mean()))
-    shares = max(1, workers // kv_heads)
-    share = max(256, -(-int(keys.sum()) // (shares * 128)) * 128)
-    cuts = int(keys.sum()) // share
-    parts = cuts + min(cuts, len(keys))  # partial results: two at a group's first cut, one more at each further
-    cut = max(float((tiles * cost).sum()) / shares, 2 * float(cost.min())) + 8.0 + \
-        parts * float(rows.mean()) * kv_heads * 4 * (head_dim + 4) * 2 / 3e6
-    return share if cut < whole else 0
+    best, share = max(float(each.max()), -(-len(keys) * kv_heads // workers) * float(each.mean())), 0
+    total, work = int(keys.sum()) + 256 * len(keys), float((tiles * cost).sum())
+    even = max(256, -(-total // (max(1, workers // kv_heads) * 128)) * 128)
+    for s in (even, 2 * even, 4 * even):
+        shares = -(-total // s)
+        cuts = max(0, shares - 1)
+        parts = cuts + min(cuts, len(keys))  # partial results: two at a group's first cut, one more at each further
+        cut = work / shares * -(-shares * kv_heads // workers) + 8.0 + 0.3 * float(keys.max()) / s + \
+            parts * float(rows.mean()) * kv_heads * 4 * (head_dim + 4) * 2 / 3e6
+        if cut < best:
+            best, share = cut, s
+    return share
 
 
 class MaskedPlan:
@@ -349,7 +359,7 @@ class MaskedAttentionOps:
             status=self._status_ptr, dtype=self._dt_code, num_q_heads=q_heads, num_kv_heads=self.n_heads, head_dim=D,
             block_size=self.block_size, num_blocks=self.num_blocks, num_slots=self.batch_size,
             max_blocks_per_seq=self.max_blocks_per_seq, max_units=room[0], unit_tokens=room[5], max_items=room[1],
-            max_merge=room[2], window=window, sinks=sinks)
+            max_merge=room[2], max_parts=room[6], window=window, sinks=sinks)
         view.args_ptr = ctypes.addressof(view.args)
         lib = _lib.load()
         view.fn = lib.nf_tree_attention if kind == "tree" else lib.nf_window_attention

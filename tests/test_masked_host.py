@@ -105,7 +105,8 @@ def test_even_shares_cover_every_group_in_order():
     for n, most, share, align in ((1, 5, 64, 16), (9, 3000, 448, 16), (40, 200, 64, 16), (5, 9000, 256, 128), (64, 1041, 464, 16)):
         keys = rng.integers(1, most, size=n)
         least = 4 * align
-        g, k0, k1, at = even_shares(keys, share, align, least)
+        each = int(rng.integers(0, 60))
+        g, k0, k1, at = even_shares(keys, share, align, least, each)
         assert (k0 < k1).all() and (k0 % align == 0).all()
         assert (np.diff(g) >= 0).all() and set(g.tolist()) == set(range(n))
         for i in range(n):
@@ -115,7 +116,7 @@ def test_even_shares_cover_every_group_in_order():
                 assert (k1[mine] - k0[mine]).min() >= min(least, share - align)
         assert at[0] == 0 and at[-1] == len(g) and (np.diff(at) > 0).all()
         sizes = np.add.reduceat(k1 - k0, at[:-1])
-        assert sizes.max() <= share + 2 * least + align  # each bound moves by less than least
+        assert sizes.max() <= share + 2 * (least + align)  # each bound moves by less than least and the rounding
 
 
 def test_packed_lists_and_room():
