@@ -357,8 +357,10 @@ static int launch_masked(K kern, long long blocks, int threads, cudaStream_t st,
 
 template <typename T>
 static int launch_merge(const MaskedParams& p, int max_parts, cudaStream_t st, const char* what) {
-  const int ways = max_parts <= 8 ? 1 : max_parts <= 16 ? 2 : 8;
-  const long long want = ((long long)p.max_merge * p.Hkv * 2 * ways + 7) / 8, cap = (long long)sm_count() * 8;
+  // several warps a task where there are few tasks with many parts; with many tasks the loads in flight are enough
+  const long long tasks = (long long)p.max_merge * p.Hkv * 2, cap = (long long)sm_count() * 8;
+  const int ways = max_parts <= 8 || tasks > 2 * cap ? 1 : max_parts <= 16 ? 2 : 8;
+  const long long want = (tasks * ways + 7) / 8;
   const long long blocks = want < cap ? want : cap;
   if (ways == 1) return launch_masked(masked_merge_kernel<T, 1>, blocks, 256, st, p, what);
   if (ways == 2) return launch_masked(masked_merge_kernel<T, 2>, blocks, 256, st, p, what);

@@ -241,8 +241,10 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
                                           int masked, MtState<D_, NT>& st) {
   constexpr int KS = D_ / 16;
   const int lane = threadIdx.x & 31, tq = lane >> 2, n0 = 2 * (lane & 3);
-  const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, kc = lane >> 4;
-  const int vr = (lane & 7) + ((lane >> 4) & 1) * 8, vc = (lane >> 3) & 1;
+  // this lane's row and chunk of the fragments; k-step i is an exclusive or of the chunk bits (mt_off(r, 2 i + c))
+  const int kr = (lane & 7) + ((lane >> 3) & 1) * 8, vr = (lane & 7) + ((lane >> 4) & 1) * 8;
+  const uint32_t ko = mt_off(kr, lane >> 4), vo = mt_off(vr, (lane >> 3) & 1);
+  auto step_at = [](uint32_t a, int i) { return (a ^ ((i & 3) << 5)) + (i >> 2) * 2048; };
   float x[PT][NT][4];
   // fragments of both tiles (and of the values) at once where registers allow, else a tile's at a time
   constexpr bool kEarly = EARLY;
@@ -256,7 +258,7 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
     for (int t = 0; t < PT; ++t)
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        ldsm_x4(kb[t] + mt_off(kr, 2 * ks + kc), kf[t][ks][0], kf[t][ks][1], kf[t][ks][2], kf[t][ks][3]);
+        ldsm_x4(step_at(kb[t] + ko, ks), kf[t][ks][0], kf[t][ks][1], kf[t][ks][2], kf[t][ks][3]);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -268,7 +270,7 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
     for (int t = 0; t < PT; ++t) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        ldsm_x4(kb[t] + mt_off(kr, 2 * ks + kc), kf[0][ks][0], kf[0][ks][1], kf[0][ks][2], kf[0][ks][3]);
+        ldsm_x4(step_at(kb[t] + ko, ks), kf[0][ks][0], kf[0][ks][1], kf[0][ks][2], kf[0][ks][3]);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -281,7 +283,7 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
     for (int t = 0; t < PT; ++t)
 #pragma unroll
       for (int i = 0; i < KS; ++i)
-        ldsm_x4_t(vb[t] + mt_off(vr, 2 * i + vc), vf[t][i][0], vf[t][i][1], vf[t][i][2], vf[t][i][3]);
+        ldsm_x4_t(step_at(vb[t] + vo, i), vf[t][i][0], vf[t][i][1], vf[t][i][2], vf[t][i][3]);
   }
   // exponents against the reference; unseen keys -inf
   const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
@@ -338,8 +340,8 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
     for (int t = 0; t < PT; ++t) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[t][j][e] = ex2(x[t][j][e]);
-      st.l[j][0] += x[t][j][0] + x[t][j][2];
-      st.l[j][1] += x[t][j][1] + x[t][j][3];
+      const uint64_t s2 = f2_add(f2_pack(x[t][j][0], x[t][j][1]), f2_pack(x[t][j][2], x[t][j][3]));
+      f2_unpack(f2_add(f2_pack(st.l[j][0], st.l[j][1]), s2), st.l[j][0], st.l[j][1]);
     }
 #pragma unroll
   for (int t = 0; t < PT; ++t) {
@@ -367,7 +369,7 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
         uint32_t(&f)[4] = vf[kEarly ? t : 0][i];
-        if constexpr (!kEarly) ldsm_x4_t(vb[t] + mt_off(vr, 2 * i + vc), f[0], f[1], f[2], f[3]);
+        if constexpr (!kEarly) ldsm_x4_t(step_at(vb[t] + vo, i), f[0], f[1], f[2], f[3]);
 #pragma unroll
         for (int j = 0; j < NT; ++j) mt_mma<T>(st.o[i][j], f, pb[j][0], pb[j][1]);
       }
@@ -532,7 +534,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
 // registers a thread (setmaxnreg) and two steps an update 97 us, two warps a
 // head with 16 columns each 82 us (96 registers; more steps an update spill).
 template <typename T, int D_, int NT, int CW>
-__global__ void __launch_bounds__(32 * ((D_ == 64 ? 8 : 4) * CW + 1), D_ == 64 ? 1 : 2)
+__global__ void __launch_bounds__(32 * ((D_ == 64 ? 8 : 4) * CW + 1), D_ == 64 || CW == 4 ? 1 : 2)
     masked_tma_kernel(const MaskedParams p, const MtLaunch L, const __grid_constant__ CUtensorMap tk,
                       const __grid_constant__ CUtensorMap tv) {
   extern __shared__ unsigned char smem_raw[];
@@ -566,18 +568,19 @@ __global__ void __launch_bounds__(32 * ((D_ == 64 ? 8 : 4) * CW + 1), D_ == 64 ?
 }
 
 // Query rows of a group: two warps a head hold 16 columns of a 64-wide head
-// each, 8 of a 128-wide one.
+// each, four 8 of a 128-wide one.
 int masked_tma_rows(int dtype, int Hq, int Hkv, int D, int bs) {
   if (dtype != NF_BF16 && dtype != NF_F16) return 0;
   if ((D != 64 && D != 128) || bs % 16) return 0;
-  const int rows = D == 64 ? 32 : 16;
+  const int rows = 32;
   return Hq / Hkv <= rows ? rows : 0;
 }
 
 using MtKernel = void (*)(const MaskedParams, const MtLaunch, const CUtensorMap, const CUtensorMap);
 template <typename T>
 static MtKernel mt_kernel(int D, int cols) {
-  if (D == 128) return cols <= 8 ? masked_tma_kernel<T, 128, 1, 1> : masked_tma_kernel<T, 128, 1, 2>;
+  if (D == 128)
+    return cols <= 8 ? masked_tma_kernel<T, 128, 1, 1> : cols <= 16 ? masked_tma_kernel<T, 128, 1, 2> : masked_tma_kernel<T, 128, 1, 4>;
   return cols <= 8 ? masked_tma_kernel<T, 64, 1, 1> : cols <= 16 ? masked_tma_kernel<T, 64, 2, 1> : masked_tma_kernel<T, 64, 2, 2>;
 }
 
@@ -599,7 +602,9 @@ int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char
   L.n_hg = p.Hkv / hg;
   L.box_bytes = hg * 16 * p.D * 2;
   L.stage_bytes = 2 * L.box_bytes;
-  const int want = (p.D == 64 ? 1 : 2) * (max_hg / hg);
+  const int cols = p.unit_tokens * p.G;
+  const int cw = p.D == 64 ? (cols <= 16 ? 1 : 2) : (cols <= 8 ? 1 : cols <= 16 ? 2 : 4);
+  const int want = (p.D == 64 || cw == 4 ? 1 : 2) * (max_hg / hg);
   int stages = (228 * 1024 / want - 1024 - kMtHeader - 1024) / L.stage_bytes;
   L.stages = stages > kMtMaxStages ? kMtMaxStages : stages;
   if (L.stages < 2) return NF_EUNSUPPORTED;
@@ -611,9 +616,7 @@ int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char
     return NF_EUNSUPPORTED;
   L.evict_first = 1;
   L.q_align4 = (reinterpret_cast<uintptr_t>(p.q) % 4 == 0) && p.q_stride % 2 == 0;
-  const int cols = p.unit_tokens * p.G;
   const MtKernel kern = dtype == NF_BF16 ? mt_kernel<__nv_bfloat16>(p.D, cols) : mt_kernel<__half>(p.D, cols);
-  const int cw = cols <= (p.D == 64 ? 16 : 8) ? 1 : 2;
   const int threads = (hg * cw + 1) * 32, smem = kMtHeader + L.stages * L.stage_bytes + 1024;
   int per_sm = 1;
   cudaError_t e = prepare_launch(reinterpret_cast<const void*>(kern), smem, threads, &per_sm);
