@@ -8,8 +8,11 @@ namespace nf {
 
 // Columns (token, query head of the KV head) that one CTA task carries.
 constexpr int kVecCols = 4;
-// Query rows of a per-warp group (at least one token).
-constexpr int kVecRows = 16;
+// Query rows of a group of these kernels (at least one token), and the most of
+// a step's largest group that go to the kernel of few columns: above, tiles of
+// 32 columns read each key once for them.
+constexpr int kVecRows = 32;
+constexpr int kVecMost = 8;
 constexpr int kVecWarps = 8;
 
 template <typename T, int VW> struct VecLoad;
@@ -223,6 +226,207 @@ __global__ void __launch_bounds__(kVecWarps * 32, C == 1 ? 3 : 2) masked_vec_ker
   }
 }
 
+// Groups of many columns of the same types and shapes: a CTA takes 32 columns
+// of one (unit, KV head), four a warp, and walks the unit's keys 32 at a time,
+// K and V staged in shared memory as float32 (the next tile's rows travel
+// through registers meanwhile).  Scores with a key a lane (no sums across
+// lanes; rows padded so that the eight lanes of a 16-byte read hit distinct
+// banks), value sums with an element a lane.  Bound by instructions (about
+// 1,150 a warp and tile for 512 FMAs at head_dim 64): 8 float32 chunks of 200
+// tokens, 12 heads and a window of 256 keys 140 us, with four columns a CTA 294.
+// D <= 32 ND.
+template <typename T, int ND, bool VEC>
+__global__ void __launch_bounds__(256, ND <= 2 ? 2 : 1) masked_tile_kernel(const MaskedParams p) {
+  constexpr int VW = sizeof(T) == 4 ? 4 : 8;
+  extern __shared__ float4 tile_smem[];
+  const int D4 = (p.D + 3) >> 2, KP = D4 + 1;  // float4s of a row, and of a padded K row
+  float4* ks = tile_smem;             // [32][KP]
+  float4* vs = ks + 32 * KP;          // [32][D4]
+  float4* qs = vs + 32 * D4;          // [32][D4]
+  float4* ps = qs + 32 * D4;          // [8 warps][32 keys]: four columns' weights
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_units = min(__ldg(p.counts + 3), p.max_units);
+  pdl_wait();
+  const int blocks = (p.unit_tokens * p.G + 31) >> 5;
+  const long long tasks = (long long)n_units * p.Hkv * blocks, row_elems = (long long)p.Hkv * p.D;
+  for (long long task = blockIdx.x; task < tasks; task += gridDim.x) {
+    const int u = (int)(task / (p.Hkv * blocks)), rest = (int)(task - (long long)u * p.Hkv * blocks);
+    const int kvh = rest / blocks, c0 = (rest - kvh * blocks) * 32;
+    MaskedGroup g;
+    const int4 un = load_record(p.units, u, g);
+    if (!group_ok(p, g)) {
+      if (threadIdx.x == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
+      continue;
+    }
+    const int cols = g.ntok * p.G;
+    if (c0 >= cols) continue;
+    const VirtualKeys vk(p, g);
+    const int* btrow = p.bt + (long long)g.slot * p.max_blocks;
+    const int v1 = min(un.y, vk.end);
+    const T* kp = reinterpret_cast<const T*>(p.kp) + (long long)kvh * p.D;
+    const T* vp = reinterpret_cast<const T*>(p.vp) + (long long)kvh * p.D;
+    __syncthreads();  // (the task before is done with the shared tiles)
+    for (int i = threadIdx.x; i < 32 * D4 * 4; i += 256) {
+      const int c = i / (D4 * 4), e = i - c * (D4 * 4), col = c0 + c;
+      float x = 0.f;
+      if (col < cols && e < p.D) {
+        const int tok = col / p.G;
+        x = Elem<T>::to_f(reinterpret_cast<const T*>(p.q)[(long long)(g.q_row0 + tok) * p.q_stride +
+                                                         (long long)(kvh * p.G + col - tok * p.G) * p.D + e]);
+      }
+      reinterpret_cast<float*>(qs)[i] = x * p.scale_log2;
+    }
+    // this warp's columns; the tile after the one at work in registers
+    const int w0 = c0 + 4 * warp;
+    const bool busy = w0 < cols;
+    int tok[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) tok[c] = min(w0 + c, cols - 1) / p.G;
+    float m[4], l[4], o[4][ND];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      m[c] = -INFINITY;
+      l[c] = 0.f;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) o[c][i] = 0.f;
+    }
+    float4 kr[ND], vr[ND];
+    auto fetch = [&](int v0) {
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        const int f = i * 256 + threadIdx.x, r = f / D4, e = (f - r * D4) * 4, v = v0 + r;
+        kr[i] = vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r >= 32 || v >= v1) continue;
+        const long long row = key_row(p, btrow, vk.key(v));
+        if (row < 0) continue;
+        const T* a = kp + row * row_elems + e;
+        const T* b = vp + row * row_elems + e;
+        if constexpr (VEC && VW == 4) {
+          kr[i] = *reinterpret_cast<const float4*>(a);
+          vr[i] = *reinterpret_cast<const float4*>(b);
+        } else if constexpr (VEC) {
+          const uint2 x = *reinterpret_cast<const uint2*>(a), y = *reinterpret_cast<const uint2*>(b);
+          const T* h = reinterpret_cast<const T*>(&x);
+          const T* n = reinterpret_cast<const T*>(&y);
+          kr[i] = make_float4(Elem<T>::to_f(h[0]), Elem<T>::to_f(h[1]), Elem<T>::to_f(h[2]), Elem<T>::to_f(h[3]));
+          vr[i] = make_float4(Elem<T>::to_f(n[0]), Elem<T>::to_f(n[1]), Elem<T>::to_f(n[2]), Elem<T>::to_f(n[3]));
+        } else {
+          float x[4], y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[j] = e + j < p.D ? Elem<T>::to_f(a[j]) : 0.f;
+            y[j] = e + j < p.D ? Elem<T>::to_f(b[j]) : 0.f;
+          }
+          kr[i] = make_float4(x[0], x[1], x[2], x[3]);
+          vr[i] = make_float4(y[0], y[1], y[2], y[3]);
+        }
+      }
+    };
+    fetch(un.x);
+    for (int v0 = un.x; v0 < v1; v0 += 32) {
+      __syncthreads();  // the tile before is done with (and, first, the queries are in place)
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        const int f = i * 256 + threadIdx.x, r = f / D4, c = f - r * D4;
+        if (r < 32) {
+          ks[r * KP + c] = kr[i];
+          vs[r * D4 + c] = vr[i];
+        }
+      }
+      __syncthreads();
+      if (v0 + 32 < v1) fetch(v0 + 32);
+      if (!busy) continue;
+      // scores: this lane's key against the warp's four columns
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      const float4* q = qs + 4 * warp * D4;
+#pragma unroll 4
+      for (int e = 0; e < D4; ++e) {
+        const float4 k = ks[lane * KP + e];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4 x = q[c * D4 + e];
+          s[c] = fmaf(k.x, x.x, fmaf(k.y, x.y, fmaf(k.z, x.z, fmaf(k.w, x.w, s[c]))));
+        }
+      }
+      const int v = v0 + lane, key = vk.key(v);
+      bool all = true;
+      float4 w;
+      float* wp = reinterpret_cast<float*>(&w);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const bool seen = v < v1 && sees(p, g, tok[c], key);
+        all = all && seen;
+        float top = seen ? s[c] : -INFINITY;
+        const float x = top;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float mn = fmaxf(m[c], top), base = mn == -INFINITY ? 0.f : mn, al = ex2(m[c] - base);
+        m[c] = mn;
+        wp[c] = ex2(x - base);
+        l[c] = l[c] * al + wp[c];
+#pragma unroll
+        for (int i = 0; i < ND; ++i) o[c][i] *= al;
+      }
+      ps[warp * 32 + lane] = w;
+      __syncwarp();
+      const float* vf = reinterpret_cast<const float*>(vs) + lane;
+      if (__all_sync(0xffffffffu, all)) {
+#pragma unroll 4
+        for (int k = 0; k < 32; ++k) {
+          const float4 x = ps[warp * 32 + k];
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const float y = 32 * i + lane < p.D ? vf[k * D4 * 4 + 32 * i] : 0.f;
+            o[0][i] = fmaf(x.x, y, o[0][i]);
+            o[1][i] = fmaf(x.y, y, o[1][i]);
+            o[2][i] = fmaf(x.z, y, o[2][i]);
+            o[3][i] = fmaf(x.w, y, o[3][i]);
+          }
+        }
+      } else {  // keys that a column does not see are left out, whatever their value rows hold
+        for (int k = 0; k < 32; ++k) {
+          const float4 x = ps[warp * 32 + k];
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const float y = 32 * i + lane < p.D ? vf[k * D4 * 4 + 32 * i] : 0.f;
+            if (x.x != 0.f) o[0][i] = fmaf(x.x, y, o[0][i]);
+            if (x.y != 0.f) o[1][i] = fmaf(x.y, y, o[1][i]);
+            if (x.z != 0.f) o[2][i] = fmaf(x.z, y, o[2][i]);
+            if (x.w != 0.f) o[3][i] = fmaf(x.w, y, o[3][i]);
+          }
+        }
+      }
+      __syncwarp();
+    }
+    if (!busy) continue;
+    const int part = un.z & 0xffff, n_parts = un.z >> 16;
+    float* rec = n_parts > 1 ? part_base(p, g, part, kvh) : nullptr;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float sum = l[c];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const int col = w0 + c;
+      if (col >= cols) continue;
+      if (n_parts == 1) {
+        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+        T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok[c]) * p.out_stride +
+                 (long long)(kvh * p.G + col - tok[c] * p.G) * p.D;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          if (32 * i + lane < p.D) dst[32 * i + lane] = Elem<T>::from_f(o[c][i] * inv);
+      } else if (rec) {
+        float* r = rec + (long long)col * p.DP;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          if (32 * i + lane < p.D) r[32 * i + lane] = o[c][i];
+        if (lane == 0) *reinterpret_cast<float2*>(r + p.DP - 4) = make_float2(m[c], sum);
+      }
+    }
+  }
+}
+
 // Merge of split-K parts: out = sum_j 2^(m_j - M) acc_j / sum_j 2^(m_j - M)
 // l_j, always in the order of the parts.  A warp takes two rows of one
 // (group, KV head): a lane holds a float4 of one of them, so a load is whole
@@ -380,11 +584,32 @@ static int launch_vec(const MaskedParams& p, cudaStream_t st, const char* what) 
              : launch_masked(masked_vec_kernel<T, VW, LPK, EV, kVecCols>, blocks, kVecWarps * 32, st, p, what, smem);
 }
 
+template <typename T, int ND, bool VEC>
+static int launch_tile(const MaskedParams& p, cudaStream_t st, const char* what) {
+  const int D4 = (p.D + 3) / 4, smem = (32 * (D4 + 1) + 64 * D4 + 256) * 16;
+  auto kern = masked_tile_kernel<T, ND, VEC>;
+  const cudaError_t e = prepare_launch(reinterpret_cast<const void*>(kern), smem, 256, nullptr);
+  if (e != cudaSuccess) return fail(NF_ECUDA, "%s: smem attribute: %s", what, cudaGetErrorString(e));
+  long long blocks = (long long)p.max_units * p.Hkv * ((p.unit_tokens * p.G + 31) / 32);
+  const long long cap = (long long)sm_count() * 8;
+  if (blocks > cap) blocks = cap;
+  return launch_masked(kern, blocks, 256, st, p, what, smem);
+}
+
+template <typename T, bool VEC>
+static int dispatch_tile(const MaskedParams& p, cudaStream_t st, const char* what) {
+  if (p.D <= 32) return launch_tile<T, 1, VEC>(p, st, what);
+  if (p.D <= 64) return launch_tile<T, 2, VEC>(p, st, what);
+  if (p.D <= 128) return launch_tile<T, 4, VEC>(p, st, what);
+  return launch_tile<T, 8, VEC>(p, st, what);
+}
+
 template <typename T>
 static int dispatch_vec(const MaskedParams& p, cudaStream_t st, const char* what) {
   constexpr int VW = sizeof(T) == 4 ? 4 : 8;
   const bool vec = p.D % VW == 0 &&
                    ((reinterpret_cast<uintptr_t>(p.kp) | reinterpret_cast<uintptr_t>(p.vp)) & 15) == 0;
+  if (p.unit_tokens * p.G > kVecMost) return vec ? dispatch_tile<T, true>(p, st, what) : dispatch_tile<T, false>(p, st, what);
   if (!vec) return launch_vec<T, 1, 32, 8>(p, st, what);
   // eight lanes a key where registers allow (three shuffles a score, four keys at a time)
   const int n = p.D / VW;

@@ -132,6 +132,9 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
     """
     slots, q_lens, q_starts, ctx = (np.asarray(a, dtype=np.int64) for a in (slots, q_lens, q_starts, ctx))
     t_unit, t_item = max(1, unit_rows // group), item_rows // group
+    span = q_lens + (ctx if words is not None else np.minimum(ctx, window + sinks))
+    if not item_rows and int((-(-q_lens // t_unit) * span).sum()) * kv_heads < 256 * workers:
+        t_unit = max(1, 8 // group)  # few groups of few keys: smaller ones, for the kernel of few columns, fill the GPU
     routed = (q_lens > t_unit) & (t_item > 0)
     per = np.where(routed, max(1, t_item), t_unit)
     n_groups = -(-q_lens // per)
