@@ -13,6 +13,13 @@
 // whatever the number of drafted tokens.  (tcgen05 needs 64 rows or more; a
 // group has at most 32, larger ones go to nf_masked_tc.cu.)
 //
+// 64 decodes with a window of 4,096 and 64 sinks, 8 KV heads of 128 (1.09 GB):
+// 167-170 us with the merge, the copy bandwidth.  64 with a window of 1,024, 8
+// KV heads of 64 (130 MB): 29 us, of which 20 are the bytes and the rest is
+// the ramp of 148 CTAs and the merge's launch.  37 trees of 7 tokens (28 columns)
+// on 4,096 keys: 82 us with two warps a head on alternate steps, 97 and 115
+// with one warp (its registers hold four column tiles then).
+//
 // Only steps that some column does not wholly see apply the mask.  There the
 // weights of unseen keys are 0; as 0 * NaN would still reach the sum, such a
 // step looks its value rows over and, where they hold anything not finite,
@@ -41,7 +48,7 @@ struct __align__(16) MtStep {
 constexpr int kMtFirst = 1, kMtLast = 2, kMtMasked = 4;
 
 struct MtLaunch {
-  int HG, n_hg, stages, stage_bytes, box_bytes, one_box, evict_first, q_align4;
+  int HG, n_hg, stages, stage_bytes, box_bytes, one_box, q_align4;
 };
 
 // Byte offset of key row r, 16-byte chunk c, in one head's staged tile.
@@ -80,7 +87,7 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
   // the switch to another task needs four dependent round trips (ticket, share,
   // record, block id): each is asked for kGap steps after the one before
   constexpr int kGap = 2, kAhead = 4 * kGap;
-  const uint64_t pol = L.evict_first ? l2_evict_first() : l2_evict_last();
+  const uint64_t pol = l2_evict_first();  // a share's keys are read by one CTA
   int k = 0, s = 0;
   uint32_t pe = 1;
   bool ok = true;
@@ -614,7 +621,6 @@ int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char
   if (!L.one_box && !(encode_pool_map(&tk, p.kp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, hg, false) &&
                       encode_pool_map(&tv, p.vp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, hg, false)))
     return NF_EUNSUPPORTED;
-  L.evict_first = 1;
   L.q_align4 = (reinterpret_cast<uintptr_t>(p.q) % 4 == 0) && p.q_stride % 2 == 0;
   const MtKernel kern = dtype == NF_BF16 ? mt_kernel<__nv_bfloat16>(p.D, cols) : mt_kernel<__half>(p.D, cols);
   const int threads = (hg * cw + 1) * 32, smem = kMtHeader + L.stages * L.stage_bytes + 1024;

@@ -245,6 +245,7 @@ class MaskedPlan:
         self.args_ptr = 0
         self.fn = None
         self.owner = None
+        self.generation = 0  # of the cache's pools
         self.streams = set()  # streams that the buffers are known to
         self.ready = None
         self.upload_bytes = 0
@@ -338,7 +339,7 @@ class MaskedAttentionOps:
         else:
             view = into
             if (view.kind, view.window, view.sinks, view.q_heads) != (kind, window, sinks, q_heads) \
-                    or view.owner is not self:
+                    or view.owner is not self or view.generation != self._generation:
                 raise ValueError("into is the plan of another cache, window or set of heads")
             if any(n > r for n, r in zip(sizes, view.room)):
                 raise ValueError(f"the step's lists {sizes} do not fit the plan's room {view.room}")
@@ -366,7 +367,7 @@ class MaskedAttentionOps:
         view.args_ptr = ctypes.addressof(view.args)
         lib = _lib.load()
         view.fn = lib.nf_tree_attention if kind == "tree" else lib.nf_window_attention
-        view.owner = self
+        view.owner, view.generation = self, self._generation
         view.ready = torch.cuda.Event()
         view.ready.record(torch.cuda.current_stream(self.device))
         view.streams = {self._stream()}
@@ -402,7 +403,7 @@ class MaskedAttentionOps:
             raise ValueError("q and out must be on the same device")
         if view.owner is not self:
             raise ValueError("the plan belongs to another cache")
-        if view.args.block_tables != self._bt_ptr:
+        if view.generation != self._generation:
             raise ValueError("the plan was made before the cache's last init_batch")
         width = view.q_heads * self.head_dim
         shape = q.shape

@@ -170,6 +170,7 @@ class PagedKVCache(MaskedAttentionOps, PageOps):
         self.prefix_cache: PrefixCache | None = None
         self._plan: StepPlan | None = None
         self.steps_closed = 0  # forward passes whose last layer has appended
+        self._generation = 0  # of the pools: plans of windows and trees are for one
         # KV heads sharded over several GPUs: a sharding.PeerExchange whose gathered buffers receive every
         # rank's attention output (Attention.forward then returns the gathered rows); None on one GPU
         self.exchange = None
@@ -180,6 +181,7 @@ class PagedKVCache(MaskedAttentionOps, PageOps):
         if self.device.type != "cuda":
             raise _lib.NifreError("PagedKVCache needs a CUDA device: nifre_b200 has no CPU path")
         self.batch_size = batch_size
+        self._generation += 1
         self.pos = torch.zeros(batch_size, dtype=torch.long, device=self.device)
         self.pos_host = np.zeros(batch_size, dtype=np.int64)
         self.max_blocks_per_seq = (self.max_seq_len + self.block_size - 1) // self.block_size
@@ -231,7 +233,7 @@ class PagedKVCache(MaskedAttentionOps, PageOps):
         self.prefix_cache = None
         self._plan = None
         self._k_all = self._v_all = None
-        self._bt_ptr = None  # plans made before are not of the next batch
+        self._generation += 1  # plans made before are not of the next batch
 
     # ------------------------------------------------------------------ reference API
     def try_load_prefix(self, batch_idx: int, token_ids: list[int]) -> int:

@@ -326,6 +326,18 @@ def test_plans_of_other_caches_and_kinds_are_refused():
         a.cache.window_attention_step(0, a.q[0], w, out)
 
 
+def test_plans_of_an_earlier_batch_are_refused():
+    st = Step([10], [2], 4, 2, 64, 16, HF, seed=3)
+    view = st.cache.plan_window(st.plan, 4, q_heads=4)
+    out = torch.empty_like(st.q[0])
+    st.cache.window_attention_step(0, st.q[0], view, out)
+    st.cache.init_batch(1)  # the pools may come back at the same addresses
+    with pytest.raises(ValueError, match="init_batch"):
+        st.cache.window_attention_step(0, st.q[0], view, out)
+    with pytest.raises(ValueError, match="into"):
+        st.cache.plan_window(st.cache.plan([0], [2], [0]), 4, q_heads=4, into=view)
+
+
 def test_bad_records_are_flagged_not_followed():
     """Work lists and block tables with values out of range: skipped and flagged by the kernels' own checks."""
     from nifre_b200 import _lib
