@@ -69,7 +69,7 @@ struct TcCfg {
 };
 
 constexpr int kTcItemRing = 4;
-constexpr uint32_t kTcTmemPtr = 512, kTcPoison = 520, kTcSlots = 576, kTcStats = 1024;
+constexpr uint32_t kTcTmemPtr = 512, kTcPoison = 528, kTcSlots = 576, kTcStats = 1024;
 
 struct TcBars {
   uint32_t hdr;
@@ -90,28 +90,33 @@ struct TcBars {
   __device__ uint32_t join_empty() const { return hdr + 456; }  // half 0 has read them
 };
 
-// One work item as every role sees it.
-struct TcItem {
-  MaskedGroup g;
-  VirtualKeys vk;
-  int kvh, k0, k1, part, nkt, n_half;
+// One work item as every role sees it: the producer derives it once, the
+// others read the fields they need from its slot in shared memory.
+struct __align__(16) TcItem {
+  int kvh, k0, k1, part;  // KV head (-1: no more items), virtual keys [k0, k1), part | n_parts << 16
+  int nkt, n_half;
   int whole0, whole1;  // tiles that every row sees wholly: [whole0, whole1)
-  bool bad, dup;
-  __device__ TcItem(const MaskedParams& p, int item, int4 un, const MaskedGroup& gr, int TT)
-      : g(gr), vk(p, gr) {
-    kvh = item;
+  MaskedGroup g;
+  int kept, gap, dup, bad;  // (kept, gap: VirtualKeys)
+  TcItem() = default;
+  __device__ TcItem(const MaskedParams& p, int head, int4 un, const MaskedGroup& gr, int TT) : g(gr) {
+    const VirtualKeys vk(p, gr);
+    kvh = head;
     k0 = un.x;
     k1 = min(un.y, vk.end);
     part = un.z;
-    bad = !group_ok(p, g) || k0 < 0 || (k0 & 15) || k0 >= k1 || g.ntok > 2 * TT;
+    kept = vk.kept;
+    gap = vk.gap;
+    bad = head < 0 || !group_ok(p, g) || k0 < 0 || (k0 & 15) || k0 >= k1 || g.ntok > 2 * TT;
     nkt = bad ? 0 : (k1 - k0 + 127) >> 7;
     n_half = g.ntok > TT ? 2 : 1;
     dup = n_half == 1 && nkt > 1;
-    const int v_lo = p.tree ? 0 : max(vk.kept, g.pos0 + g.ntok - p.window - vk.gap);
-    const int v_hi = min(k1, p.tree ? g.ctx : g.pos0 + 1 - vk.gap);
+    const int v_lo = p.tree ? 0 : max(kept, g.pos0 + g.ntok - p.window - gap);
+    const int v_hi = min(k1, p.tree ? g.ctx : g.pos0 + 1 - gap);
     whole0 = max(v_lo - k0 + 127, 0) >> 7;
     whole1 = max(v_hi - k0, 0) >> 7;
   }
+  __device__ __forceinline__ int key(int v) const { return v < kept ? v : v + gap; }
   __device__ __forceinline__ bool active(int h, int j) const {
     return j >= 0 && j < nkt && (dup ? (j & 1) == h : h < n_half);
   }
@@ -122,6 +127,7 @@ struct TcItem {
   // whether some row of the group may not see the whole of tile j
   __device__ __forceinline__ bool masked(int j) const { return j < whole0 || j >= whole1; }
 };
+static_assert(sizeof(TcItem) == 80 && kTcSlots + kTcItemRing * sizeof(TcItem) <= kTcStats, "item slots");
 
 // Bits [lo, hi) of word w of a 128-bit row.
 __device__ __forceinline__ uint32_t run_bits(int lo, int hi, int w) {
@@ -155,8 +161,8 @@ __device__ __forceinline__ void row_bits(const MaskedParams& p, const TcItem& w,
     return;
   }
   const int pos = w.g.pos0 + t;
-  const int a = (w.vk.gap ? p.sinks : min(p.sinks, pos + 1)) - v0;
-  const int b = max(pos - p.window + 1, 0) - w.vk.gap - v0, c = min(pos - w.vk.gap - v0 + 1, lim);
+  const int a = (w.gap ? p.sinks : min(p.sinks, pos + 1)) - v0;
+  const int b = max(pos - p.window + 1, 0) - w.gap - v0, c = min(pos - w.gap - v0 + 1, lim);
 #pragma unroll
   for (int q = 0; q < 4; ++q) bits[q] = run_bits(0, min(a, lim), q) | run_bits(max(b, 0), c, q);
 }
@@ -168,25 +174,18 @@ __device__ __noinline__ bool seen_by_any(const MaskedParams& p, const MaskedGrou
   return false;
 }
 
-// The ring that hands items to the CTA's warps; a slot holds the KV head
-// (-1: no more) and the unit's record.
+// The ring that hands items to the CTA's warps.
 struct TcRing {
   const TcBars& bar;
-  unsigned char* slots;
+  TcItem* slots;
   Ring r;
-  __device__ TcRing(const TcBars& b, unsigned char* base) : bar(b), slots(base + kTcSlots) {}
-  __device__ int4* slot(int st) const { return reinterpret_cast<int4*>(slots + 64 * st); }
+  __device__ TcRing(const TcBars& b, unsigned char* base) : bar(b), slots(reinterpret_cast<TcItem*>(base + kTcSlots)) {}
   // the item in slot st (until release)
-  __device__ TcItem item(const MaskedParams& p, int st, int TT) const {
-    const int4* sl = slot(st);
-    const int4 a = sl[0], b = sl[1], c = sl[2], d = sl[3];
-    return TcItem(p, a.x, b, MaskedGroup{c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w}, TT);
-  }
-  __device__ int kv_head(int st) const { return slot(st)->x; }
+  __device__ const TcItem& item(int st) const { return slots[st]; }
   // waits for the next item: its slot (-1 at the end, or when the wait ran out)
   __device__ int next(int* status) {
     if (!mbar_wait(bar.item_full(r.st), r.ph, status)) return -1;
-    return kv_head(r.st) < 0 ? -1 : r.st;
+    return slots[r.st].kvh < 0 ? -1 : r.st;
   }
   __device__ void release() {
     __syncwarp();
@@ -201,8 +200,8 @@ struct TcClaim {
   int task = -1, u = 0;
   int2 sh = make_int2(0, 0);
 };
-__device__ __forceinline__ bool tc_claim(const MaskedParams& p, TcRing& ring, int tasks, TcClaim& cl, int& item,
-                                         int4& un, MaskedGroup& g) {
+__device__ __forceinline__ bool tc_claim(const MaskedParams& p, TcRing& ring, int tasks, TcClaim& cl, int TT,
+                                         TcItem& w) {
   const int lane = threadIdx.x & 31;
   while (++cl.u >= cl.sh.y && cl.task < tasks) {
     int pos = blockIdx.x;  // the first task is the CTA's own, the queue hands out the rest
@@ -215,29 +214,26 @@ __device__ __forceinline__ bool tc_claim(const MaskedParams& p, TcRing& ring, in
     cl.sh = load_share(p.item_shares, pos / p.Hkv, p.max_items);
     cl.u = cl.sh.x - 1;
   }
-  item = cl.task < tasks ? cl.task % p.Hkv : -1;  // (the KV head)
-  un = make_int4(0, 0, 0, 0);
-  g = MaskedGroup{};
-  if (item >= 0) un = load_record(p.items, cl.u, g);
+  const int head = cl.task < tasks ? cl.task % p.Hkv : -1;
+  int4 un = make_int4(0, 0, 0, 0);
+  MaskedGroup g{};
+  if (head >= 0) un = load_record(p.items, cl.u, g);
+  w = TcItem(p, head, un, g, TT);
   if (!mbar_wait(ring.bar.item_empty(ring.r.st), ring.r.ph ^ 1, p.status)) return false;
   if (lane == 0) {
-    int4* sl = ring.slot(ring.r.st);
-    sl[0] = make_int4(item, 0, 0, 0);
-    sl[1] = un;
-    sl[2] = make_int4(g.slot, g.q_row0, g.ntok, g.pos0);
-    sl[3] = make_int4(g.ctx, g.n_draft, g.mask0, g.part_row0);
+    ring.slots[ring.r.st] = w;
     mbar_arrive(ring.bar.item_full(ring.r.st));
   }
   __syncwarp();
   ring.r.next(kTcItemRing);
-  return item >= 0;
+  return head >= 0;
 }
 
 // Block id of 16-key block `lane` (< 8) of tile j and its first key; -1: none there.
 __device__ __forceinline__ int tc_block(const MaskedParams& p, const TcItem& w, const int* btrow, int j, int lane,
                                         int& key) {
   const int v = w.k0 + (j * 8 + lane) * 16;
-  key = w.vk.key(v);
+  key = w.key(v);
   const int lb = key / p.bs;
   if (lane >= 8 || v >= w.k1) return 0;
   return lb < p.max_blocks ? __ldg(btrow + lb) : -1;
@@ -301,13 +297,10 @@ __device__ void tc_producer(const MaskedParams& p, int TT, bool q_tma, const CUt
   const int lane = threadIdx.x & 31;
   const uint64_t pol = l2_evict_last(), pol_q = l2_evict_first();
   Ring qr, kr, vr;
-  int it;
   TcClaim claim;
-  int4 un;
-  MaskedGroup g;
+  TcItem w;
   pdl_wait();  // queries, keys and values may come from the launch before this one
-  while (tc_claim(p, ring, tasks, claim, it, un, g)) {
-    const TcItem w(p, it, un, g, TT);
+  while (tc_claim(p, ring, tasks, claim, TT, w)) {
     if (w.bad) {
       if (lane == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
       continue;
@@ -392,7 +385,7 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
     __syncwarp();
   };
   for (int slot; (slot = ring.next(p.status)) >= 0;) {
-    const TcItem w = ring.item(p, slot, TT);
+    const TcItem w = ring.item(slot);
     ring.release();
     if (w.bad) continue;
     // P V runs `lag` tiles behind S: one, or two where the halves take tiles in turn (a half's next S is then issued
@@ -526,9 +519,10 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
   const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
   const uint32_t s_addr = tmem + lane_addr + C::s_col(h), o_addr = tmem + lane_addr + C::o_col(h);
   const uint32_t p_addr = tmem + lane_addr + C::p_col(h);
-  volatile int* poison = reinterpret_cast<volatile int*>(base + kTcPoison);  // [2]: the last poisoned item of each parity
+  volatile int* poison = reinterpret_cast<volatile int*>(base + kTcPoison);  // [8]: item numbers, by their low bits
   float2* stats = reinterpret_cast<float2*>(base + kTcStats);  // half 1's (m, l) of a joined item
   int n_s = 0, n_o = 0, n_join = 0;
+  const int tok0 = row / p.G, hd = row - tok0 * p.G;  // token of the half and query head of this row
   // a scale of 0 or less cannot follow the maximum and the mask: the scores are scaled before them then
   const float scale = p.scale_log2 > 0.f ? p.scale_log2 : 1.f;
   bool join_pending = false;  // half 1: its accumulator is still to be read by half 0
@@ -542,7 +536,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
     bool dup, keep;  // keep: this half looks the values of masked tiles over (where the halves share them)
     bool valid;
     {
-      const TcItem w = ring.item(p, slot, TT);
+      const TcItem& w = ring.item(slot);
       if (w.bad) continue;
       ++seq;
       v0r = vr;
@@ -553,7 +547,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
       whole1 = w.whole1;
       dup = w.dup;
       keep = w.dup || h == w.n_half - 1;
-      valid = row < TT * p.G && (dup ? 0 : h * TT) + row / p.G < w.g.ntok;
+      valid = tok0 < TT && (dup ? 0 : h * TT) + tok0 < w.g.ntok;
     }
     float m = 0.f, l = 0.f;  // the reference of the exponents, and the sum of the weights
     bool none = true;        // the row has seen no key yet
@@ -585,8 +579,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
         if (masked) {
           uint32_t bits[4] = {0u, 0u, 0u, 0u};
           if (valid) {
-            const TcItem w = ring.item(p, slot, TT);
-            row_bits(p, w, (dup ? 0 : h * TT) + row / p.G, j, bits);
+            row_bits(p, ring.item(slot), (dup ? 0 : h * TT) + tok0, j, bits);
           }
 #pragma unroll
           for (int i = 0; i < 128; ++i)
@@ -656,7 +649,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
       for (int a = 0; a < 4; ++a) f2_unpack(sum2[a], sa[2 * a], sa[2 * a + 1]);
       l = l * alpha + (((sa[0] + sa[1]) + (sa[2] + sa[3])) + ((sa[4] + sa[5]) + (sa[6] + sa[7])));
       if (masked && keep) {
-        const TcItem w = ring.item(p, slot, TT);
+        const TcItem& w = ring.item(slot);
         // this thread's value row of the tile: zeroed when past the unit's keys or not finite
         const Ring vt = v0r.ahead(j, C::VST);
         if (!mbar_wait(bar.v_full(vt.st), vt.ph, p.status)) return;
@@ -675,7 +668,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
 #pragma unroll
               for (int q = 0; q < 4; ++q) odd |= (e[q] & EX) == EX || ((e[q] >> 16) & EX) == EX;
             }
-          if (odd && seen_by_any(p, w.g, w.vk.key(v))) poison[seq & 1] = seq;
+          if (odd && seen_by_any(p, w.g, w.key(v))) poison[seq & 7] = seq;
         }
         if (odd) {
 #pragma unroll
@@ -695,8 +688,8 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
     ++n_o;
     tc_fence_after();
     if (none) m = -INFINITY;
-    const TcItem w = ring.item(p, slot, TT);
-    const int tok = (w.dup ? 0 : h * TT) + row / p.G, hd = row % p.G;
+    const TcItem& w = ring.item(slot);
+    const int tok = (dup ? 0 : h * TT) + tok0;
     float a0 = 1.f, a1 = 0.f;  // weights of this half's and half 1's accumulators
     if (w.dup) {
       ++n_join;
@@ -805,7 +798,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
       __syncwarp();
       if (lane == 0) mbar_arrive(bar.join_empty());
     }
-    if (poison[seq & 1] == seq && valid)
+    if (poison[seq & 7] == seq && valid)
       tc_row_again<T, D_>(p, w.g, w.k0, w.k1, w.part, w.kvh, tok, hd);
   }
 }
@@ -852,8 +845,7 @@ __global__ void __launch_bounds__(TcCfg<D_>::THREADS, 1)
     mbar_init(bar.join_full(), 4);
     mbar_init(bar.join_empty(), 4);
     fence_mbar_init();
-    reinterpret_cast<int*>(base + kTcPoison)[0] = 0;
-    reinterpret_cast<int*>(base + kTcPoison)[1] = 0;
+    for (int i = 0; i < 8; ++i) reinterpret_cast<int*>(base + kTcPoison)[i] = 0;
   }
   if (warp == 1) tmem_alloc(hdr + kTcTmemPtr, C::TMEM_COLS);
   tc_fence_before();
