@@ -12,7 +12,8 @@
 //     16-token box per block and 64-element part of a head) into rings;
 //   MMA warp: S_h = Q_h K^T (M = N = 128) into tensor memory, then
 //     O_h += P_h V with P_h from tensor memory;
-//   two softmax warpgroups (thread = row), one per half.
+//   two softmax warpgroups (thread = row), one per half;
+//   two value warps: the value rows of tiles under the mask (below).
 //
 // An item of one half and several tiles (a draft of up to 128 rows) would
 // leave the second warpgroup idle and be bound by the first one's
@@ -22,8 +23,8 @@
 // The mask is applied only on tiles that some row does not wholly see: each
 // row's 128 truth values are built as four words (two runs for a window, the
 // shifted mask words for a tree).  Unseen keys get weight 0; as 0 * NaN would
-// still reach the sum, a masked tile's value rows are looked over by one
-// thread each: rows that are not finite are zeroed, and where some row of the
+// still reach the sum, the value warps look over a masked tile's value rows
+// before P V reads them: rows that are not finite are zeroed, and where some row of the
 // item does see one of them, the item's rows are computed again one by one
 // (slow, and right: such values are rare and wrong already).
 //
@@ -58,7 +59,7 @@ struct TcCfg {
   static constexpr uint32_t K_OFF = Q_OFF + QST * 2 * TILE;
   static constexpr uint32_t V_OFF = K_OFF + KST * TILE;
   static constexpr uint32_t SMEM = 1024 + V_OFF + VST * TILE;  // + alignment slack
-  static constexpr int THREADS = 384;  // warp 0 producer, 1 MMA, 4-7 half 0, 8-11 half 1
+  static constexpr int THREADS = 384;  // warp 0 producer, 1 MMA, 2-3 values, 4-7 half 0, 8-11 half 1
   // setmaxnreg split of the launch's 384 x 168 registers
   static constexpr int REGS_CTRL = 72, REGS_SOFTMAX = 216;
   static_assert(REGS_CTRL * 128 + REGS_SOFTMAX * 256 <= 168 * THREADS, "register split exceeds the launch");
@@ -86,6 +87,7 @@ struct TcBars {
   __device__ uint32_t q_empty(int s) const { return hdr + 336 + 8 * s; }
   __device__ uint32_t item_full(int s) const { return hdr + 384 + 8 * s; }
   __device__ uint32_t item_empty(int s) const { return hdr + 416 + 8 * s; }
+  __device__ uint32_t v_clean(int s) const { return hdr + 464 + 8 * s; }  // (to 504) a masked tile's values are looked over
   __device__ uint32_t join_full() const { return hdr + 448; }   // half 1's accumulator and statistics are in place
   __device__ uint32_t join_empty() const { return hdr + 456; }  // half 0 has read them
 };
@@ -349,6 +351,7 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
   const uint32_t idesc_o = umma_idesc_f16(bf, 128, D_, false, true);
   Ring qr, kr, vr;
   int n_s[2] = {0, 0}, n_p[2] = {0, 0};
+  uint32_t clean = 0;  // parity of each V stage's next masked tile
   auto wait_p = [&](int h) -> bool {
     if (!mbar_wait(bar.p_full(h), n_p[h] & 1, p.status)) return false;
     ++n_p[h];
@@ -392,19 +395,18 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
     // while the other half's weights are still to come)
     const int lag = w.dup ? 2 : 1;
     int v1 = -1, v2 = -1;  // V stages of the last tile loaded and the one before
+    auto values = [&](int j, int vst) -> bool {  // tile j's values may be used
+      if (!w.masked(j)) return true;
+      if (!mbar_wait(bar.v_clean(vst), clean >> vst & 1u, p.status)) return false;
+      clean ^= 1u << vst;
+      return true;
+    };
     auto pv = [&](int j, int vst) -> bool {  // P V of tile j from V stage vst
-      bool waited = false;
-      if (w.masked(j)) {
-        // both halves' weights of a masked tile must be in before either P V: the keeper half may zero value rows
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if (w.active(h, j) && !wait_p(h)) return false;
-        waited = true;
-      }
+      if (!values(j, vst)) return false;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (!w.active(h, j)) continue;
-        if (!waited && !wait_p(h)) return false;
+        if (!wait_p(h)) return false;
         issue_pv(h, vst, j < lag);  // (a half's first tile overwrites O_h)
       }
       return true;
@@ -420,17 +422,12 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
           tc_fence_after();
           issue_s(j & 1, 0, kr.st);
         } else {
-          bool waited = false;
-          if (jp >= 0 && w.masked(jp)) {
-            for (int h = 0; h < w.n_half; ++h)
-              if (!wait_p(h)) return;
-            waited = true;
-          }
+          if (jp >= 0 && !values(jp, vst)) return;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (h >= w.n_half) continue;
             if (jp >= 0) {
-              if (!waited && !wait_p(h)) return;
+              if (!wait_p(h)) return;
               issue_pv(h, vst, jp == 0);
             }
             tc_fence_after();
@@ -508,12 +505,64 @@ __device__ __noinline__ void tc_row_again(const MaskedParams& p, const MaskedGro
   }
 }
 
+// The value warps: the rows of masked tiles, two a thread, zeroed when they
+// are past the unit's keys or not finite; an item some row of which sees such
+// a row is poisoned.
+template <typename T, int D_>
+__device__ void tc_values(const MaskedParams& p, const TcBars& bar, unsigned char* base, uint32_t v_s, TcRing& ring) {
+  using C = TcCfg<D_>;
+  constexpr uint32_t REG = 128 * 128;
+  constexpr uint32_t EX = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  const int lane = threadIdx.x & 31;
+  volatile int* poison = reinterpret_cast<volatile int*>(base + kTcPoison);
+  Ring vr;
+  int seq = 0;
+  for (int slot; (slot = ring.next(p.status)) >= 0; ring.release()) {
+    const TcItem& w = ring.item(slot);
+    if (w.bad) continue;
+    ++seq;
+    const int nkt = w.nkt;
+    for (int j = 0; j < nkt; ++j, vr.next(C::VST)) {
+      // (every tile is waited for and given back, so that these warps are never a whole turn of the ring away)
+      if (!mbar_wait(bar.v_full(vr.st), vr.ph, p.status)) return;
+      const bool masked = w.masked(j);
+#pragma unroll 1
+      for (int row = masked ? threadIdx.x & 63 : 128; row < 128; row += 64) {
+        const uint32_t vs = v_s + vr.st * C::TILE + row * 128;
+        const int v = w.k0 + 128 * j + row;
+        bool odd = v >= w.k1;
+        if (!odd) {
+#pragma unroll
+          for (int c = 0; c < D_ / 8; ++c) {
+            uint32_t e[4];
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3])
+                         : "r"(vs + (c >> 3) * REG + (((c & 7) ^ (row & 7)) << 4)));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) odd |= (e[q] & EX) == EX || ((e[q] >> 16) & EX) == EX;
+          }
+          if (odd && seen_by_any(p, w.g, w.key(v))) poison[seq & 7] = seq;
+        }
+        if (odd) {
+#pragma unroll
+          for (int c = 0; c < D_ / 8; ++c)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (c >> 3) * REG + ((c & 7) << 4)), "r"(0)
+                         : "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+        if (masked) mbar_arrive(bar.v_clean(vr.st));
+        mbar_arrive(bar.v_empty(vr.st));
+      }
+    }
+  }
+}
+
 template <typename T, int D_>
 __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBars& bar, unsigned char* base,
-                           uint32_t tmem, uint32_t v_s, int h, TcRing& ring) {
+                           uint32_t tmem, int h, TcRing& ring) {
   using C = TcCfg<D_>;
-  constexpr int NDH = D_ / 64;
-  constexpr uint32_t REG = 128 * 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quad = warp & 3, row = quad * 32 + lane;  // tensor-memory lanes of this warp: quad*32..
   const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
@@ -526,27 +575,21 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
   // a scale of 0 or less cannot follow the maximum and the mask: the scores are scaled before them then
   const float scale = p.scale_log2 > 0.f ? p.scale_log2 : 1.f;
   bool join_pending = false;  // half 1: its accumulator is still to be read by half 0
-  Ring vr;
   int seq = 0;
   // The item itself stays in its slot of shared memory while the tiles run (its fields would cost the tile loop the
   // registers of the scores); what masked tiles and the epilogue need is read there again.
   for (int slot; (slot = ring.next(p.status)) >= 0; ring.release()) {
-    Ring v0r;  // V stage of the item's first tile
     int nkt, whole0, whole1;
-    bool dup, keep;  // keep: this half looks the values of masked tiles over (where the halves share them)
-    bool valid;
+    bool dup, valid;
     {
       const TcItem& w = ring.item(slot);
       if (w.bad) continue;
       ++seq;
-      v0r = vr;
-      vr = vr.ahead(w.nkt, C::VST);
       if (w.tiles(h) == 0) continue;
       nkt = w.nkt;
       whole0 = w.whole0;
       whole1 = w.whole1;
       dup = w.dup;
-      keep = w.dup || h == w.n_half - 1;
       valid = tok0 < TT && (dup ? 0 : h * TT) + tok0 < w.g.ntok;
     }
     float m = 0.f, l = 0.f;  // the reference of the exponents, and the sum of the weights
@@ -648,37 +691,6 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
 #pragma unroll
       for (int a = 0; a < 4; ++a) f2_unpack(sum2[a], sa[2 * a], sa[2 * a + 1]);
       l = l * alpha + (((sa[0] + sa[1]) + (sa[2] + sa[3])) + ((sa[4] + sa[5]) + (sa[6] + sa[7])));
-      if (masked && keep) {
-        const TcItem& w = ring.item(slot);
-        // this thread's value row of the tile: zeroed when past the unit's keys or not finite
-        const Ring vt = v0r.ahead(j, C::VST);
-        if (!mbar_wait(bar.v_full(vt.st), vt.ph, p.status)) return;
-        const uint32_t vs = v_s + vt.st * C::TILE + row * 128;
-        const int v = w.k0 + 128 * j + row;
-        bool odd = v >= w.k1;
-        if (!odd) {
-          constexpr uint32_t EX = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-#pragma unroll
-          for (int dh = 0; dh < NDH; ++dh)
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              uint32_t e[4];
-              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3])
-                           : "r"(vs + dh * REG + ((c ^ (row & 7)) << 4)));
-#pragma unroll
-              for (int q = 0; q < 4; ++q) odd |= (e[q] & EX) == EX || ((e[q] >> 16) & EX) == EX;
-            }
-          if (odd && seen_by_any(p, w.g, w.key(v))) poison[seq & 7] = seq;
-        }
-        if (odd) {
-#pragma unroll
-          for (int dh = 0; dh < NDH; ++dh)
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + dh * REG + c * 16), "r"(0) : "memory");
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-      }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -826,7 +838,8 @@ __global__ void __launch_bounds__(TcCfg<D_>::THREADS, 1)
     }
     for (int s = 0; s < C::VST; ++s) {
       mbar_init(bar.v_full(s), 1);
-      mbar_init(bar.v_empty(s), 1);
+      mbar_init(bar.v_empty(s), 1 + 2);  // P V's commit and the value warps
+      mbar_init(bar.v_clean(s), 2);
     }
     for (int h = 0; h < 2; ++h) {
       mbar_init(bar.s_full(h), 1);
@@ -840,7 +853,7 @@ __global__ void __launch_bounds__(TcCfg<D_>::THREADS, 1)
     }
     for (int s = 0; s < kTcItemRing; ++s) {
       mbar_init(bar.item_full(s), 1);
-      mbar_init(bar.item_empty(s), 1 + 4 * 2);  // the MMA warp and the softmax warps
+      mbar_init(bar.item_empty(s), 1 + 2 + 4 * 2);  // the MMA, value and softmax warps
     }
     mbar_init(bar.join_full(), 4);
     mbar_init(bar.join_empty(), 4);
@@ -861,9 +874,11 @@ __global__ void __launch_bounds__(TcCfg<D_>::THREADS, 1)
       tc_producer<T, D_>(p, TT, q_tma, &tq, &tk, &tv, bar, q_s, k_s, v_s, tasks, ring);
     else if (warp == 1)
       tc_mma<D_>(p, TT, bar, tmem, q_s, k_s, v_s, std::is_same<T, __nv_bfloat16>::value, ring);
+    else
+      tc_values<T, D_>(p, bar, base, v_s, ring);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
-    tc_softmax<T, D_>(p, TT, out16, bar, base, tmem, v_s, (warp - 4) >> 2, ring);
+    tc_softmax<T, D_>(p, TT, out16, bar, base, tmem, (warp - 4) >> 2, ring);
   }
   tc_fence_before();
   __syncthreads();
