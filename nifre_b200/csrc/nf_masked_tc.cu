@@ -54,6 +54,7 @@ struct TcCfg {
   static constexpr int QST = D_ == 64 ? 2 : 1;    // Q ring (an item's halves per stage)
   static constexpr int KST = D_ == 64 ? 4 : 2;
   static constexpr int VST = D_ == 64 ? 5 : 3;    // (held one tile longer than K)
+  static constexpr int V_BLOCK = 16 * D_ * 2;     // 16 keys of a V tile: 128-byte rows, [d / 64][key]
   static constexpr bool P_ALIAS = D_ == 128;      // P_h over the first 64 columns of S_h (no room left)
   static constexpr uint32_t Q_OFF = 2048;         // after the header
   static constexpr uint32_t K_OFF = Q_OFF + QST * 2 * TILE;
@@ -241,8 +242,11 @@ __device__ __forceinline__ int tc_block(const MaskedParams& p, const TcItem& w, 
   return lb < p.max_blocks ? __ldg(btrow + lb) : -1;
 }
 
-// Copies of one 128-key K or V tile, lane b < nb the 16-key block b.
-template <int D_>
+// Copies of one 128-key K or V tile, lane b < nb the 16-key block b.  A block
+// of a 128-wide head is two boxes of 64 elements a K tile, whose rows are
+// evenly spaced for S, and one box of both a V tile, where a block is one k-step
+// of P V (fewer copies: 2 KB a copy is what the copies' rate suffers from).
+template <int D_, bool V>
 __device__ __forceinline__ void tc_load(const MaskedParams& p, const CUtensorMap* tm, uint32_t dst0, uint32_t full,
                                         int phys, int key, int nb, int kvh, uint64_t pol, int lane) {
   constexpr int NDH = D_ / 64;
@@ -254,13 +258,14 @@ __device__ __forceinline__ void tc_load(const MaskedParams& p, const CUtensorMap
       atomicOr(p.status, NF_STATUS_BAD_BLOCK);
       phys = 0;
     }
+    if constexpr (D_ == 64) {
+      tma_load_4d(dst0 + lane * 2048, tm, 0, kvh, off, phys, full, pol);
+    } else if constexpr (V) {
+      tma_load_5d(dst0 + lane * 4096, tm, 0, off, 0, kvh, phys, full, pol);
+    } else {
 #pragma unroll
-    for (int dh = 0; dh < NDH; ++dh) {
-      const uint32_t dst = dst0 + dh * 128 * 128 + lane * 2048;
-      if constexpr (D_ == 64)
-        tma_load_4d(dst, tm, 0, kvh, off, phys, full, pol);
-      else
-        tma_load_5d(dst, tm, 0, dh, kvh, off, phys, full, pol);
+      for (int dh = 0; dh < NDH; ++dh)
+        tma_load_5d(dst0 + dh * 128 * 128 + lane * 2048, tm, 0, dh, kvh, off, phys, full, pol);
     }
   }
 }
@@ -331,10 +336,10 @@ __device__ void tc_producer(const MaskedParams& p, int TT, bool q_tma, const CUt
     for (int j = 0; j < w.nkt; ++j) {
       const int nb = min(8, (w.k1 - w.k0 - j * 128 + 15) >> 4);
       if (!mbar_wait(bar.k_empty(kr.st), kr.ph ^ 1, p.status)) return;
-      tc_load<D_>(p, tk, k_s + kr.st * C::TILE, bar.k_full(kr.st), cur, key, nb, w.kvh, pol, lane);
+      tc_load<D_, false>(p, tk, k_s + kr.st * C::TILE, bar.k_full(kr.st), cur, key, nb, w.kvh, pol, lane);
       kr.next(C::KST);
       if (!mbar_wait(bar.v_empty(vr.st), vr.ph ^ 1, p.status)) return;
-      tc_load<D_>(p, tv, v_s + vr.st * C::TILE, bar.v_full(vr.st), cur, key, nb, w.kvh, pol, lane);
+      tc_load<D_, true>(p, tv, v_s + vr.st * C::TILE, bar.v_full(vr.st), cur, key, nb, w.kvh, pol, lane);
       vr.next(C::VST);
       if (j + 1 < w.nkt) cur = tc_block(p, w, btrow, j + 1, lane, key);
     }
@@ -361,7 +366,7 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
   tmem = __shfl_sync(0xffffffffu, tmem, 0);
   const uint64_t dq = umma_sdesc_sw128(__shfl_sync(0xffffffffu, q_s, 0), 16, 1024);
   const uint64_t dk = umma_sdesc_sw128(__shfl_sync(0xffffffffu, k_s, 0), 16, 1024);
-  const uint64_t dv = umma_sdesc_sw128(__shfl_sync(0xffffffffu, v_s, 0), REG, 1024);
+  const uint64_t dv = umma_sdesc_sw128(__shfl_sync(0xffffffffu, v_s, 0), D_ == 64 ? REG : 2048, 1024);
   auto issue_pv = [&](int h, int vst, bool first) {
     tc_fence_after();
     const uint64_t b0 = dv + (uint64_t)(vst * (C::TILE >> 4));
@@ -369,7 +374,7 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
     if (leader) {
       umma_f16_ts(d, a0, b0, idesc_o, first ? 0u : 1u);
 #pragma unroll
-      for (int kk = 1; kk < 8; ++kk) umma_f16_ts(d, a0 + kk * 8, b0 + (uint64_t)(kk * 16 * 128 >> 4), idesc_o, 1u);
+      for (int kk = 1; kk < 8; ++kk) umma_f16_ts(d, a0 + kk * 8, b0 + (uint64_t)(kk * C::V_BLOCK >> 4), idesc_o, 1u);
       umma_commit(bar.o_done(h));
     }
     __syncwarp();
@@ -511,7 +516,6 @@ __device__ __noinline__ void tc_row_again(const MaskedParams& p, const MaskedGro
 template <typename T, int D_>
 __device__ void tc_values(const MaskedParams& p, const TcBars& bar, unsigned char* base, uint32_t v_s, TcRing& ring) {
   using C = TcCfg<D_>;
-  constexpr uint32_t REG = 128 * 128;
   constexpr uint32_t EX = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   const int lane = threadIdx.x & 31;
   volatile int* poison = reinterpret_cast<volatile int*>(base + kTcPoison);
@@ -528,7 +532,7 @@ __device__ void tc_values(const MaskedParams& p, const TcBars& bar, unsigned cha
       const bool masked = w.masked(j);
 #pragma unroll 1
       for (int row = masked ? threadIdx.x & 63 : 128; row < 128; row += 64) {
-        const uint32_t vs = v_s + vr.st * C::TILE + row * 128;
+        const uint32_t vs = v_s + vr.st * C::TILE + (row >> 4) * C::V_BLOCK + (row & 15) * 128;
         const int v = w.k0 + 128 * j + row;
         bool odd = v >= w.k1;
         if (!odd) {
@@ -536,7 +540,7 @@ __device__ void tc_values(const MaskedParams& p, const TcBars& bar, unsigned cha
           for (int c = 0; c < D_ / 8; ++c) {
             uint32_t e[4];
             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(e[0]), "=r"(e[1]), "=r"(e[2]), "=r"(e[3])
-                         : "r"(vs + (c >> 3) * REG + (((c & 7) ^ (row & 7)) << 4)));
+                         : "r"(vs + (c >> 3) * 2048 + (((c & 7) ^ (row & 7)) << 4)));
 #pragma unroll
             for (int q = 0; q < 4; ++q) odd |= (e[q] & EX) == EX || ((e[q] >> 16) & EX) == EX;
           }
@@ -545,7 +549,7 @@ __device__ void tc_values(const MaskedParams& p, const TcBars& bar, unsigned cha
         if (odd) {
 #pragma unroll
           for (int c = 0; c < D_ / 8; ++c)
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (c >> 3) * REG + ((c & 7) << 4)), "r"(0)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + (c >> 3) * 2048 + ((c & 7) << 4)), "r"(0)
                          : "memory");
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
@@ -941,7 +945,7 @@ int launch_masked_tc(const MaskedParams& p, int dtype, void* stream, const char*
   const int out16 = reinterpret_cast<uintptr_t>(p.out) % 16 == 0 && p.out_stride % 8 == 0;
   CUtensorMap tq, tk, tv;
   if (!encode_pool_map(&tk, p.kp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, 1, false) ||
-      !encode_pool_map(&tv, p.vp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, 1, false) ||
+      !encode_pool_map(&tv, p.vp, dtype, p.D, p.Hkv, p.bs, p.num_blocks, 1, p.D == 128) ||
       (q_tma && !encode_rows_map(&tq, p.q, dtype, p.D, p.Hq, p.rows, p.q_stride, p.G, TT)))
     return fail(NF_ECUDA, "%s: tensor map encoding failed", what);
   if (!q_tma) tq = tk;  // (not used)
