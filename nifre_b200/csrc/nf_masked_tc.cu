@@ -28,15 +28,19 @@
 // item does see one of them, the item's rows are computed again one by one
 // (slow, and right: such values are rare and wrong already).
 //
-// Bound by the softmax pass: for heads of 64 a tile's 32,768 exponentials take
-// 2,048 of its 3,100 to 3,400 cycles and the two products 512; for heads of 128
-// S, the weights and P V of a half follow one another (3,815 cycles a pair of
-// tiles, 2,048 of them products).  A chunk of 2,048 tokens with a window of
-// 4,096, 32 heads of 128: 152 us (900 TFLOP/s; 165 when it runs without a pause
-// and the clock falls); 4 chunks of 512 with windows of 1,024, 32 heads of 64:
-// 47 us; 16 trees of 32 tokens on contexts up to 4,096,
-// same heads: 45 us, where the transitions
-// between items (about 5,000 cycles each) weigh as much as the tiles.
+// What bounds it, measured with copies of the kernel that leave work out: for
+// heads of 64 the exponentials (4 chunks of 512 tokens, windows of 1,024, 32
+// heads: 46 us; 37 without them): a pair of tiles takes 3,100 cycles, 2,048 of them on
+// the special-function unit and 1,024 in products.  For heads of 128 (a chunk
+// of 2,048 tokens, window 4,096, 32 heads: 139 us, 980 TFLOP/s; longer when it
+// runs without a pause and the clock falls) first the copies of 16-key blocks (128 us
+// with an eighth of them; 144 before a value block was one copy instead of two), then
+// the chain S, weights, P V of a half.  Both run 256 items on 148 SMs, two turns
+// where 1.73 would do; parts to even that out would cost as much in merging.
+// 16 trees of 32 tokens on contexts up to 4,096, 32 heads of 64: 43 us, where the
+// copies and the transitions between items weigh most.  Taken and dropped: two
+// threads a row (the exchange of their maxima costs 450 cycles a tile), the next
+// scores loaded before the weights are stored, S in two products of 64 keys.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
