@@ -265,7 +265,7 @@ class MaskedAttentionOps:
         ``plan``).  ``into``: a plan of the same window from an earlier step of
         the batch, whose device buffers are filled again, so that a CUDA graph
         captured with it reads the new step (refill on the stream that
-        replays it); ValueError where the new lists do not fit them (then
+        replays it, or once its calls are done); ValueError where the new lists do not fit them (then
         capture again with a new plan).
         """
         if int(window) != window or window <= 0:
@@ -349,6 +349,7 @@ class MaskedAttentionOps:
         if into is not None:
             view.buf.copy_(host, non_blocking=True)
             view.ready.record(torch.cuda.current_stream(self.device))
+            view.streams = {self._stream()}  # the others wait for this upload
             return view
         view.buf = host.to(self.device, non_blocking=True)
         D, room = self.head_dim, view.room

@@ -402,6 +402,26 @@ def test_captured_decode_steps_with_refilled_plans(shape):
     cache.check_status()
 
 
+def test_refilled_plan_on_another_stream():
+    """A call on another stream than the refill's, whose stream is busy, waits for the refill."""
+    st = Step([2000, 700], [1, 1], 8, 8, 64, 16, BF, seed=15)
+    view = st.cache.plan_window(st.plan, 100, 4, q_heads=8)
+    other, out = torch.cuda.Stream(), torch.zeros_like(st.q[0])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(other):
+        st.cache.window_attention_step(0, st.q[0], view, out)
+    torch.cuda.synchronize()
+    st.ctx = [c + 1 for c in st.ctx]
+    st.plan = st._append([0, 1], [1, 1], st.start, st.rows, q_heads=8)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(20_000_000)
+    assert st.cache.plan_window(st.plan, 100, 4, q_heads=8, into=view) is view
+    with torch.cuda.stream(other):
+        st.cache.window_attention_step(0, st.q[0], view, out)
+    torch.cuda.synchronize()
+    st.check(out, lambda s: window_seen(st.ctx[s], st.n[s], 100, 4))
+
+
 def test_two_plans_on_two_streams():
     """Plans have work queues and partial rows of their own: different plans' calls may overlap."""
     st = Step([2000, 1500, 900], [1, 8, 20], 32, 8, 64, 16, BF, seed=14)
