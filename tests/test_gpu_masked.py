@@ -361,6 +361,22 @@ def test_bad_records_are_flagged_not_followed():
         st.cache.check_status()
 
 
+@pytest.mark.parametrize("field,value", [(4, 99), (5, 139), (6, -1), (6, 1000), (0, 8), (0, 4096)])
+def test_bad_tensor_core_items_are_flagged_not_followed(field, value):
+    from nifre_b200 import _lib
+    from nifre_b200.masked import WorkLists
+    st = Step([40, 40], [70, 70], 4, 2, 64, 16, BF, seed=16)
+    view = st.cache.plan_window(st.plan, 30, 0, q_heads=4)
+    at, _ = WorkLists.offsets(view.room)
+    assert view.buf[1] == 2 and view.buf[0] == 0  # two items, no units
+    view.buf[at[1] + field] = value
+    out = torch.full((140, 256), 7, dtype=BF, device=DEV)
+    st.cache.window_attention_step(0, st.q[0], view, out)
+    with pytest.raises(_lib.NifreError, match="bad slot=1"):
+        st.cache.check_status()
+    assert int((out == 7).all(1).sum()) == 70  # the other sequence's rows are there
+
+
 @pytest.mark.parametrize("shape", [SHAPES[i] for i in (0, 3, 5)], ids=[IDS[i] for i in (0, 3, 5)])
 def test_captured_decode_steps_with_refilled_plans(shape):
     """A CUDA graph of a layer's append and windowed attention, replayed over the next steps of the batch with
