@@ -133,8 +133,10 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
     slots, q_lens, q_starts, ctx = (np.asarray(a, dtype=np.int64) for a in (slots, q_lens, q_starts, ctx))
     t_unit, t_item = max(1, unit_rows // group), item_rows // group
     span = q_lens + (ctx if words is not None else np.minimum(ctx, window + sinks))
-    if not item_rows and int((-(-q_lens // t_unit) * span).sum()) * kv_heads < 256 * workers:
-        t_unit = max(1, 8 // group)  # few groups of few keys: smaller ones, for the kernel of few columns, fill the GPU
+    if not item_rows and int((-(-q_lens // t_unit) * span).sum()) * kv_heads < 100 * workers:
+        # few groups of few keys: smaller ones, for the kernel of few columns, fill the GPU (float32, 12 heads: a tree of
+        # 16 tokens on 500 keys 17.7 us, 19.6 in tiles; on 3000 keys 30.9 and 20.9)
+        t_unit = max(1, 8 // group)
     routed = (q_lens > t_unit) & (t_item > 0)
     per = np.where(routed, max(1, t_item), t_unit)
     n_groups = -(-q_lens // per)
@@ -161,7 +163,7 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
             cuts.append((mine, mine, mine, mine))
             continue
         k = keys[mine]
-        share = share or share_for(k, ntok[mine] * group, workers, kv_heads, head_dim)
+        share = share or share_for(k, ntok[mine] * group, workers, kv_heads, head_dim, item_rows)
         if share:
             g, k0, k1, at = even_shares(k, share, align, least, each)
         else:  # whole groups, the longest first
@@ -193,12 +195,22 @@ def build_lists(slots, q_lens, q_starts, ctx, group: int, unit_rows: int, item_r
                      int(ntok[~on_items].max()) if (~on_items).any() else 0, int(parts.max()))
 
 
-def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
+def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int, item_rows: int) -> int:
     """Keys per share of units: one a worker, and 64 at least.  (Finer shares and a queue over them cost more in
     partial results than they even out: 64 windows of 4096 keys, 296 CTAs, 165 us in 127 shares, 175 in 444, 178 in
-    592.)  ``head_dim`` 0: the kernel of other types and shapes, a CTA a (unit, KV head, four rows), eight an SM,
-    which is quick on 256 keys and would rather not merge."""
-    if not head_dim:
+    592.)  Without ``item_rows`` the kernels of other types and shapes: of few rows, a CTA a (unit, KV head, four
+    rows), eight an SM, which is quick on 256 keys and would rather not merge; of more, a CTA a (unit, KV head), two an
+    SM with narrow heads, and no cuts (0) where there are CTAs enough or keys few (a float32 chunk of 200 tokens,
+    12 heads, window 256: 31 us, 39 uncut; 8 of them 128 uncut, 141 cut); with long shares several a CTA, which
+    even out (16 trees of 16 tokens on up to 4000 keys: 204 us, 244 in one turn)."""
+    if not item_rows:
+        if rows.max() > 8:
+            ctas, total = workers * (2 if head_dim <= 64 else 1), int(keys.sum()) * kv_heads
+            while total >= 1024 * ctas:
+                ctas *= 2
+            if len(keys) * kv_heads >= ctas or keys.max() <= 128:
+                return 0
+            return max(64, -(-total // (ctas * 32)) * 32)
         each = kv_heads * max(1, -(-int(rows.max()) // 4))  # CTAs a unit
         return max(256 if len(keys) * each >= 48 else 128,
                    -(-int(keys.sum()) * each // (workers * 8 * 16)) * 16)
@@ -206,7 +218,7 @@ def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> in
     return max(64, -(-int(keys.sum() + 48 * len(keys)) // (workers * 16)) * 16)
 
 
-def item_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int) -> int:
+def item_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int, item_rows: int) -> int:
     """Keys per share of tensor-core items, 0 for whole groups.
 
     Whole groups need no merge, but the workers end unevenly; equal shares cost
@@ -330,7 +342,7 @@ class MaskedAttentionOps:
             raise RuntimeError("plans are made outside a CUDA graph capture (and refilled with into=)")
         unit_rows, item_rows = self.masked_limits(q_heads)
         lists = build_lists(plan.slots, plan.q_lens, plan.q_starts, plan.ctx_before, q_heads // self.n_heads, unit_rows,
-                            item_rows, self.sm_count, self.n_heads, self.head_dim if item_rows else 0, window,
+                            item_rows, self.sm_count, self.n_heads, self.head_dim, window,
                             sinks, words)
         sizes = lists.sizes()
         if into is None:

@@ -100,6 +100,17 @@ def test_tree_visibility_and_bits():
         assert back == seen.astype(int).tolist()
 
 
+def test_shares_of_the_other_kernels():
+    """Groups of more than 8 rows are cut where there are fewer of them than CTAs, by length; never below 64 keys."""
+    from nifre_b200.masked import unit_share_for
+    rows, cut = np.array([16]), lambda keys, n, d=64: unit_share_for(np.full(n, keys), rows, 148, 12, d, 0)
+    assert cut(500, 25) == 0 and cut(100, 1) == 0
+    assert cut(3000, 1) == 128 and cut(200, 1) == 64
+    assert 1024 >= cut(4000, 25) >= 512
+    assert cut(3000, 1, 128) == 2 * cut(3000, 1)
+    assert unit_share_for(np.array([3000]), np.array([8]), 148, 12, 64, 0) >= 128
+
+
 def test_even_shares_cover_every_group_in_order():
     rng = np.random.default_rng(1)
     for n, most, share, align in ((1, 5, 64, 16), (9, 3000, 448, 16), (40, 200, 64, 16), (5, 9000, 256, 128), (64, 1041, 464, 16)):
