@@ -236,9 +236,10 @@ __global__ void __launch_bounds__(kVecWarps * 32, C == 1 ? 3 : 2) masked_vec_ker
 // 1,150 a warp and tile for 512 FMAs at head_dim 64): 8 float32 chunks of 200
 // tokens, 12 heads and a window of 256 keys 127 us, with four columns a CTA 294;
 // 25 trees of 16 tokens on up to 4,000 keys, 12 heads, 446 us.
-// D <= 32 ND.
+// D <= 32 ND; two CTAs an SM up to 128 (in 128 registers: 6 trees of 20 tokens on
+// up to 2,000 keys, 8 float32 heads of 128, 94 us, 125 with one CTA).
 template <typename T, int ND, bool VEC>
-__global__ void __launch_bounds__(256, ND <= 2 ? 2 : 1) masked_tile_kernel(const MaskedParams p) {
+__global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const MaskedParams p) {
   constexpr int VW = sizeof(T) == 4 ? 4 : 8;
   extern __shared__ float4 tile_smem[];
   const int D4 = (p.D + 3) >> 2, KP = D4 + 1;  // float4s of a row, and of a padded K row
@@ -602,6 +603,7 @@ template <typename T, bool VEC>
 static int dispatch_tile(const MaskedParams& p, cudaStream_t st, const char* what) {
   if (p.D <= 32) return launch_tile<T, 1, VEC>(p, st, what);
   if (p.D <= 64) return launch_tile<T, 2, VEC>(p, st, what);
+  if (p.D <= 96) return launch_tile<T, 3, VEC>(p, st, what);
   if (p.D <= 128) return launch_tile<T, 4, VEC>(p, st, what);
   return launch_tile<T, 8, VEC>(p, st, what);
 }

@@ -200,12 +200,12 @@ def unit_share_for(keys, rows, workers: int, kv_heads: int, head_dim: int, item_
     partial results than they even out: 64 windows of 4096 keys, 296 CTAs, 165 us in 127 shares, 175 in 444, 178 in
     592.)  Without ``item_rows`` the kernels of other types and shapes: of few rows, a CTA a (unit, KV head, four
     rows), eight an SM, which is quick on 256 keys and would rather not merge; of more, a CTA a (unit, KV head), two an
-    SM with narrow heads, and no cuts (0) where there are CTAs enough or keys few (a float32 chunk of 200 tokens,
+    SM with heads of up to 128, and no cuts (0) where there are CTAs enough or keys few (a float32 chunk of 200 tokens,
     12 heads, window 256: 31 us, 39 uncut; 8 of them 128 uncut, 141 cut); with long shares several a CTA, which
     even out (16 trees of 16 tokens on up to 4000 keys: 204 us, 244 in one turn)."""
     if not item_rows:
         if rows.max() > 8:
-            ctas, total = workers * (2 if head_dim <= 64 else 1), int(keys.sum()) * kv_heads
+            ctas, total = workers * (2 if head_dim <= 128 else 1), int(keys.sum()) * kv_heads
             while total >= 1024 * ctas:
                 ctas *= 2
             if len(keys) * kv_heads >= ctas or keys.max() <= 128:

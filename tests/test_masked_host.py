@@ -107,7 +107,7 @@ def test_shares_of_the_other_kernels():
     assert cut(500, 25) == 0 and cut(100, 1) == 0
     assert cut(3000, 1) == 128 and cut(200, 1) == 64
     assert 1024 >= cut(4000, 25) >= 512
-    assert cut(3000, 1, 128) == 2 * cut(3000, 1)
+    assert cut(3000, 1, 256) == 2 * cut(3000, 1, 128)
     assert unit_share_for(np.array([3000]), np.array([8]), 148, 12, 64, 0) >= 128
 
 
