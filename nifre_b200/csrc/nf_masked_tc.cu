@@ -8,8 +8,8 @@
 // place in the pools, so the gap between a window's sinks and its last keys
 // costs nothing: tiles hold visible keys (rounded to 16) only.
 //
-//   producer warp: tensor copies of the queries and of K and V tiles (one
-//     16-token box per block and 64-element part of a head) into rings;
+//   producer warp: tensor copies of the queries and of K and V tiles (a
+//     block's 16 tokens a copy, two for the K of 128-wide heads) into rings;
 //   MMA warp: S_h = Q_h K^T (M = N = 128) into tensor memory, then
 //     O_h += P_h V with P_h from tensor memory;
 //   two softmax warpgroups (thread = row), one per half;
