@@ -207,20 +207,20 @@ class PageOps:
             self._own_blocks(s, first // bs, -(-(c + q) // bs))
         moves, pos = [], []
         for s, c, path in zip(slots, ctx, kept):
+            pos += (s, c + len(path))
             blocks, started = self.block_tables[s]._physical_blocks, 0
             for j, t in enumerate(path):
                 if t == j:
                     continue
                 a, b = c + t, c + j
                 src, dst = blocks[a // bs] * bs + a % bs, blocks[b // bs] * bs + b % bs
-                if started and src == moves[-4] + moves[-2] and dst == moves[-3] + moves[-2]:
-                    moves[-2] += 1  # one run of rows
+                if started and moves[-2] < bs and src == moves[-4] + moves[-2] and dst == moves[-3] + moves[-2]:
+                    moves[-2] += 1  # one record, of bs rows at most (blocks with consecutive ids would make it longer)
                 else:
                     moves += (src, dst, 1, started)
                     started = 1
-            self.pos_host[s] = c + len(path)
-            pos += (s, c + len(path))
         self._move_rows(moves, pos, bs)
+        self.pos_host[slots] = pos[1::2]
 
     def _own_blocks(self, slot: int, first: int, end: int) -> None:
         """Replace blocks first .. end-1 of the slot's table that others hold too by copies of its own."""

@@ -323,3 +323,41 @@ def test_speculative_decoding_run():
     for s in range(3):
         c.truncate(s, c.length(s))
     _same(c, m)
+
+
+@pytest.mark.parametrize("slots", [2, 140])
+@pytest.mark.parametrize("how", ["compacted", "reused"])
+def test_keep_tokens_moves_paths_longer_than_a_block(slots, how):
+    """Paths of 30 rows in a row, in blocks with consecutive ids (after compact(), and in slots that were cleared and
+    filled again); lists that travel as arguments and lists in device memory."""
+    g = torch.Generator().manual_seed(8)
+    c = _cache(L=2, hkv=1, slots=slots, max_len=64, num_blocks=4 * slots)
+    m = _model(c)
+    every = list(range(slots))
+    if how == "reused":
+        _grow(c, every, [60] * slots, g, m)
+        for s in every:
+            c.reset_slot(s)
+            m[s] = _cut(m, s, 0)
+    else:
+        c.block_allocator.set_free_order(torch.randperm(c.num_blocks, generator=g).tolist())
+    _grow(c, every, [20] * slots, g, m)
+    plan = _grow(c, every, [40] * slots, g, m)
+    if how == "compacted":
+        c.reset_slot(slots - 1)
+        m[slots - 1] = _cut(m, slots - 1, 0)
+        c.compact()
+        plan = None
+        for s in every:
+            c.truncate(s, min(c.length(s), 20))
+            m[s] = _cut(m, s, 20)
+        _grow(c, [slots - 1], [20], g, m)
+        c.compact()
+        plan = _grow(c, every, [40] * slots, g, m)
+    paths = [list(range(1, 31)) for _ in every]
+    paths[0] = [0, 2, *range(5, 38)]
+    c.keep_tokens(plan, paths)
+    for s in every:
+        m[s] = [[t[[*range(20), *(20 + j for j in paths[s])]].clone() for t in pair] for pair in m[s]]
+        c.truncate(s, c.length(s))
+    _same(c, m)

@@ -357,3 +357,63 @@ def test_page_and_plan_refusals_before_any_launch():
     for call in (lambda: dense.fork([0], [1]), dense.compact):
         with pytest.raises(ValueError, match="dense"):
             call()
+
+
+def _host_cache(slots=4, num_blocks=40, bs=16, max_len=512):
+    """A cache's host side without a device; ``moved``: what _move_rows was asked for."""
+    c = PagedKVCache(1, max_len, 2, 64, device="cpu", dtype=torch.float16, block_size=bs)
+    c.batch_size, c.num_blocks, c._dev_index = slots, num_blocks, 0
+    c.pos_host = np.zeros(slots, dtype=np.int64)
+    c.block_allocator = BlockAllocator(num_blocks)
+    c.block_tables = [BlockTable(c.block_allocator, bs) for _ in range(slots)]
+    c._init_holes(slots)
+    c.moved = []
+    c._move_rows = lambda moves, pos, most: c.moved.append((list(moves), list(pos), most))
+    return c
+
+
+@pytest.mark.parametrize("bs", [16, 5])
+@pytest.mark.parametrize("ascending", [True, False])
+def test_kept_paths_longer_than_a_block(bs, ascending):
+    """Records of a kept path have block_size rows at most, also where consecutive blocks have consecutive ids, and
+    move every row of the path behind the context in order."""
+    from types import SimpleNamespace
+    c = _host_cache(slots=3, bs=bs, num_blocks=60)
+    if ascending:  # ids are handed out from the end of the free list
+        c.block_allocator.set_free_order(range(59, -1, -1))
+    ctx, n = [20, 0, 7], [40, 40, 3]
+    paths = [list(range(1, 31)), [0, *range(2, 40)], [2]]
+    for s in range(3):
+        c.block_tables[s].ensure_capacity(ctx[s] + n[s])
+        c.pos_host[s] = ctx[s] + n[s]
+    row = lambda s, t: c.block_tables[s].resolve(t)[0] * bs + t % bs  # noqa: E731
+    rows = np.arange(60 * bs)
+    want = [[row(s, t) for t in [*range(ctx[s]), *(ctx[s] + j for j in paths[s])]] for s in range(3)]
+    plan = SimpleNamespace(closed=True, slots=np.arange(3), ctx_before=np.asarray(ctx), q_lens=np.asarray(n), n_seqs=3)
+    c.keep_tokens(plan, paths)
+    ((moves, pos, most),) = c.moved
+    assert most == bs
+    for a, b, count, _ in np.asarray(moves).reshape(-1, 4).tolist():
+        assert 0 < count <= most
+        for i in range(count):
+            rows[b + i] = rows[a + i]
+    for s in range(3):
+        kept = ctx[s] + len(paths[s])
+        assert [rows[row(s, t)] for t in range(kept)] == want[s]
+        assert pos[2 * s:2 * s + 2] == [s, kept] and c.length(s) == kept
+
+
+def test_a_refused_move_leaves_the_positions():
+    from types import SimpleNamespace
+    c = _host_cache()
+    c.block_tables[0].ensure_capacity(30)
+    c.pos_host[0] = 30
+
+    def refuse(*a):
+        raise _lib.NifreError("nf_kv_move")
+
+    c._move_rows = refuse
+    plan = SimpleNamespace(closed=True, slots=np.asarray([0]), ctx_before=np.asarray([20]), q_lens=np.asarray([10]), n_seqs=1)
+    with pytest.raises(_lib.NifreError):
+        c.keep_tokens(plan, [[1, 3]])
+    assert c.length(0) == 30
