@@ -818,6 +818,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
       __syncwarp();
       if (lane == 0) mbar_arrive(bar.join_empty());
     }
+    __syncwarp();  // (eight lanes have stored a row together: before its own lane stores it again)
     if (poison[seq & 7] == seq && valid)
       tc_row_again<T, D_>(p, w.g, w.k0, w.k1, w.part, w.kvh, tok, hd);
   }
