@@ -208,16 +208,14 @@ __global__ void __launch_bounds__(kVecWarps * 32, C == 1 ? 3 : 2) masked_vec_ker
       for (int w = 0; w < kVecWarps; ++w) {
         const float* st = joined + (w * C + c) * DJ;
         const float f = ex2(st[p.D] - base);
-        if (st[p.D] != -INFINITY) {  // (a warp whose keys the column does not see)
-          A = fmaf(st[e], f, A);
-          L = fmaf(st[p.D + 1], f, L);
-        }
+        A = fmaf(st[e], f, A);
+        L = fmaf(st[p.D + 1], f, L);
       }
       if (n_parts == 1) {
         const int t = col / p.G, head = kvh * p.G + (col - t * p.G);
-        const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-        reinterpret_cast<T*>(p.out)[(long long)(g.q_row0 + t) * p.out_stride + (long long)head * p.D + e] =
-            Elem<T>::from_f(A * inv);
+        T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + t) * p.out_stride + (long long)head * p.D + e;
+        *dst = Elem<T>::from_f(A * state_inverse(L));
+        if (no_output(p, g, t, L)) *dst = Elem<T>::from_f(kNaN);
       } else if (rec) {
         float* r = rec + (long long)col * p.DP;
         r[e] = A;
@@ -413,12 +411,14 @@ __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const
       const int col = w0 + c;
       if (col >= cols) continue;
       if (n_parts == 1) {
-        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+        const float inv = state_inverse(sum);
         T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok[c]) * p.out_stride +
                  (long long)(kvh * p.G + col - tok[c] * p.G) * p.D;
 #pragma unroll
         for (int i = 0; i < ND; ++i)
           if (32 * i + lane < p.D) dst[32 * i + lane] = Elem<T>::from_f(o[c][i] * inv);
+        if (no_output(p, g, tok[c], sum))
+          for (int e = lane; e < p.D; e += 32) dst[e] = Elem<T>::from_f(kNaN);
       } else if (rec) {
         float* r = rec + (long long)col * p.DP;
 #pragma unroll
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(256, 4) masked_merge_kernel(const MaskedParams
           A.x *= sc; A.y *= sc; A.z *= sc; A.w *= sc; L *= sc;
 #pragma unroll
           for (int u = 0; u < PB; ++u)
-            if (ml[u].x != -INFINITY) {  // (a part without seen keys)
+            if (ml[u].y != 0.f) {  // (0: no part, or one without seen keys)
               const float w = ex2(ml[u].x - b);
               A.x = fmaf(x[u].x, w, A.x); A.y = fmaf(x[u].y, w, A.y);
               A.z = fmaf(x[u].z, w, A.z); A.w = fmaf(x[u].w, w, A.w);
@@ -516,18 +516,16 @@ __global__ void __launch_bounds__(256, 4) masked_merge_kernel(const MaskedParams
           for (int w = 1; w < WAYS; ++w) {
             const float2 s = join_s[warp + w][lane];
             const float4 x = join_a[warp + w][lane];
-            if (s.x != -INFINITY) {
-              const float f = ex2(s.x - b);
-              A.x = fmaf(x.x, f, A.x); A.y = fmaf(x.y, f, A.y); A.z = fmaf(x.z, f, A.z); A.w = fmaf(x.w, f, A.w);
-              L = fmaf(s.y, f, L);
-            }
+            const float f = ex2(s.x - b);
+            A.x = fmaf(x.x, f, A.x); A.y = fmaf(x.y, f, A.y); A.z = fmaf(x.z, f, A.z); A.w = fmaf(x.w, f, A.w);
+            L = fmaf(s.y, f, L);
           }
         }
       }
       if (way != 0 || !base || c >= D4) continue;
-      const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-      const float o[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
       const int tok = row / p.G;
+      const float inv = state_inverse(L);
+      const float o[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
       T* d = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride +
              (long long)(kvh * p.G + row - tok * p.G) * p.D + 4 * c;
       if (sizeof(T) == 2 && 4 * c + 4 <= p.D && (reinterpret_cast<uintptr_t>(d) & 7) == 0) {
@@ -538,6 +536,8 @@ __global__ void __launch_bounds__(256, 4) masked_merge_kernel(const MaskedParams
         for (int e = 0; e < 4; ++e)
           if (4 * c + e < p.D) d[e] = Elem<T>::from_f(o[e]);
       }
+      if (no_output(p, g, tok, L))
+        for (int e = 0; e < 4 && 4 * c + e < p.D; ++e) d[e] = Elem<T>::from_f(kNaN);
     }
   }
 }
@@ -653,6 +653,7 @@ static int masked_check(const NfMaskedArgs* a, bool tree, const char* what, Mask
       (a->ws_rows && !a->ws))
     return fail(NF_EINVAL, "%s: null pointer argument", what);
   if (a->q_row_stride < 0 || a->out_row_stride < 0) return fail(NF_EINVAL, "%s: negative row stride", what);
+  if (!isfinite(a->scale)) return fail(NF_EINVAL, "%s: scale is not finite", what);
   if (tree && (!a->masks || a->mask_words <= 0)) return fail(NF_EINVAL, "%s: null mask words", what);
   if (!tree && (a->window <= 0 || a->sinks < 0))
     return fail(NF_EINVAL, "%s: window (%d) must be positive and sinks (%d) not negative", what, a->window, a->sinks);

@@ -137,6 +137,31 @@ __device__ __forceinline__ float* part_base(const MaskedParams& p, const MaskedG
   return p.ws + (row * p.Hq + (long long)kvh * g.ntok * p.G) * p.DP;
 }
 
+// A softmax state (m, l, values) holds the largest score, the sum of the
+// weights 2^(x - m) and the weighted values.  m passes NaN over, so m = -inf
+// does not say that nothing was seen: a state whose seen scores are NaN has
+// l = NaN, and joins keep it (its weight is 2^-inf = 0, and 0 * NaN is NaN).
+// l = 0 is left for no key seen, whose output is 0, and for seen scores that
+// are all -inf, whose output is 0 / 0; only then is it asked which.
+__device__ __forceinline__ bool sees_any(const MaskedParams& p, const MaskedGroup g, int t) {
+  if (!p.tree || g.ctx > 0) return true;  // (a window holds the token itself)
+  const int words = (g.n_draft + 31) >> 5;
+  uint32_t any = 0;
+  for (int i = 0; i < words; ++i) {
+    const uint32_t w = __ldg(p.masks + g.mask0 + (long long)t * words + i);
+    any |= i + 1 < words || !(g.n_draft & 31) ? w : w & ((1u << (g.n_draft & 31)) - 1);
+  }
+  return any != 0;
+}
+
+// The factor from a final state's weighted values to the output; where l is 0,
+// no_output() after the store says whether that 0 / 0 was an output.
+__device__ __forceinline__ float state_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ bool no_output(const MaskedParams& p, const MaskedGroup& g, int t, float l) {
+  return l == 0.f && sees_any(p, g, t);
+}
+constexpr float kNaN = __builtin_nanf("");
+
 // The tensor-map path (NF_EUNSUPPORTED, nothing launched: not for this shape).
 int launch_masked_tma(const MaskedParams& p, int dtype, void* stream, const char* what);
 // The tensor-core items.

@@ -475,7 +475,8 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
 }
 
 // One row's attention over the item's keys in plain float32, one key at a
-// time (an item whose values are not finite where some of its rows see them).
+// time (an item whose values are not finite where some of its rows see them,
+// a row without a sum of weights).
 template <typename T, int D_>
 __device__ __noinline__ void tc_row_again(const MaskedParams& p, const MaskedGroup g, int k0, int k1, int part, int kvh,
                                           int tok, int hd) {
@@ -503,7 +504,7 @@ __device__ __noinline__ void tc_row_again(const MaskedParams& p, const MaskedGro
     for (int d = 0; d < D_; ++d) acc[d] = fmaf(e, Elem<T>::to_f(vr[d]), acc[d] * a);
   }
   if (part >> 16 == 1) {
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const float inv = no_output(p, g, tok, l) ? kNaN : state_inverse(l);
     T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride + (long long)head * D_;
     for (int d = 0; d < D_; ++d) dst[d] = Elem<T>::from_f(acc[d] * inv);
   } else if (float* rec = part_base(p, g, part & 0xffff, kvh)) {
@@ -601,7 +602,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
       valid = tok0 < TT && (dup ? 0 : h * TT) + tok0 < w.g.ntok;
     }
     float m = 0.f, l = 0.f;  // the reference of the exponents, and the sum of the weights
-    bool none = true;        // the row has seen no key yet
+    bool none = true;        // no score of the row has had a place in a maximum yet
     int n = 0;  // tiles done
     for (int j = dup ? h : 0; j < nkt; j += dup ? 2 : 1, ++n) {
       if (!mbar_wait(bar.s_full(h), n_s & 1, p.status)) return;
@@ -735,7 +736,7 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
     // the row's place in out, in elements (-1: not a row)
     long long at = -1;
     if (n_parts == 1) {
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      const float inv = state_inverse(l);
       a0 *= inv;
       a1 *= inv;
       if (valid) at = (long long)(w.g.q_row0 + tok) * p.out_stride + (long long)(w.kvh * p.G + hd) * D_;
@@ -819,7 +820,8 @@ __device__ void tc_softmax(const MaskedParams& p, int TT, bool out16, const TcBa
       if (lane == 0) mbar_arrive(bar.join_empty());
     }
     __syncwarp();  // (eight lanes have stored a row together: before its own lane stores it again)
-    if (poison[seq & 7] == seq && valid)
+    // (l = 0: nothing seen, or 0 / 0)
+    if (valid && (poison[seq & 7] == seq || (l == 0.f && n_parts == 1)))
       tc_row_again<T, D_>(p, w.g, w.k0, w.k1, w.part, w.kvh, tok, hd);
   }
 }

@@ -501,6 +501,7 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
     if (!last) continue;
     const int cols = g.ntok * p.G, n_parts = part >> 16;
     float* rec = n_parts > 1 ? part_base(p, g, part & 0xffff, kvh) : nullptr;
+    uint32_t zero = 0;  // columns whose output is 0 / 0, or nothing
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -512,13 +513,14 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
         if (c >= cols) continue;
         const int tok = c / p.G, head = kvh * p.G + (c - tok * p.G);
         if (n_parts == 1) {
-          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+          const float inv = state_inverse(l);
           T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride + (long long)head * D_ + tq;
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
             dst[16 * i] = Elem<T>::from_f(st.o[i][j][e] * inv);
             dst[16 * i + 8] = Elem<T>::from_f(st.o[i][j][2 + e] * inv);
           }
+          if (l == 0.f) zero |= 1u << (2 * j + e);
         } else if (rec) {
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
@@ -531,6 +533,13 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
                    make_float2(st.none >> (2 * j + e) & 1u ? -INFINITY : st.m[j][e], l));
         }
       }
+    for (; zero; zero &= zero - 1) {
+      const int b = __ffs(zero) - 1, c = c0 + 8 * (b >> 1) + n0 + (b & 1), tok = c / p.G;
+      if (!no_output(p, g, tok, 0.f)) continue;
+      T* dst = reinterpret_cast<T*>(p.out) + (long long)(g.q_row0 + tok) * p.out_stride +
+               (long long)(kvh * p.G + (c - tok * p.G)) * D_ + tq;
+      for (int i = 0; i < 2 * KS; ++i) dst[8 * i] = Elem<T>::from_f(kNaN);
+    }
   }
 }
 

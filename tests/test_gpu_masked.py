@@ -238,6 +238,97 @@ def test_strided_unaligned_queries_and_scale(dtype):
     assert (buf[:, :9] == 7).all() and (buf[:, 521:] == 7).all()
 
 
+def _split(monkeypatch, keys=16, item_keys=128):
+    """Parts of ``keys`` keys, and of ``item_keys`` for the tensor cores' items; the last one as short as it comes."""
+    from nifre_b200 import masked
+    even = masked.even_shares
+    monkeypatch.setattr(masked, "unit_share_for", lambda *a: keys)
+    monkeypatch.setattr(masked, "item_share_for", lambda *a: item_keys)
+    monkeypatch.setattr(masked, "even_shares", lambda k, share, align, least, each=0: even(k, share, align, 1, 0))
+
+
+def _tree_out(st, masks, hq):
+    view = st.cache.plan_tree(st.plan, masks=masks, q_heads=hq)
+    out = torch.full((st.rows, hq * st.d), 7, dtype=st.dtype, device=DEV)
+    return st.cache.tree_attention_step(0, st.q[0], view, out).clone()
+
+
+def _set_key(st, s, t, x, what="k"):
+    block, off = st.cache.block_tables[s].resolve(t)
+    getattr(st.cache, what)[0][block, off] = x
+
+
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+def test_scores_that_are_not_numbers_reach_the_output(shape, split, monkeypatch):
+    """A NaN query row, and a NaN key that a row sees -- as the only seen key of a warp, a part, a step, or of the row
+    -- give NaN in all of the row; the other rows keep their bits."""
+    hq, hkv, d, bs, dtype = shape
+    if split:
+        _split(monkeypatch)
+    n = [1, 1, 5, 2, 40, 200, 33, 2]
+    st = Step([8, 0, 48, 16, 64, 128, 0, 70], n, hq, hkv, d, bs, dtype, seed=21, pad=1)
+    masks = [np.eye(m, dtype=bool) for m in n]
+    masks[4][7, [0, 20]] = True
+    masks[5][::3, :90] = True
+    masks[6][20:, 5] = True
+    want = _tree_out(st, masks, hq)
+    keys = {0: 0, 1: 0, 2: 3, 4: 20, 5: 150, 6: 5}  # the drafted token of each sequence whose key is NaN
+    for s, j in keys.items():
+        _set_key(st, s, st.ctx[s] + j, float("nan"))
+    _set_key(st, 3, 10, float("nan"))  # and a key of a context: every row of its sequence
+    st.q[0][st.start[5] + 170] = float("nan")
+    st.q[0][st.start[7] + 1] = float("nan")
+    st.q[0][st.start[4] + 2, d // 2] = float("nan")  # one element of the first head's query
+    out = _tree_out(st, masks, hq)
+    for s, m in enumerate(n):
+        for i in range(m):
+            row, was = out[st.start[s] + i], want[st.start[s] + i]
+            if (s in keys and masks[s][i, keys[s]]) or s == 3 or (s, i) in ((5, 170), (7, 1)):
+                assert torch.isnan(row).all(), (s, i)
+            elif (s, i) == (4, 2):
+                assert torch.isnan(row[:d]).all() and torch.equal(row[d:], was[d:])
+            else:
+                assert torch.equal(row, was), (s, i)
+    st.cache.check_status()
+
+
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+def test_scores_of_minus_infinity(shape, split, monkeypatch):
+    """Seen keys that score -inf weigh nothing beside others; a row that sees only such keys is 0 / 0."""
+    hq, hkv, d, bs, dtype = shape
+    if split:
+        _split(monkeypatch)
+    ctx, n = [0, 0, 48, 0, 128], [2, 5, 6, 40, 180]
+    st = Step(ctx, n, hq, hkv, d, bs, dtype, seed=22, pad=1)
+    st.q.view(1, st.rows, hq, d)[..., 0] = 1
+    masks = [np.eye(m, dtype=bool) for m in n]
+    masks[1][:, 4] = True
+    masks[3][10:, :4] = True
+    masks[3][30] = False
+    low = {0: [1], 1: [0, 1, 4], 2: [5], 3: [0, 1, 2, 3, 20], 4: list(range(100, 180))}
+    for s, js in low.items():
+        for j in js:
+            block, off = st.cache.block_tables[s].resolve(ctx[s] + j)
+            st.cache.k[0][block, off, :, 0] = float("-inf")
+    out = _tree_out(st, masks, hq)
+    for s, m in enumerate(n):
+        finite = np.asarray(masks[s]).copy()
+        finite[:, low[s]] = False
+        seen = tree_seen(ctx[s], torch.as_tensor(finite))
+        rows = st.start[s] + np.arange(m)
+        ref, wabs, most = attend(st.q[0][rows].view(m, hq, d), st.k[s][0], st.v[s][0], seen, d ** -0.5)
+        tol = tolerance(ref, wabs, most, ctx[s] + m, d, dtype)
+        for i in range(m):
+            row = out[rows[i]].view(hq, d).double()
+            if not seen[i].any() and masks[s][i].any():
+                assert torch.isnan(row).all(), (s, i)
+            else:
+                assert ((row - ref[i]).abs() <= tol[i]).all(), (s, i)
+    st.cache.check_status()
+
+
 def test_large_scores_and_long_window():
     """Scores far from 0 (one key takes all the weight) and a running maximum that moves late."""
     st = Step([3000], [4], 8, 2, 64, 16, BF, seed=9)

@@ -191,6 +191,14 @@ def test_window_entry_point_refuses(change, match):
     assert match in lib.nf_last_error().decode()
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf")])
+def test_a_scale_that_is_not_finite_is_refused(scale):
+    lib = _lib.load()
+    for fn in (lib.nf_window_attention, lib.nf_tree_attention):
+        a = _args(scale=scale)
+        assert fn(ctypes.addressof(a), None) == 1 and b"scale" in lib.nf_last_error()
+
+
 def test_tree_entry_point_and_limits_refuse():
     lib = _lib.load()
     a = _args(masks=None)
