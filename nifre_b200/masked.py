@@ -359,6 +359,8 @@ class MaskedAttentionOps:
         host = torch.from_numpy(lists.pack(view.room)).pin_memory()
         view.upload_bytes = host.numel() * 4
         if into is not None:
+            if self._stream() not in view.streams:
+                self._adopt_stream(view, self._stream())
             view.buf.copy_(host, non_blocking=True)
             view.ready.record(torch.cuda.current_stream(self.device))
             view.streams = {self._stream()}  # the others wait for this upload
@@ -449,11 +451,12 @@ class MaskedAttentionOps:
 
     @staticmethod
     def _adopt_stream(view, stream) -> None:
-        """First call of a plan on another stream than its own: the upload comes first, and the buffers stay until
-        that stream is done with them.  (A capturing stream orders and keeps nothing: its graph's user does.)"""
+        """First call or refill of a plan on another stream than its last upload's: that upload comes first, and the
+        buffers stay until this stream is done with them.  (A capturing stream orders and keeps nothing: its graph's
+        user does.)"""
         if torch.cuda.is_current_stream_capturing():
             return
-        cur = torch.cuda.current_stream()
+        cur = torch.cuda.current_stream(view.buf.device)
         cur.wait_event(view.ready)
         view.buf.record_stream(cur)
         if view.ws.numel():

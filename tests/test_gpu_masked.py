@@ -529,6 +529,34 @@ def test_refilled_plan_on_another_stream():
     st.check(out, lambda s: window_seen(st.ctx[s], st.n[s], 100, 4))
 
 
+def test_refill_and_calls_on_another_stream_than_the_plans():
+    """A plan made on a busy stream, refilled and called on another one and dropped at once: the first upload does not
+    come after the refill, and the first stream's allocations do not get the plan's memory while the other runs."""
+    st = Step([2000, 700], [1, 1], 8, 8, 64, 16, BF, seed=24)
+    other = torch.cuda.Stream()
+    warm = st.cache.plan_window(st.plan, 100, 4, q_heads=8)
+    out = torch.empty_like(st.q[0])
+    st.cache.window_attention_step(0, st.q[0], warm, out)
+    outs = [torch.zeros_like(out) for _ in range(2)]
+    torch.cuda.synchronize()
+    torch.cuda._sleep(200_000_000)
+    view = st.cache.plan_window(st.plan, 100, 4, q_heads=8)
+    sizes = view.buf.numel(), view.ws.numel()
+    st.ctx = [c + 1 for c in st.ctx]
+    with torch.cuda.stream(other):
+        st.plan = st._append([0, 1], [1, 1], st.start, st.rows, q_heads=8)
+        assert st.cache.plan_window(st.plan, 100, 4, q_heads=8, into=view) is view
+        st.cache.window_attention_step(0, st.q[0], view, outs[0])
+        torch.cuda._sleep(200_000_000)
+        st.cache.window_attention_step(0, st.q[0], view, outs[1])
+    del view
+    other_bufs = [torch.zeros(sizes[0], dtype=torch.int32, device=DEV), torch.full((sizes[1],), 5.0, device=DEV)]
+    torch.cuda.synchronize()
+    assert int(other_bufs[0].count_nonzero()) == 0 and bool((other_bufs[1] == 5).all())
+    for o in outs:
+        st.check(o, lambda s: window_seen(st.ctx[s], st.n[s], 100, 4))
+
+
 def test_two_plans_on_two_streams():
     """Plans have work queues and partial rows of their own: different plans' calls may overlap."""
     st = Step([2000, 1500, 900], [1, 8, 20], 32, 8, 64, 16, BF, seed=14)

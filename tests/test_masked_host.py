@@ -425,3 +425,31 @@ def test_a_refused_move_leaves_the_positions():
     with pytest.raises(_lib.NifreError):
         c.keep_tokens(plan, [[1, 3]])
     assert c.length(0) == 30
+
+
+def test_a_refill_on_another_stream_is_ordered_and_kept(monkeypatch):
+    """The refill's copy waits for the last upload, and the buffers are recorded for the stream it runs on."""
+    from types import SimpleNamespace
+    from nifre_b200.masked import MaskedPlan
+    log = []
+    now = SimpleNamespace(name="B", wait_event=lambda e: log.append("B waits for the upload"))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: now)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
+    c = _host_cache()
+    c._sm_count, c._generation, c._stream = 148, 1, lambda: now.name
+    c.pos_host[:] = [20, 0, 0, 0]
+    plan = SimpleNamespace(slots=np.asarray([0]), q_lens=np.asarray([2]), q_starts=np.asarray([0]), owner=c, generation=1,
+                           ctx_before=np.asarray([18]), n_seqs=1, q_heads=4, rows_needed=2, closed=True)
+    view = MaskedPlan("window", 8, 0, 4, 2)
+    view.owner, view.generation, view.room, view.streams = c, 1, (64,) * 5 + (8, 4), {"A"}
+    view.buf = SimpleNamespace(device="cuda", copy_=lambda *a, **k: log.append("copy"),
+                               record_stream=lambda s: log.append("buf kept for " + s.name))
+    view.ws = SimpleNamespace(numel=lambda: 8, record_stream=lambda s: log.append("ws kept for " + s.name))
+    view.ready = SimpleNamespace(record=lambda s: log.append("upload on " + s.name))
+    assert c.plan_window(plan, 8, q_heads=4, into=view) is view
+    assert log == ["B waits for the upload", "buf kept for B", "ws kept for B", "copy", "upload on B"]
+    assert view.streams == {"B"}
+    del log[:]
+    c.plan_window(plan, 8, q_heads=4, into=view)  # again on the same stream
+    assert log == ["copy", "upload on B"]
