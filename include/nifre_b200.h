@@ -446,8 +446,9 @@ int nf_cascade_limits(int32_t dtype, int32_t num_q_heads, int32_t num_kv_heads, 
  * Workspace: ws (16-byte aligned), ws_rows partial rows of num_q_heads *
  * (head_dim rounded up to a multiple of 4, plus 4) floats; queue: int32[4], zero when
  * allocated, left zero by every call (calls that share it or ws must not
- * overlap).  Bad records are skipped and flagged in *status.  Up to three
- * launches, in stream order.
+ * overlap).  Bad records are skipped and flagged in *status, and so are the keys
+ * of blocks whose table entries are out of range: they take no part.  Up to
+ * three launches, in stream order.
  */
 typedef struct NfMaskedArgs {
   void* out;

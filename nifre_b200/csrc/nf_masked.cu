@@ -245,6 +245,8 @@ __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const
   float4* vs = ks + 32 * KP;          // [32][D4]
   float4* qs = vs + 32 * D4;          // [32][D4]
   float4* ps = qs + 32 * D4;          // [8 warps][32 keys]: four columns' weights
+  // the last fetched tiles (even, odd) with rows in a block that is not there
+  volatile int* missing = reinterpret_cast<volatile int*>(ps + 8 * 32);
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_units = min(__ldg(p.counts + 3), p.max_units);
@@ -300,7 +302,10 @@ __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const
         kr[i] = vr[i] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (r >= 32 || v >= v1) continue;
         const long long row = key_row(p, btrow, vk.key(v));
-        if (row < 0) continue;
+        if (row < 0) {
+          missing[v0 >> 5 & 1] = v0;
+          continue;
+        }
         const T* a = kp + row * row_elems + e;
         const T* b = vp + row * row_elems + e;
         if constexpr (VEC && VW == 4) {
@@ -351,12 +356,13 @@ __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const
         }
       }
       const int v = v0 + lane, key = vk.key(v);
+      const bool there = v < v1 && (missing[v0 >> 5 & 1] != v0 || key_row(p, btrow, key) >= 0);
       bool all = true;
       float4 w;
       float* wp = reinterpret_cast<float*>(&w);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const bool seen = v < v1 && sees(p, g, tok[c], key);
+        const bool seen = there && sees(p, g, tok[c], key);
         all = all && seen;
         float top = seen ? s[c] : -INFINITY;
         const float x = top;
@@ -589,7 +595,7 @@ static int launch_vec(const MaskedParams& p, cudaStream_t st, const char* what) 
 
 template <typename T, int ND, bool VEC>
 static int launch_tile(const MaskedParams& p, cudaStream_t st, const char* what) {
-  const int D4 = (p.D + 3) / 4, smem = (32 * (D4 + 1) + 64 * D4 + 256) * 16;
+  const int D4 = (p.D + 3) / 4, smem = (32 * (D4 + 1) + 64 * D4 + 256 + 1) * 16;
   auto kern = masked_tile_kernel<T, ND, VEC>;
   const cudaError_t e = prepare_launch(reinterpret_cast<const void*>(kern), smem, 256, nullptr);
   if (e != cudaSuccess) return fail(NF_ECUDA, "%s: smem attribute: %s", what, cudaGetErrorString(e));

@@ -252,7 +252,8 @@ __device__ __forceinline__ int tc_block(const MaskedParams& p, const TcItem& w, 
 // of P V (fewer copies: 2 KB a copy is what the copies' rate suffers from).
 template <int D_, bool V>
 __device__ __forceinline__ void tc_load(const MaskedParams& p, const CUtensorMap* tm, uint32_t dst0, uint32_t full,
-                                        int phys, int key, int nb, int kvh, uint64_t pol, int lane) {
+                                        int phys, int key, int nb, int kvh, uint64_t pol, int lane,
+                                        volatile int* poison, int seq) {
   constexpr int NDH = D_ / 64;
   if (lane == 0) mbar_arrive_expect_tx(full, nb * NDH * 2048);
   __syncwarp();
@@ -260,7 +261,8 @@ __device__ __forceinline__ void tc_load(const MaskedParams& p, const CUtensorMap
     const int off = key % p.bs;
     if (phys < 0 || phys >= p.num_blocks) {
       atomicOr(p.status, NF_STATUS_BAD_BLOCK);
-      phys = 0;
+      phys = 0;  // stands in: the item's rows are computed again without the block
+      poison[seq & 7] = seq;
     }
     if constexpr (D_ == 64) {
       tma_load_4d(dst0 + lane * 2048, tm, 0, kvh, off, phys, full, pol);
@@ -301,12 +303,14 @@ __device__ void tc_load_queries(const MaskedParams& p, const TcItem& w, int TT, 
 
 template <typename T, int D_>
 __device__ void tc_producer(const MaskedParams& p, int TT, bool q_tma, const CUtensorMap* tq, const CUtensorMap* tk,
-                            const CUtensorMap* tv, const TcBars& bar, uint32_t q_s, uint32_t k_s, uint32_t v_s,
-                            int tasks, TcRing& ring) {
+                            const CUtensorMap* tv, const TcBars& bar, unsigned char* base, uint32_t q_s, uint32_t k_s,
+                            uint32_t v_s, int tasks, TcRing& ring) {
   using C = TcCfg<D_>;
   constexpr int NDH = D_ / 64;
   const int lane = threadIdx.x & 31;
   const uint64_t pol = l2_evict_last(), pol_q = l2_evict_first();
+  volatile int* poison = reinterpret_cast<volatile int*>(base + kTcPoison);
+  int seq = 0;
   Ring qr, kr, vr;
   TcClaim claim;
   TcItem w;
@@ -316,6 +320,7 @@ __device__ void tc_producer(const MaskedParams& p, int TT, bool q_tma, const CUt
       if (lane == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
       continue;
     }
+    ++seq;
     const int* btrow = p.bt + (long long)w.g.slot * p.max_blocks;
     int key, cur = tc_block(p, w, btrow, 0, lane, key);
     if (!mbar_wait(bar.q_empty(qr.st), qr.ph ^ 1, p.status)) return;
@@ -340,10 +345,11 @@ __device__ void tc_producer(const MaskedParams& p, int TT, bool q_tma, const CUt
     for (int j = 0; j < w.nkt; ++j) {
       const int nb = min(8, (w.k1 - w.k0 - j * 128 + 15) >> 4);
       if (!mbar_wait(bar.k_empty(kr.st), kr.ph ^ 1, p.status)) return;
-      tc_load<D_, false>(p, tk, k_s + kr.st * C::TILE, bar.k_full(kr.st), cur, key, nb, w.kvh, pol, lane);
+      tc_load<D_, false>(p, tk, k_s + kr.st * C::TILE, bar.k_full(kr.st), cur, key, nb, w.kvh, pol, lane, poison, seq);
+      __syncwarp();  // (the item's mark comes before the V tile is announced, and so before every epilogue)
       kr.next(C::KST);
       if (!mbar_wait(bar.v_empty(vr.st), vr.ph ^ 1, p.status)) return;
-      tc_load<D_, true>(p, tv, v_s + vr.st * C::TILE, bar.v_full(vr.st), cur, key, nb, w.kvh, pol, lane);
+      tc_load<D_, true>(p, tv, v_s + vr.st * C::TILE, bar.v_full(vr.st), cur, key, nb, w.kvh, pol, lane, poison, seq);
       vr.next(C::VST);
       if (j + 1 < w.nkt) cur = tc_block(p, w, btrow, j + 1, lane, key);
     }
@@ -475,8 +481,8 @@ __device__ void tc_mma(const MaskedParams& p, int TT, const TcBars& bar, uint32_
 }
 
 // One row's attention over the item's keys in plain float32, one key at a
-// time (an item whose values are not finite where some of its rows see them,
-// a row without a sum of weights).
+// time (an item whose values are not finite where some of its rows see them or
+// whose blocks are not all there, a row without a sum of weights).
 template <typename T, int D_>
 __device__ __noinline__ void tc_row_again(const MaskedParams& p, const MaskedGroup g, int k0, int k1, int part, int kvh,
                                           int tok, int hd) {
@@ -882,7 +888,7 @@ __global__ void __launch_bounds__(TcCfg<D_>::THREADS, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_CTRL));
     if (warp == 0)
-      tc_producer<T, D_>(p, TT, q_tma, &tq, &tk, &tv, bar, q_s, k_s, v_s, tasks, ring);
+      tc_producer<T, D_>(p, TT, q_tma, &tq, &tk, &tv, bar, base, q_s, k_s, v_s, tasks, ring);
     else if (warp == 1)
       tc_mma<D_>(p, TT, bar, tmem, q_s, k_s, v_s, std::is_same<T, __nv_bfloat16>::value, ring);
     else

@@ -452,6 +452,42 @@ def test_bad_records_are_flagged_not_followed():
         st.cache.check_status()
 
 
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+def test_keys_of_missing_blocks_are_left_out(shape, split, monkeypatch):
+    """Block ids out of range: flagged, and their keys take no part, whatever the other blocks hold."""
+    from nifre_b200 import _lib
+    hq, hkv, d, bs, dtype = shape
+    if split:
+        _split(monkeypatch, item_keys=256)
+    ctx, n = [40, 200, 400, 300, 150, 500], [1, 3, 12, 40, 100, 130]
+    st = Step(ctx, n, hq, hkv, d, bs, dtype, seed=25, pad=1)
+    gone = {0: [0], 1: [2], 2: [1, 4], 3: [3], 4: [0, (150 + 20) // bs]}  # logical blocks; sequence 5 has all of its own
+    for s, blocks in gone.items():
+        for b in blocks:
+            st.cache.bt_dev[s, b] = 1 << 20 if b % 2 else -1
+    gone[5] = []
+    lost = lambda s: [t for b in gone[s] for t in range(b * bs, min((b + 1) * bs, ctx[s] + n[s]))]  # noqa: E731
+    masks = [np.eye(m, dtype=bool) for m in n]
+
+    def check(out, seen_of):
+        with pytest.raises(_lib.NifreError, match="bad block=1"):
+            st.cache.check_status()
+        for s, m in enumerate(n):
+            seen = seen_of(s).clone()
+            seen[:, lost(s)] = False
+            rows = slice(st.start[s], st.start[s] + m)
+            ref, wabs, most = attend(st.q[0][rows].view(m, hq, d), st.k[s][0], st.v[s][0], seen, d ** -0.5)
+            tol = tolerance(ref, wabs, most, ctx[s] + m, d, dtype)
+            err = (out[rows].view(m, hq, d).double() - ref).abs()[seen.any(1)]
+            assert (err <= tol[seen.any(1)]).all(), (s, float(err.max()))
+
+    check(_tree_out(st, masks, hq), lambda s: tree_seen(ctx[s], torch.as_tensor(masks[s])))
+    view = st.cache.plan_window(st.plan, 170, 70, q_heads=hq)
+    out = st.cache.window_attention_step(0, st.q[0], view, torch.full_like(st.q[0], 7))
+    check(out, lambda s: window_seen(ctx[s], n[s], 170, 70))
+
+
 @pytest.mark.parametrize("field,value", [(4, 99), (5, 139), (6, -1), (6, 1000), (0, 8), (0, 4096)])
 def test_bad_tensor_core_items_are_flagged_not_followed(field, value):
     from nifre_b200 import _lib
