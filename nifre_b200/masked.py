@@ -338,6 +338,10 @@ class MaskedAttentionOps:
             raise ValueError(f"q_heads must be a positive multiple of the cache's {self.n_heads} heads, got {q_heads}")
         if int(plan.slots.max()) >= self.batch_size:
             raise IndexError(f"cache slot out of range [0, {self.batch_size})")
+        if plan.generation != self._generation:
+            raise ValueError("the step's plan is another cache's, or was made before the cache's last init_batch")
+        if (self.pos_host[plan.slots] != plan.ctx_before + (plan.q_lens if plan.closed else 0)).any():
+            raise ValueError("a slot's length has changed since the step was planned")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("plans are made outside a CUDA graph capture (and refilled with into=)")
         unit_rows, item_rows = self.masked_limits(q_heads)

@@ -30,6 +30,7 @@ advances only when the last layer of a step has appended
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
 
 import numpy as np
@@ -95,6 +96,9 @@ def _prefill_order(tiles, kv_heads: int) -> np.ndarray:
     return items[np.argsort(-costs[items // kv_heads], kind="stable")].astype(np.int32)
 
 
+_GENERATIONS = itertools.count(1)
+
+
 class StepPlan:
     """Device metadata of one forward pass over a ragged batch.
 
@@ -132,6 +136,7 @@ class StepPlan:
         # per-plan constant arguments of the layers' C ABI calls, built on first use
         self.append_args = self.decode_args = None
         self.holes = False  # some sequence's blocks were freed behind its window
+        self.generation = None  # of the cache's pools when the plan was made
         self.views = {}  # the step's plans of windows, made by Attention: (window, sinks, query heads) -> MaskedPlan
 
     @property
@@ -170,7 +175,7 @@ class PagedKVCache(MaskedAttentionOps, PageOps):
         self.prefix_cache: PrefixCache | None = None
         self._plan: StepPlan | None = None
         self.steps_closed = 0  # forward passes whose last layer has appended
-        self._generation = 0  # of the pools: plans of windows and trees are for one
+        self._generation = next(_GENERATIONS)  # of the pools, no other cache's: plans of windows and trees are for one
         # KV heads sharded over several GPUs: a sharding.PeerExchange whose gathered buffers receive every
         # rank's attention output (Attention.forward then returns the gathered rows); None on one GPU
         self.exchange = None
@@ -181,7 +186,7 @@ class PagedKVCache(MaskedAttentionOps, PageOps):
         if self.device.type != "cuda":
             raise _lib.NifreError("PagedKVCache needs a CUDA device: nifre_b200 has no CPU path")
         self.batch_size = batch_size
-        self._generation += 1
+        self._generation = next(_GENERATIONS)
         self.pos = torch.zeros(batch_size, dtype=torch.long, device=self.device)
         self.pos_host = np.zeros(batch_size, dtype=np.int64)
         self.max_blocks_per_seq = (self.max_seq_len + self.block_size - 1) // self.block_size
@@ -233,7 +238,7 @@ class PagedKVCache(MaskedAttentionOps, PageOps):
         self.prefix_cache = None
         self._plan = None
         self._k_all = self._v_all = None
-        self._generation += 1  # plans made before are not of the next batch
+        self._generation = next(_GENERATIONS)  # plans made before are not of the next batch
 
     # ------------------------------------------------------------------ reference API
     def try_load_prefix(self, batch_idx: int, token_ids: list[int]) -> int:
@@ -590,6 +595,7 @@ class PagedKVCache(MaskedAttentionOps, PageOps):
 
         plan = StepPlan(slots, q_lens, q_starts, ctx, split, max_units, seq_split)
         plan.upload_bytes = host.nbytes
+        plan.generation = self._generation
         # what a captured graph of the per-layer kernels depends on besides the cache's own buffers
         plan.layout_key = (meta.data_ptr(), off_ct, off_tok, off_slot, off_units, off_counts, max_units, S, T,
                            n_ct, n_tok, n_tiles, q_heads)

@@ -429,6 +429,29 @@ def test_plans_of_an_earlier_batch_are_refused():
         st.cache.plan_window(st.cache.plan([0], [2], [0]), 4, q_heads=4, into=view)
 
 
+def test_step_plans_of_an_earlier_batch_or_length_are_refused():
+    st = Step([10, 20], [2, 1], 4, 2, 64, 16, HF, seed=26)
+    c = st.cache
+    c.truncate(1, 20)
+    with pytest.raises(ValueError, match="changed"):
+        c.plan_window(st.plan, 4, q_heads=4)
+    plan = c.plan([0, 1], [2, 1], [0, 2], q_heads=4)
+    c.plan_window(plan, 4)  # of an open step
+    kv = torch.zeros(3, 128, dtype=HF, device=DEV)
+    c.append_step(0, kv, kv, plan)
+    view = c.plan_tree(plan, [[-1, 0], None])  # and of a closed one
+    c.keep_tokens(plan, [[1], []])
+    with pytest.raises(ValueError, match="changed"):
+        c.plan_tree(plan, [[-1, 0], None], into=view)
+    other = Step([10, 20], [2, 1], 4, 2, 64, 16, HF, seed=26)
+    with pytest.raises(ValueError, match="another cache's"):
+        c.plan_window(other.plan, 4, q_heads=4)
+    other.cache.init_batch(2)
+    other.cache.pos_host[:] = [12, 21]
+    with pytest.raises(ValueError, match="init_batch"):
+        other.cache.plan_window(other.plan, 4, q_heads=4)
+
+
 def test_bad_records_are_flagged_not_followed():
     """Work lists and block tables with values out of range: skipped and flagged by the kernels' own checks."""
     from nifre_b200 import _lib

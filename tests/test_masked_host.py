@@ -437,12 +437,12 @@ def test_a_refill_on_another_stream_is_ordered_and_kept(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: t)
     c = _host_cache()
-    c._sm_count, c._generation, c._stream = 148, 1, lambda: now.name
+    c._sm_count, c._stream = 148, lambda: now.name
     c.pos_host[:] = [20, 0, 0, 0]
-    plan = SimpleNamespace(slots=np.asarray([0]), q_lens=np.asarray([2]), q_starts=np.asarray([0]), owner=c, generation=1,
+    plan = SimpleNamespace(slots=np.asarray([0]), q_lens=np.asarray([2]), q_starts=np.asarray([0]), generation=c._generation,
                            ctx_before=np.asarray([18]), n_seqs=1, q_heads=4, rows_needed=2, closed=True)
     view = MaskedPlan("window", 8, 0, 4, 2)
-    view.owner, view.generation, view.room, view.streams = c, 1, (64,) * 5 + (8, 4), {"A"}
+    view.owner, view.generation, view.room, view.streams = c, c._generation, (64,) * 5 + (8, 4), {"A"}
     view.buf = SimpleNamespace(device="cuda", copy_=lambda *a, **k: log.append("copy"),
                                record_stream=lambda s: log.append("buf kept for " + s.name))
     view.ws = SimpleNamespace(numel=lambda: 8, record_stream=lambda s: log.append("ws kept for " + s.name))
@@ -453,3 +453,21 @@ def test_a_refill_on_another_stream_is_ordered_and_kept(monkeypatch):
     del log[:]
     c.plan_window(plan, 8, q_heads=4, into=view)  # again on the same stream
     assert log == ["copy", "upload on B"]
+
+
+def test_plans_of_another_batch_or_of_changed_slots_are_refused():
+    from types import SimpleNamespace
+    a, b = _host_cache(), _host_cache()
+    assert a._generation != b._generation
+    a.pos_host[:2] = [12, 9]
+    plan = SimpleNamespace(slots=np.asarray([0, 1]), q_lens=np.asarray([2, 3]), q_starts=np.asarray([0, 2]), closed=True,
+                           ctx_before=np.asarray([10, 6]), n_seqs=2, q_heads=4, rows_needed=5, generation=b._generation)
+    for call in (lambda: a.plan_window(plan, 8), lambda: a.plan_tree(plan, [None, None])):
+        plan.generation = b._generation
+        with pytest.raises(ValueError, match="another cache's"):
+            call()
+        plan.generation = a._generation
+        for closed, pos in ((True, [11, 9]), (True, [12, 0]), (False, [12, 9])):
+            plan.closed, a.pos_host[:2] = closed, pos
+            with pytest.raises(ValueError, match="changed"):
+                call()
