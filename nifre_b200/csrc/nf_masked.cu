@@ -357,13 +357,13 @@ __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const
       }
       const int v = v0 + lane, key = vk.key(v);
       const bool there = v < v1 && (missing[v0 >> 5 & 1] != v0 || key_row(p, btrow, key) >= 0);
-      bool all = true;
+      unsigned unseen = 0;  // columns that do not see the key
       float4 w;
       float* wp = reinterpret_cast<float*>(&w);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const bool seen = there && sees(p, g, tok[c], key);
-        all = all && seen;
+        if (!seen) unseen |= 1u << c;
         float top = seen ? s[c] : -INFINITY;
         const float x = top;
 #pragma unroll
@@ -375,10 +375,14 @@ __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const
 #pragma unroll
         for (int i = 0; i < ND; ++i) o[c][i] *= al;
       }
+      // -0 for a key that is not seen: a seen one's weight may have underflowed to 0
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (unseen >> c & 1u) wp[c] = -0.f;
       ps[warp * 32 + lane] = w;
       __syncwarp();
       const float* vf = reinterpret_cast<const float*>(vs) + lane;
-      if (__all_sync(0xffffffffu, all)) {
+      if (__all_sync(0xffffffffu, unseen == 0)) {
 #pragma unroll 4
         for (int k = 0; k < 32; ++k) {
           const float4 x = ps[warp * 32 + k];
@@ -392,15 +396,16 @@ __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const
           }
         }
       } else {  // keys that a column does not see are left out, whatever their value rows hold
+        constexpr unsigned kUnseen = 0x80000000u;
         for (int k = 0; k < 32; ++k) {
           const float4 x = ps[warp * 32 + k];
 #pragma unroll
           for (int i = 0; i < ND; ++i) {
             const float y = 32 * i + lane < p.D ? vf[k * D4 * 4 + 32 * i] : 0.f;
-            if (x.x != 0.f) o[0][i] = fmaf(x.x, y, o[0][i]);
-            if (x.y != 0.f) o[1][i] = fmaf(x.y, y, o[1][i]);
-            if (x.z != 0.f) o[2][i] = fmaf(x.z, y, o[2][i]);
-            if (x.w != 0.f) o[3][i] = fmaf(x.w, y, o[3][i]);
+            if (__float_as_uint(x.x) != kUnseen) o[0][i] = fmaf(x.x, y, o[0][i]);
+            if (__float_as_uint(x.y) != kUnseen) o[1][i] = fmaf(x.y, y, o[1][i]);
+            if (__float_as_uint(x.z) != kUnseen) o[2][i] = fmaf(x.z, y, o[2][i]);
+            if (__float_as_uint(x.w) != kUnseen) o[3][i] = fmaf(x.w, y, o[3][i]);
           }
         }
       }

@@ -381,6 +381,14 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
         for (int j = 0; j < NT; ++j) mt_mma<T>(st.o[i][j], f, pb[j][0], pb[j][1]);
       }
     } else {
+      constexpr unsigned kUnseen = 0x80000000u;  // -0: a seen key's weight may have underflowed to 0
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = tq + (e >> 1) * 8, tok = e & 1 ? st.tok[j] >> 16 : st.tok[j] & 0xffff;
+          if (row >= nv[t] || !sees(p, g, tok, key0[t] + row)) x[t][j][e] = -0.f;
+        }
       for (int row = 0; row < 16; ++row) {
         const int src = (row & 7) * 4 + (lane & 3);
 #pragma unroll
@@ -396,8 +404,8 @@ __device__ __forceinline__ void mt_update(const MaskedParams& p, const MaskedGro
               unsigned short b;
               asm volatile("ld.shared.u16 %0, [%1];" : "=h"(b) : "r"(vb[t] + mt_off(row, d >> 3) + (d & 7) * 2));
               const float v = Elem<T>::to_f(*reinterpret_cast<T*>(&b));
-              if (w0 != 0.f) st.o[i][j][2 * h] = fmaf(w0, v, st.o[i][j][2 * h]);
-              if (w1 != 0.f) st.o[i][j][2 * h + 1] = fmaf(w1, v, st.o[i][j][2 * h + 1]);
+              if (__float_as_uint(w0) != kUnseen) st.o[i][j][2 * h] = fmaf(w0, v, st.o[i][j][2 * h]);
+              if (__float_as_uint(w1) != kUnseen) st.o[i][j][2 * h + 1] = fmaf(w1, v, st.o[i][j][2 * h + 1]);
             }
         }
       }

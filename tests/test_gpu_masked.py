@@ -329,6 +329,30 @@ def test_scores_of_minus_infinity(shape, split, monkeypatch):
     st.cache.check_status()
 
 
+@pytest.mark.parametrize("split", [False, True])
+@pytest.mark.parametrize("shape", SHAPES, ids=IDS)
+def test_values_of_seen_keys_with_weights_near_zero(shape, split, monkeypatch):
+    """A value that is not finite reaches every row that sees its key, also where the key's weight underflows to 0 and
+    other rows of its tile do not see it (as 0 * NaN does in the definition's arithmetic)."""
+    hq, hkv, d, bs, dtype = shape
+    if split:
+        _split(monkeypatch)
+    ctx, n = [16, 40, 100], [5, 30, 150]
+    st = Step(ctx, n, hq, hkv, d, bs, dtype, seed=27, pad=1)
+    st.q.view(1, st.rows, hq, d)[..., 0] = 100
+    masks = [np.tril(np.ones((m, m), dtype=bool)) for m in n]
+    for s in range(3):
+        block, off = st.cache.block_tables[s].resolve(ctx[s] + 2)
+        st.cache.k[0][block, off, :, 0] = -3e4  # scores of -3e6 / sqrt(d)
+        st.cache.v[0][block, off] = float("nan")
+    out = _tree_out(st, masks, hq)
+    for s, m in enumerate(n):
+        for i in range(m):
+            row = out[st.start[s] + i]
+            assert (torch.isnan(row) if i >= 2 else torch.isfinite(row)).all(), (s, i)
+    st.cache.check_status()
+
+
 def test_large_scores_and_long_window():
     """Scores far from 0 (one key takes all the weight) and a running maximum that moves late."""
     st = Step([3000], [4], 8, 2, 64, 16, BF, seed=9)
