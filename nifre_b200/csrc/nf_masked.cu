@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kVecWarps * 32, C == 1 ? 3 : 2) masked_vec_ker
     const int kvh = rest / chunks, c0 = (rest - kvh * chunks) * C;
     MaskedGroup g;
     const int4 un = load_record(p.units, u, g);
-    if (!group_ok(p, g)) {
+    if (!unit_ok(p, un, g)) {
       if (threadIdx.x == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
       continue;
     }
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const
     const int kvh = rest / blocks, c0 = (rest - kvh * blocks) * 32;
     MaskedGroup g;
     const int4 un = load_record(p.units, u, g);
-    if (!group_ok(p, g)) {
+    if (!unit_ok(p, un, g)) {
       if (threadIdx.x == 0) atomicOr(p.status, NF_STATUS_BAD_SLOT);
       continue;
     }

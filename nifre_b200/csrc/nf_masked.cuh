@@ -80,6 +80,11 @@ __device__ __forceinline__ bool group_ok(const MaskedParams& p, const MaskedGrou
   return g.n_draft > 0 && g.mask0 >= 0 && g.mask0 + g.ntok * words <= p.mask_words;
 }
 
+// And a unit's: its first key, and no more tokens than the launch was sized for.
+__device__ __forceinline__ bool unit_ok(const MaskedParams& p, const int4& un, const MaskedGroup& g) {
+  return group_ok(p, g) && un.x >= 0 && (un.x & 15) == 0 && g.ntok <= p.unit_tokens;
+}
+
 // Virtual keys of a group: 16-key blocks wholly before the first token's
 // window and past the sinks are left out.  Virtual key v is key v for
 // v < kept, else v + gap; `end` virtual keys in all.
@@ -115,7 +120,7 @@ __device__ __forceinline__ bool sees(const MaskedParams& p, const MaskedGroup& g
 // Pool row of key k of a slot (-1: no such block; flagged).
 __device__ __forceinline__ long long key_row(const MaskedParams& p, const int* btrow, int k) {
   const int lb = k / p.bs;
-  const int phys = lb < p.max_blocks ? __ldg(btrow + lb) : -1;
+  const int phys = (unsigned)lb < (unsigned)p.max_blocks ? __ldg(btrow + lb) : -1;
   if (phys < 0 || phys >= p.num_blocks) {
     atomicOr(p.status, NF_STATUS_BAD_BLOCK);
     return -1;

@@ -243,7 +243,7 @@ __device__ __forceinline__ int tc_block(const MaskedParams& p, const TcItem& w, 
   key = w.key(v);
   const int lb = key / p.bs;
   if (lane >= 8 || v >= w.k1) return 0;
-  return lb < p.max_blocks ? __ldg(btrow + lb) : -1;
+  return (unsigned)lb < (unsigned)p.max_blocks ? __ldg(btrow + lb) : -1;
 }
 
 // Copies of one 128-key K or V tile, lane b < nb the 16-key block b.  A block

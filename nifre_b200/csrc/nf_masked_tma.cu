@@ -107,7 +107,7 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
   while (w < total) {
     const int hg = w % L.n_hg, h0 = hg * L.HG;
     const bool more = u + 1 < sh.y;  // the next unit is this share's
-    if (u >= sh.y || !group_ok(p, g)) {
+    if (u >= sh.y || !unit_ok(p, un, g)) {
       if (u < sh.y) atomicOr(p.status, NF_STATUS_BAD_SLOT);
       if (more) {
         ++u;
@@ -152,7 +152,7 @@ __device__ void mt_producer(const MaskedParams& p, const MtLaunch& L, const CUte
       }
       const int key0 = vk.key(v), key1 = key0 + 15, last_pos = g.pos0 + g.ntok - 1;
       const int lb = key0 / p.bs;
-      int phys = lb < p.max_blocks ? __ldg(btrow + lb) : -1;
+      int phys = (unsigned)lb < (unsigned)p.max_blocks ? __ldg(btrow + lb) : -1;
       // a block that is not there: nothing of it is seen (nv 0 on a masked step), and block 0 stands in
       const bool bad = phys < 0 || phys >= p.num_blocks;
       if (bad) {

@@ -499,6 +499,29 @@ def test_bad_records_are_flagged_not_followed():
         st.cache.check_status()
 
 
+@pytest.mark.parametrize("dtype,n", [(F32, 1), (F32, 4), (BF, 1), (BF, 7)])
+@pytest.mark.parametrize("field,value", [(0, -16), (0, -(1 << 31)), (0, 8), (6, 40)])
+def test_bad_units_are_flagged_not_followed(dtype, n, field, value):
+    """A first key below 0 or inside a group of 16, more tokens than the launch is sized for."""
+    from nifre_b200 import _lib
+    from nifre_b200.masked import WorkLists
+    st = Step([40, 40], [n, n], 4, 1, 64, 16, dtype, seed=28, room=64)
+    view = st.cache.plan_window(st.plan, 30, 0, q_heads=4)
+    at, _ = WorkLists.offsets(view.room)
+    wide = torch.zeros(80, 256, dtype=dtype, device=DEV)  # rows enough for the larger group
+    wide[:2 * n] = st.q[0]
+    row, rows = view.buf[at[0] + 5:at[0] + 7].tolist()  # of the first unit's group
+    view.buf[at[0] + field] = value
+    out = torch.full((80, 256), 7, dtype=dtype, device=DEV)
+    st.cache.window_attention_step(0, wide, view, out)
+    with pytest.raises(_lib.NifreError, match="bad slot=1"):
+        st.cache.check_status()
+    left = torch.ones(80, dtype=torch.bool)
+    left[:2 * n] = False
+    left[row:row + rows] = True
+    assert torch.equal((out == 7).all(1).cpu(), left)
+
+
 @pytest.mark.parametrize("split", [False, True])
 @pytest.mark.parametrize("shape", SHAPES, ids=IDS)
 def test_keys_of_missing_blocks_are_left_out(shape, split, monkeypatch):
