@@ -146,7 +146,7 @@ class PageOps:
             elif have != want:
                 changed.append((s, d))
         if changed:
-            self._refork(changed, held)
+            self._refork(changed, held, dst)
         self.pos_host[dst] = [held[s][0] for s in src]
         if self._hole_end.any():
             self._hole_first[dst], self._hole_end[dst] = self._hole_first[src], self._hole_end[src]
@@ -158,17 +158,23 @@ class PageOps:
             pos += (d, n)
         self._move_rows(moves, pos, bs)
 
-    def _refork(self, pairs, held) -> None:
-        """Give the destination slots of the pairs their sources' full blocks and a last block of their own."""
+    def _refork(self, pairs, held, dst) -> None:
+        """Give the destination slots of the pairs their sources' full blocks and a last block of their own.
+        ``dst``: all of the call's destinations, which an exhausted pool leaves empty."""
         tables, alloc = self.block_tables, self.block_allocator
-        for _, d in reversed(pairs):  # the last released block is the next one allocated
-            tables[d].clear()
-            self.pos_host[d] = 0
-            self._clear_hole(d)
-        need = sum(held[s][2] > 0 for s, _ in pairs)
-        if need > alloc.free_count:
-            self._move_rows([], [x for _, d in pairs for x in (d, 0)], 0)
-            raise BlockPoolExhaustedError(f"need {need} blocks, only {alloc.free_count} free")
+
+        def empty(slots):
+            for d in reversed(slots):  # the last released block is the next one allocated
+                tables[d].clear()
+                self.pos_host[d] = 0
+                self._clear_hole(d)
+
+        empty([d for _, d in pairs])
+        need, free = sum(held[s][2] > 0 for s, _ in pairs), alloc.free_count
+        if need > free:
+            empty(dst)
+            self._move_rows([], [x for d in dst for x in (d, 0)], 0)
+            raise BlockPoolExhaustedError(f"need {need} blocks, only {free} free")
         for s, d in pairs:
             tables[d].share(held[s][3])
             if held[s][2]:

@@ -471,3 +471,21 @@ def test_plans_of_another_batch_or_of_changed_slots_are_refused():
             plan.closed, a.pos_host[:2] = closed, pos
             with pytest.raises(ValueError, match="changed"):
                 call()
+
+
+def test_a_fork_that_the_pool_cannot_hold_leaves_every_destination_empty():
+    """Also those that an earlier fork had given the right blocks."""
+    from nifre_b200 import BlockPoolExhaustedError
+    c = _host_cache(num_blocks=5)
+    c.block_tables[0].ensure_capacity(40)
+    c.pos_host[0] = 40
+    c.fork([0], [1])
+    assert c.length(1) == 40 and c.block_allocator.free_count == 1
+    c.block_tables[3].ensure_capacity(16)
+    c.pos_host[3] = 16
+    with pytest.raises(BlockPoolExhaustedError, match="need 1 blocks, only 0 free"):
+        c.fork([0, 0], [1, 2])
+    assert [c.length(s) for s in range(4)] == [40, 0, 0, 16]
+    assert len(c.block_tables[1]) == len(c.block_tables[2]) == 0
+    assert c.moved[-1][:2] == ([], [1, 0, 2, 0])
+    assert c.block_allocator.free_count == 1  # slot 1's own last block
