@@ -410,7 +410,9 @@ int nf_cascade_limits(int32_t dtype, int32_t num_q_heads, int32_t num_kv_heads, 
  *   window:  k <= p and (k > p - window or k < sinks),
  *   tree:    k < ctx, or bit k - ctx of the token's mask row is set,
  * and its output is sum_k softmax_k(q . k * scale) v_k over the keys it sees,
- * 0 when it sees none.  A key that a token does not see contributes nothing
+ * 0 when it sees none (scale finite; a seen score or value that is NaN reaches
+ * the output, and seen scores that are all -inf give NaN).  A key that a token
+ * does not see contributes nothing
  * to it, whatever its rows hold (NaN and infinities included).  Query head j
  * reads KV head j / (num_q_heads / num_kv_heads); every dtype, head_dim up to
  * 256, any block size and group size.

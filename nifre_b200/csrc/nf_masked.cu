@@ -41,9 +41,9 @@ template <typename H> struct VecLoad<H, 1> {
 // key and value bytes (column chunks of a group read them again, from L2) and,
 // for short key ranges, by the latency of the dependent loads: eight warps on
 // a unit make that two or three steps, and one unit a sequence needs no merge
-// (8 float32 decodes of 12 heads over 130 keys: 7.2 us; 41 with a warp a unit
+// (8 float32 decodes of 12 heads over 130 keys: 7.6 us; 41 with a warp a unit
 // of 64 keys and a merge.  64 float32 decodes with full contexts, 0.9 GB:
-// 162 us, 86 % of the copy bandwidth.)
+// 164 us, 86 % of the copy bandwidth.)
 template <typename T, int VW, int LPK, int EV, int C>
 __global__ void __launch_bounds__(kVecWarps * 32, C == 1 ? 3 : 2) masked_vec_kernel(const MaskedParams p) {
   constexpr int KPW = 32 / LPK;  // keys per step of the warp
@@ -232,10 +232,10 @@ __global__ void __launch_bounds__(kVecWarps * 32, C == 1 ? 3 : 2) masked_vec_ker
 // lanes; rows padded so that the eight lanes of a 16-byte read hit distinct
 // banks), value sums with an element a lane.  Bound by instructions (about
 // 1,150 a warp and tile for 512 FMAs at head_dim 64): 8 float32 chunks of 200
-// tokens, 12 heads and a window of 256 keys 127 us, with four columns a CTA 294;
-// 25 trees of 16 tokens on up to 4,000 keys, 12 heads, 446 us.
+// tokens, 12 heads and a window of 256 keys 129 us, with four columns a CTA 294;
+// 25 trees of 16 tokens on 500 to 4,000 keys, 12 heads, 308 us, on 4,000 515.
 // D <= 32 ND; two CTAs an SM up to 128 (in 128 registers: 6 trees of 20 tokens on
-// up to 2,000 keys, 8 float32 heads of 128, 94 us, 125 with one CTA).
+// 500 to 2,000 keys, 8 float32 heads of 128, 77 to 82 us; one CTA took a third more).
 template <typename T, int ND, bool VEC>
 __global__ void __launch_bounds__(256, ND <= 4 ? 2 : 1) masked_tile_kernel(const MaskedParams p) {
   constexpr int VW = sizeof(T) == 4 ? 4 : 8;

@@ -26,18 +26,27 @@
 // still reach the sum, the value warps look over a masked tile's value rows
 // before P V reads them: rows that are not finite are zeroed, and where some row of the
 // item does see one of them, the item's rows are computed again one by one
-// (slow, and right: such values are rare and wrong already).
+// (slow, and right: such values are rare and wrong already).  So they are where
+// a block of the item is not there.  Scores that are NaN, or all -inf: see sees_any.
 //
-// What bounds it, measured with copies of the kernel that leave work out: for
-// heads of 64 the exponentials (4 chunks of 512 tokens, windows of 1,024, 32
-// heads: 46 us; 37 without them): a pair of tiles takes 3,100 cycles, 2,048 of them on
-// the special-function unit and 1,024 in products.  For heads of 128 (a chunk
-// of 2,048 tokens, window 4,096, 32 heads: 139 us, 980 TFLOP/s; longer when it
-// runs without a pause and the clock falls) first the copies of 16-key blocks (128 us
-// with an eighth of them; 144 before a value block was one copy instead of two), then
-// the chain S, weights, P V of a half.  Both run 256 items on 148 SMs, two turns
-// where 1.73 would do; parts to even that out would cost as much in merging.
-// 16 trees of 32 tokens on contexts up to 4,096, 32 heads of 64: 43 us, where the
+// Scores, maxima, sums of weights, accumulators and partial results are float32.
+// The weights alone are rounded, once, to the pools' type for P V (both
+// operands have one 16-bit type): each is off by half a step at most, 2^-8 of it
+// in bf16 and 2^-11 in fp16, and the sum of weights is taken before.
+//
+// What is known of its bounds, from copies of the kernel that leave work out.
+// Heads of 64 (4 chunks of 512 tokens, windows of 1,024, 32 heads): 46 us, 37
+// without the exponentials, which are thus 9 of them.  A pair of tiles takes
+// 3,100 cycles (2,048 on the special-function unit, 1,024 in products), about 29
+// us for the two items of nine pairs an SM has; the rest is outside that loop:
+// the start and the epilogue of the items, which nothing hides, edge tiles
+// under the mask, and the second turn of 256 items on 148 SMs.  Heads
+// of 128 (a chunk of 2,048 tokens, window 4,096, 32 heads): 160 us in calls one
+// after another (860 TFLOP/s), 140 in replays short enough for the clock to
+// stay up; first the copies of 16-key blocks (139 -> 128 us with an eighth of
+// them; 144 before a value block was one copy instead of two), then the chain S,
+// weights, P V of a half.  Parts to even the two turns out cost as much in merging.
+// 16 trees of 32 tokens on contexts up to 4,096, 32 heads of 64: 44 us, where the
 // copies and the transitions between items weigh most.  Taken and dropped: two
 // threads a row (the exchange of their maxima costs 450 cycles a tile), the next
 // scores loaded before the weights are stored, S in two products of 64 keys.

@@ -10,20 +10,28 @@
 // and no others.  Consumer warp h computes KV head h for all of the group's
 // columns (token x query head) at once: S^T = K Q^T and O^T += V^T P^T with
 // mma.sync m16n8k16, the columns as NT tiles of 8, so K and V are read once
-// whatever the number of drafted tokens.  (tcgen05 needs 64 rows or more; a
-// group has at most 32, larger ones go to nf_masked_tc.cu.)
+// whatever the number of drafted tokens.  (A group has at most 32 query rows;
+// tcgen05 with the queries as its rows wants 64 or more, and larger groups go to
+// nf_masked_tc.cu.  Keys as the 128 rows and the queries as up to 32 columns
+// would fit tcgen05 too; that form has not been built.)
 //
 // 64 decodes with a window of 4,096 and 64 sinks, 8 KV heads of 128 (1.09 GB):
-// 167-170 us with the merge, the copy bandwidth.  64 with a window of 1,024, 8
-// KV heads of 64 (130 MB): 29 us, of which 20 are the bytes and the rest is
+// 170 us with the merge, the copy bandwidth.  64 with a window of 1,024, 8
+// KV heads of 64 (130 MB): 30 us, of which 20 are the bytes and the rest is
 // the ramp of 148 CTAs and the merge's launch.  37 trees of 7 tokens (28 columns)
-// on 4,096 keys: 82 us with two warps a head on alternate steps, 97 and 115
-// with one warp (its registers hold four column tiles then).
+// on 4,096 keys: 72 us with two warps a head of 16 columns each.
+//
+// Scores, maxima, sums of weights and outputs are float32.  The weights alone
+// are rounded, once, to the pools' type for the second product (mma.sync takes
+// both operands in one 16-bit type): each is off by half a step at most, 2^-8 of
+// it in bf16 and 2^-11 in fp16, and the sum of weights is taken before, so an
+// output is off by that much of sum w |v| at most.
 //
 // Only steps that some column does not wholly see apply the mask.  There the
 // weights of unseen keys are 0; as 0 * NaN would still reach the sum, such a
 // step looks its value rows over and, where they hold anything not finite,
-// adds the seen rows one by one instead.
+// adds the seen rows one by one instead.  Scores that are NaN, or all -inf: see
+// sees_any.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -552,11 +560,12 @@ __device__ void mt_consumer(const MaskedParams& p, const MtLaunch& L, unsigned c
 }
 
 // CW: consumer warps a KV head, each with NT tiles of 8 of the group's columns.
-// Measured on 37 trees of 7 tokens over 4096 keys (1B shape, 28 columns, 310
-// MB): one warp a head with all 32 columns 115 us (latency of one update at a
-// time: 10 cycles an instruction with two warps a scheduler), the same with 232
-// registers a thread (setmaxnreg) and two steps an update 97 us, two warps a
-// head with 16 columns each 82 us (96 registers; more steps an update spill).
+// Measured side by side on 37 trees of 7 tokens over 4096 keys (1B shape, 28
+// columns, 310 MB; the build with two warps takes 72 us now): one warp a head
+// with all 32 columns 115 us (latency of one update at a time: 10 cycles an
+// instruction with two warps a scheduler), the same with 232 registers a thread
+// (setmaxnreg) and two steps an update 97 us, two warps a head with 16 columns
+// each 82 us (96 registers; more steps an update spill).
 template <typename T, int D_, int NT, int CW>
 __global__ void __launch_bounds__(32 * ((D_ == 64 ? 8 : 4) * CW + 1), D_ == 64 || CW == 4 ? 1 : 2)
     masked_tma_kernel(const MaskedParams p, const MtLaunch L, const __grid_constant__ CUtensorMap tk,
